@@ -273,6 +273,123 @@ int gdn_prefill_backward_qk4_v8_d128_k_last(
     float *dA_log, float *ddt_bias, float *d_state,
     void *workspace, size_t workspace_bytes, void *stream);
 
+/*
+ * Channelwise gated linear recurrence -- no counterpart in the reference.  The
+ * diagonal sibling of the GDN recurrence: one fp32 state per channel, with the
+ * same gates, one per channel,
+ *   g = exp(-exp(A_log) softplus(a + dt_bias)),  beta = sigmoid(b),
+ *   h <- g h + beta x,  out = h.
+ * type      element type of x, a, b, out and of their gradients: GDN_BF16,
+ *           GDN_FP16 or GDN_FP32; everything is computed and carried in fp32
+ *           and a result is rounded once, when it is stored
+ * x, a, b   [T, D], a token's channels contiguous, `*_stride` elements from one
+ *           token to the next (so they may be parts of one projection's output)
+ * A_log, dt_bias [D] fp32
+ * Pointers need the alignment of their elements; where D and the strides are
+ * multiples of 4 and the pointers aligned to 4 elements the kernels use wide
+ * accesses.  1 <= D <= 2^24, T <= 2^31.
+ */
+#define GDN_BF16 0
+#define GDN_FP16 1
+#define GDN_FP32 2
+
+/*
+ * Prefill of N sequences packed into total_tokens rows.
+ * cu_seqlens  [N+1] int64 on the device as in gdn_prefill_qk4_v8_d128_k_last,
+ *             except that cu_seqlens[N] may be less than total_tokens: the
+ *             rows behind the last sequence are not read, and left as they
+ *             were in `out` or, with `zero_behind`, set to zero.
+ *             Bad values set device status 1 and nothing is written.  NULL:
+ *             N sequences of total_tokens / N tokens each.
+ * state       [N,D] fp32 initial states or NULL (zeros); with `slots`
+ *             ([N] int32 on the device, distinct) a pool [pool_slots,D] of
+ *             which sequence n uses row slots[n] (outside the pool: device
+ *             status 3, nothing is written)
+ * out         [T,D]; final_state [N,D] fp32 (the pool with `slots`), may be
+ *             `state`; an empty sequence's final state is its initial state
+ * carries     NULL, or gdn_recurrence_carry_bytes(T, D) bytes (16-byte
+ *             aligned) that receive the state before every 64th row, which
+ *             the backward takes
+ * packed      NULL, or gdn_recurrence_packed_bytes(T, D) bytes (16-byte
+ *             aligned) that receive x, a, b in 8 bits (the format of
+ *             gdn_checkpoint_pack, groups along a row): [3,T,D] values, then
+ *             [3,T,ceil(D/128)] scales
+ * workspace   gdn_recurrence_workspace_bytes(T, D) bytes, 1024-byte aligned;
+ *             calls that overlap in time need one each
+ * One launch for up to 256 rows, else two.  Results are the same bits on
+ * every run.
+ */
+size_t gdn_recurrence_workspace_bytes(int64_t total_tokens, int64_t channels);
+size_t gdn_recurrence_carry_bytes(int64_t total_tokens, int64_t channels);
+size_t gdn_recurrence_packed_bytes(int64_t total_tokens, int64_t channels);
+int gdn_recurrence_prefill(int type, const void *x, int64_t x_stride, const void *a, int64_t a_stride,
+                           const void *b, int64_t b_stride, const float *A_log, const float *dt_bias,
+                           const float *state, const int32_t *slots, int64_t pool_slots,
+                           const int64_t *cu_seqlens, int64_t num_seqs, int64_t total_tokens,
+                           int64_t channels, int zero_behind, void *out, float *final_state, float *carries,
+                           void *packed, void *workspace, size_t workspace_bytes, void *stream);
+
+/*
+ * Gradients of (out, final_state) of the prefill, given d_out ([T,D] of
+ * `type`, d_out_stride between rows) and d_final_state ([N,D] fp32 or NULL).
+ * dx, da, db  [T,D] of `type`; rows behind the last sequence as in `out`
+ * dA_log, ddt_bias [D] fp32;  d_state [N,D] fp32 or NULL (not computed)
+ * carries     what the forward saved, or NULL: the call then runs the
+ *             recurrence once more to find them
+ * packed      NULL, or what the forward wrote: x, a, b (may then be NULL) are
+ *             read from there, and the gradients are those at the 8-bit
+ *             values, the states before the tokens restarted from `carries`
+ *             (required) at every 64th row
+ * workspace   gdn_recurrence_backward_workspace_bytes(T, D) bytes
+ * Deterministic.  No host synchronisation.
+ */
+size_t gdn_recurrence_backward_workspace_bytes(int64_t total_tokens, int64_t channels);
+int gdn_recurrence_backward(int type, const void *x, int64_t x_stride, const void *a, int64_t a_stride,
+                            const void *b, int64_t b_stride, const void *packed, const float *A_log,
+                            const float *dt_bias, const float *state, const int64_t *cu_seqlens,
+                            int64_t num_seqs, int64_t total_tokens, int64_t channels, int zero_behind,
+                            const void *d_out, int64_t d_out_stride, const float *d_final_state, const float *carries, void *dx,
+                            void *da, void *db, float *dA_log, float *ddt_bias, float *d_state,
+                            void *workspace, size_t workspace_bytes, void *stream);
+
+/*
+ * Decode: num_tokens (1 to GDN_DECODE_MTP_MAX_TOKENS) tokens per request, in
+ * order.  x, a, b [B * num_tokens, D] with row strides; state [B,D] fp32, NULL
+ * for zeros, or with `slots` a pool as above (a request whose slot is outside
+ * the pool is skipped, device status 3); new_state may be `state`;
+ * intermediate_states NULL or [B,num_tokens,D] fp32, the state after each token.
+ */
+int gdn_recurrence_decode(int type, const void *x, int64_t x_stride, const void *a, int64_t a_stride,
+                          const void *b, int64_t b_stride, const float *A_log, const float *dt_bias,
+                          const float *state, const int32_t *slots, int64_t pool_slots, int64_t batch,
+                          int64_t num_tokens, int64_t channels, void *out, float *new_state,
+                          float *intermediate_states, void *stream);
+
+/*
+ * Activation checkpoints in 8 bits -- no counterpart in the reference.  A row's
+ * values in groups of 128 (the last group may be shorter) share one power of
+ * two 2^(E-127), E in one byte: the smallest with max|v| <= 127 2^(E-127), at
+ * least 1 and at most 248 (136 for fp16), beyond which values are limited to
+ * 127 2^(E-127).  A value is int8 rint(v / 2^(E-127)), ties to even; the error
+ * is at most half a unit, and unpacking is exact in bf16 and fp32 (in fp16
+ * down to its smallest subnormal).  A group that holds a NaN or an infinity
+ * gets E = 255 and unpacks to NaN.
+ * Each call handles up to GDN_CHECKPOINT_MAX_TENSORS tensors of one type in
+ * one launch.  `data` is read by pack (row r at (r / inner) * outer_stride +
+ * (r % inner) * inner_stride elements, its cols contiguous) and written by
+ * unpack (contiguous [rows, cols]; inner and strides unused but inner >= 1).
+ */
+#define GDN_CHECKPOINT_MAX_TENSORS 4
+typedef struct {
+  void *data;
+  void *values;  /* [rows, cols] int8 */
+  void *scales;  /* [rows, ceil(cols / 128)] uint8 */
+  int64_t rows, cols;
+  int64_t inner, outer_stride, inner_stride;
+} gdn_checkpoint_tensor;
+int gdn_checkpoint_pack(int type, const gdn_checkpoint_tensor *tensors, int count, void *stream);
+int gdn_checkpoint_unpack(int type, const gdn_checkpoint_tensor *tensors, int count, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

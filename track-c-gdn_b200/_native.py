@@ -51,6 +51,23 @@ SIGNATURES = {
          _P, _P, _P, _P, _P, _P, _P, _P, _P, ctypes.c_size_t, _P]),
     "gdn_prefill_qk4_v8_d128_k_last_noalloc": (
         ctypes.c_int, [_P, _P, _P, _P, _P, _P, _P, _P, _P, _I64, _I64, _F, _P, _P, _P]),
+    "gdn_recurrence_workspace_bytes": (ctypes.c_size_t, [_I64, _I64]),
+    "gdn_recurrence_carry_bytes": (ctypes.c_size_t, [_I64, _I64]),
+    "gdn_recurrence_packed_bytes": (ctypes.c_size_t, [_I64, _I64]),
+    "gdn_recurrence_backward_workspace_bytes": (ctypes.c_size_t, [_I64, _I64]),
+    "gdn_recurrence_prefill": (
+        ctypes.c_int,
+        [ctypes.c_int, _P, _I64, _P, _I64, _P, _I64, _P, _P, _P, _P, _I64, _P, _I64, _I64, _I64, ctypes.c_int,
+         _P, _P, _P, _P, _P, ctypes.c_size_t, _P]),
+    "gdn_recurrence_backward": (
+        ctypes.c_int,
+        [ctypes.c_int, _P, _I64, _P, _I64, _P, _I64, _P, _P, _P, _P, _P, _I64, _I64, _I64, ctypes.c_int, _P, _I64,
+         _P, _P, _P, _P, _P, _P, _P, _P, _P, ctypes.c_size_t, _P]),
+    "gdn_recurrence_decode": (
+        ctypes.c_int,
+        [ctypes.c_int, _P, _I64, _P, _I64, _P, _I64, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _P, _P, _P, _P]),
+    "gdn_checkpoint_pack": (ctypes.c_int, [ctypes.c_int, _P, ctypes.c_int, _P]),
+    "gdn_checkpoint_unpack": (ctypes.c_int, [ctypes.c_int, _P, ctypes.c_int, _P]),
 }
 
 ABI_VERSION = 1

@@ -6,4 +6,7 @@
 #include "gdn_prefill_bwd.cu"
 #include "gdn_capi.cu"
 #include "gdn_prefill_noalloc.cu"
+#include "gdn_recurrence.cu"
+#include "gdn_checkpoint.cu"
+#include "gdn_recurrence_capi.cu"
 #include "gdn_debug_probe.cu"  // compiled only with -DGDN_DEBUG_CHECKS

@@ -69,8 +69,8 @@ def library_sources() -> List[Path]:
     pkg = REPO / PACKAGE
     files = sorted((pkg / "csrc").glob("*.cu")) + sorted((pkg / "csrc").glob("*.cuh"))
     files += sorted((REPO / "include").glob("*.h"))
-    files += [pkg / n for n in ("__init__.py", "_native.py", "build.py", "decode.py",
-                                "prefill.py", "shard.py")]
+    files += [pkg / n for n in ("__init__.py", "_native.py", "build.py", "checkpoint.py", "decode.py",
+                                "prefill.py", "recurrence.py", "shard.py")]
     return [f.relative_to(REPO) for f in files]
 
 
