@@ -1,7 +1,7 @@
 // gdn_checkpoint.cu -- activations to int8 groups and back (format in
 // gdn_recurrence.cuh: 128 values of a row share one power of two).
 //
-// A warp takes kRows groups at once, loads them all before it works on the
+// A warp takes kPackRows groups at once, loads them all before it works on the
 // first, finds each group's largest magnitude with one warp reduction on the
 // fp32 bits, and writes a byte per value and a byte per group.  Bound by HBM:
 // 3 bytes a value each way for 2-byte types.
@@ -11,7 +11,7 @@ namespace gdn {
 namespace rec {
 
 constexpr int kPackTensors = 4;  // tensors of one launch
-constexpr int kRows = 4;
+constexpr int kPackRows = 4;
 
 struct PackTensor {
   const void *data;  // pack: the input; unpack: unused
@@ -40,11 +40,11 @@ __device__ __forceinline__ int tensor_of(const Pack &p, int64_t item) {
 template <typename E, bool kVec>
 __global__ void __launch_bounds__(kThreads) checkpoint_pack_kernel(const __grid_constant__ Pack p) {
   const int lane = threadIdx.x & 31;
-  const int64_t item0 = (static_cast<int64_t>(blockIdx.x) * kWarps + (threadIdx.x >> 5)) * kRows;
-  Raw<E> raw[kRows];
-  int left[kRows];
+  const int64_t item0 = (static_cast<int64_t>(blockIdx.x) * kWarps + (threadIdx.x >> 5)) * kPackRows;
+  Raw<E> raw[kPackRows];
+  int left[kPackRows];
 #pragma unroll
-  for (int i = 0; i < kRows; ++i) {
+  for (int i = 0; i < kPackRows; ++i) {
     raw[i] = {};
     left[i] = 0;
     if (item0 + i < p.items) {
@@ -56,7 +56,7 @@ __global__ void __launch_bounds__(kThreads) checkpoint_pack_kernel(const __grid_
     }
   }
 #pragma unroll
-  for (int i = 0; i < kRows; ++i) {
+  for (int i = 0; i < kPackRows; ++i) {
     if (item0 + i >= p.items) break;
     const PackTensor &t = p.t[tensor_of(p, item0 + i)];
     const int64_t n = item0 + i - t.first, row = n / t.groups, c0 = n % t.groups * kGroupValues;
@@ -79,10 +79,10 @@ __global__ void __launch_bounds__(kThreads) checkpoint_pack_kernel(const __grid_
 template <typename E, bool kVec>
 __global__ void __launch_bounds__(kThreads) checkpoint_unpack_kernel(const __grid_constant__ Pack p) {
   const int lane = threadIdx.x & 31;
-  const int64_t item0 = (static_cast<int64_t>(blockIdx.x) * kWarps + (threadIdx.x >> 5)) * kRows;
-  uint32_t q[kRows], ex[kRows];
+  const int64_t item0 = (static_cast<int64_t>(blockIdx.x) * kWarps + (threadIdx.x >> 5)) * kPackRows;
+  uint32_t q[kPackRows], ex[kPackRows];
 #pragma unroll
-  for (int i = 0; i < kRows; ++i) {
+  for (int i = 0; i < kPackRows; ++i) {
     q[i] = ex[i] = 0;
     if (item0 + i < p.items) {
       const PackTensor &t = p.t[tensor_of(p, item0 + i)];
@@ -100,7 +100,7 @@ __global__ void __launch_bounds__(kThreads) checkpoint_unpack_kernel(const __gri
     }
   }
 #pragma unroll
-  for (int i = 0; i < kRows; ++i) {
+  for (int i = 0; i < kPackRows; ++i) {
     if (item0 + i >= p.items) break;
     const PackTensor &t = p.t[tensor_of(p, item0 + i)];
     const int64_t n = item0 + i - t.first, row = n / t.groups, c0 = n % t.groups * kGroupValues;
@@ -113,7 +113,7 @@ __global__ void __launch_bounds__(kThreads) checkpoint_unpack_kernel(const __gri
 
 template <typename E>
 cudaError_t launch_checkpoint_e(const Pack &p, bool vec, bool unpack, cudaStream_t stream) {
-  const int64_t per_block = kWarps * kRows;
+  const int64_t per_block = kWarps * kPackRows;
   const unsigned blocks = static_cast<unsigned>((p.items + per_block - 1) / per_block);
   auto kernel = unpack ? (vec ? checkpoint_unpack_kernel<E, true> : checkpoint_unpack_kernel<E, false>)
                        : (vec ? checkpoint_pack_kernel<E, true> : checkpoint_pack_kernel<E, false>);

@@ -17,75 +17,10 @@
 // after it.  A serial chain thus has one link per 32 chunks, and the order of
 // all roundings is fixed: results do not depend on timing.  Tiles are taken
 // by ticket in chunk order, so a CTA only ever waits for CTAs that already run.
-#include <type_traits>
-
-#include "gdn_recurrence.cuh"
+#include "gdn_recurrence_tile.cuh"
 
 namespace gdn {
 namespace rec {
-
-struct Header {
-  uint32_t ticket;
-  uint32_t bad;  // cu_seqlens or slots are not valid: write nothing
-  uint32_t pad[254];
-};
-static_assert(sizeof(Header) == 1024, "words start 1024 bytes into the workspace");
-
-struct Seqs {
-  const int64_t *cu;  // [N + 1], or null: N sequences of S tokens each
-  int64_t N, T, S;
-  const int32_t *slots;  // state row of a sequence, or null: its number
-  int64_t pool;
-  __device__ __forceinline__ int64_t at(int64_t n) const { return cu != nullptr ? cu[n] : n * S; }
-  __device__ __forceinline__ int64_t row(int64_t n) const { return slots != nullptr ? slots[n] : n; }
-  __device__ __forceinline__ int64_t total() const { return cu != nullptr ? cu[N] : T; }
-};
-
-// Checks cu_seqlens and slots with all threads of a CTA; returns the device
-// status code of what is wrong, or 0.
-__device__ __forceinline__ int check_seqs(const Seqs &s) {
-  int bad_cu = 0, bad_slot = 0;
-  if (s.cu != nullptr) {
-    if (threadIdx.x == 0) bad_cu = s.cu[0] != 0 || s.cu[s.N] > s.T;
-    for (int64_t n = threadIdx.x; n < s.N; n += blockDim.x) bad_cu |= s.cu[n] > s.cu[n + 1];
-  }
-  if (s.slots != nullptr)
-    for (int64_t n = threadIdx.x; n < s.N; n += blockDim.x)
-      bad_slot |= s.slots[n] < 0 || s.slots[n] >= s.pool;
-  bad_cu = __syncthreads_or(bad_cu);
-  bad_slot = __syncthreads_or(bad_slot);
-  return bad_cu ? kDevStatusBadSeqlens : bad_slot ? kDevStatusBadSlot : 0;
-}
-
-// Empties the words and checks the sequences, before the tiles run.
-__global__ void __launch_bounds__(1024) recurrence_init_kernel(Header *hdr, ulonglong2 *words, int64_t n,
-                                                               const Seqs s) {
-  const ulonglong2 e = make_ulonglong2(kEmptyWord, kEmptyWord);
-  for (int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; i < n;
-       i += static_cast<int64_t>(gridDim.x) * blockDim.x)
-    words[i] = e;
-  if (blockIdx.x == 0) {
-    const int code = check_seqs(s);
-    if (threadIdx.x == 0) {
-      hdr->ticket = 0;
-      hdr->bad = code != 0;
-      if (code) set_device_status(code);
-    }
-  }
-}
-
-// First n in [0, N] with at(n) >= v (N if none), by all lanes of a warp.
-__device__ __forceinline__ int64_t first_at_or_after(const Seqs &s, int64_t v, int lane) {
-  if (s.cu == nullptr) return s.S > 0 ? min((v + s.S - 1) / s.S, s.N) : 0;
-  int64_t lo = 0, hi = s.N;
-  while (lo < hi) {
-    const int64_t step = (hi - lo + 31) / 32, i = lo + (lane + 1) * step - 1;
-    const int64_t k = __popc(__ballot_sync(0xffffffffu, i < hi && s.cu[i] < v));
-    hi = min(hi, lo + (k + 1) * step - 1);
-    lo += k * step;
-  }
-  return lo;
-}
 
 // The sequences that start or end in a chunk, by token of the chunk (-1: none).
 struct ChunkSeqs {
@@ -200,201 +135,6 @@ __device__ __forceinline__ void zero_rows(void *p, int64_t from, int64_t to, int
                                           int lane, int left) {
   for (int64_t t = from + warp; t < to; t += kWarps)
     store4<E, kVec>(static_cast<E *>(p) + t * D + c0, lane, left, 0, 0);
-}
-
-// ---- prefill -------------------------------------------------------------------
-struct Forward {
-  const void *x, *a, *b;
-  int64_t x_stride, a_stride, b_stride;  // elements from one token to the next
-  const float *A_log, *dt_bias;
-  const float *state;  // rows of D, or null: zeros
-  Seqs s;
-  int64_t D;
-  void *out;       // [T, D], or null
-  float *final;    // rows of D, or null; may be `state`
-  float *carries;  // [chunk][tile][128] states that enter the chunks, or null
-  uint8_t *packed; // 8-bit x, a, b (kPack)
-  int zero_behind; // write zeros to out behind the last sequence
-  Header *hdr;     // kChain
-  Chain chain;
-};
-
-// kChain: one tile per CTA, joined by look-back.  Without it a CTA walks the
-// chunks of its 128 channels one after the other and nothing is shared: one
-// launch, for short inputs.
-template <typename E, bool kVec, bool kPack, bool kChain>
-__global__ void __launch_bounds__(kThreads, 2)
-recurrence_forward_kernel(const __grid_constant__ Forward p) {
-  __shared__ Shared sh;
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int nd = static_cast<int>((p.D + kTileCh - 1) / kTileCh);
-  int64_t chunk = 0;
-  int d;
-  if constexpr (kChain) {
-    if (tid == 0) {
-      sh.broken = 0;
-      sh.ticket = p.hdr->bad ? -1 : static_cast<int>(atomicAdd(&p.hdr->ticket, 1u));
-    }
-    __syncthreads();
-    if (sh.ticket < 0) return;
-    chunk = sh.ticket / nd;
-    d = sh.ticket % nd;
-  } else {
-    d = blockIdx.x;
-    const int code = check_seqs(p.s);
-    if (code) {
-      if (tid == 0) set_device_status(code);
-      return;
-    }
-  }
-  const int64_t total = p.s.total();
-  const int64_t last = total > 0 ? (total - 1) / kChunkTok : 0;
-  const int64_t c0 = static_cast<int64_t>(d) * kTileCh;
-  const int left = static_cast<int>(min(p.D - c0, int64_t{kTileCh}));
-  if (p.zero_behind) {
-    const int64_t base = chunk * kChunkTok;
-    zero_rows<E, kVec>(p.out, max(base, total), kChain ? min(base + kChunkTok, p.s.T) : p.s.T, p.D, c0, warp,
-                       lane, left);
-  }
-  if (chunk > last) return;
-  const Params par = load_params<kVec>(p.A_log + c0, p.dt_bias + c0, lane, left);
-  float h[4] = {0.f, 0.f, 0.f, 0.f};
-
-  for (;; ++chunk) {
-    const int64_t base = chunk * kChunkTok, t0 = base + warp * kTok;
-    const int valid = static_cast<int>(max(int64_t{0}, min(int64_t{kTok}, total - t0)));
-
-    // loads of a batch of tokens, then their gates
-    uint64_t g[kTok][2], u[kTok][2];
-    constexpr int kBatch = sizeof(E) == 4 ? 4 : 8;
-#pragma unroll
-    for (int i0 = 0; i0 < kTok; i0 += kBatch) {
-      Raw<E> xr[kBatch], ar[kBatch], br[kBatch];
-#pragma unroll
-      for (int i = 0; i < kBatch; ++i) {
-        xr[i] = ar[i] = br[i] = {};
-        if (i0 + i < valid) {
-          const int64_t t = t0 + i0 + i;
-          xr[i] = load4<E, kVec>(static_cast<const E *>(p.x) + t * p.x_stride + c0, lane, left);
-          ar[i] = load4<E, kVec>(static_cast<const E *>(p.a) + t * p.a_stride + c0, lane, left);
-          br[i] = load4<E, kVec>(static_cast<const E *>(p.b) + t * p.b_stride + c0, lane, left);
-        }
-      }
-#pragma unroll
-      for (int i = 0; i < kBatch; ++i) {
-        uint64_t x[2], a[2], b[2];
-        xr[i].pairs(x[0], x[1]);
-        ar[i].pairs(a[0], a[1]);
-        br[i].pairs(b[0], b[1]);
-        if constexpr (kPack) {
-          if (i0 + i < valid) {
-            const int64_t t = t0 + i0 + i;
-            const uint64_t *v[3] = {x, a, b};
-#pragma unroll
-            for (int w = 0; w < 3; ++w) {
-              const uint32_t ex = group_exponent(
-                  __reduce_max_sync(0xffffffffu, abs_max_bits(v[w][0], v[w][1])), exp_cap<E>());
-              const uint32_t q = quantise4(v[w][0], v[w][1], ex, exp_cap<E>());
-              uint8_t *dst = p.packed + (w * p.s.T + t) * p.D + c0;
-              if constexpr (kVec) {
-                if (4 * lane < left) reinterpret_cast<uint32_t *>(dst)[lane] = q;
-              } else {
-#pragma unroll
-                for (int j = 0; j < 4; ++j)
-                  if (lane + 32 * j < left) dst[lane + 32 * j] = static_cast<uint8_t>(q >> (8 * j));
-              }
-              if (lane == 0)
-                p.packed[3 * p.s.T * p.D + (w * p.s.T + t) * nd + d] = static_cast<uint8_t>(ex);
-            }
-          }
-        }
-#pragma unroll
-        for (int k = 0; k < 2; ++k)
-          gate_pair(x[k], a[k], b[k], par.dt[k], par.c[k], g[i0 + i][k], u[i0 + i][k]);
-      }
-    }
-
-    find_sequences(p.s, sh.seqs, base, chunk == last, warp, lane, [&](int64_t n) {
-      if (p.final == nullptr) return;
-      const int64_t row = p.s.row(n) * p.D + c0;
-      const float4 v = p.state != nullptr ? load_f32<kVec>(p.state + row, lane, left)
-                                          : make_float4(0.f, 0.f, 0.f, 0.f);
-      store_f32<kVec>(p.final + row, lane, left, v);
-    });
-    const unsigned starts = __ballot_sync(0xffffffffu, lane < kTok && sh.seqs.start[warp * kTok + (lane & 7)] >= 0);
-    const unsigned ends = __ballot_sync(0xffffffffu, lane < kTok && sh.seqs.end[warp * kTok + (lane & 7)] >= 0);
-    const bool enters = sh.seqs.start[0] < 0;  // the state before the chunk matters
-
-    // the map of this warp's tokens; a start's u becomes the state after it
-    uint64_t A2[2] = {f2_dup(1.f), f2_dup(1.f)}, H2[2] = {0, 0};
-#pragma unroll
-    for (int i = 0; i < kTok; ++i) {
-      if (i >= valid) {
-#pragma unroll
-        for (int k = 0; k < 2; ++k) g[i][k] = f2_dup(1.f), u[i][k] = 0;
-      }
-      if ((starts >> i) & 1) {
-        if (p.state != nullptr) {
-          const float4 v = load_f32<kVec>(
-              p.state + p.s.row(sh.seqs.start[warp * kTok + i]) * p.D + c0, lane, left);
-          u[i][0] = f2_fma(g[i][0], f2_pack(v.x, v.y), u[i][0]);
-          u[i][1] = f2_fma(g[i][1], f2_pack(v.z, v.w), u[i][1]);
-        }
-#pragma unroll
-        for (int k = 0; k < 2; ++k) A2[k] = f2_dup(-1.f), H2[k] = u[i][k];
-      } else {
-#pragma unroll
-        for (int k = 0; k < 2; ++k) A2[k] = f2_mul(A2[k], g[i][k]), H2[k] = f2_fma(g[i][k], H2[k], u[i][k]);
-      }
-    }
-    put_map(sh.own[warp], lane,
-            Map4{{f2_lo(A2[0]), f2_hi(A2[0]), f2_lo(A2[1]), f2_hi(A2[1])},
-                 {f2_lo(H2[0]), f2_hi(H2[0]), f2_lo(H2[1]), f2_hi(H2[1])}});
-    __syncthreads();
-
-    if constexpr (kChain) {
-      const bool group_end = chunk % kGroup == kGroup - 1;
-      if (warp == 0 && chunk < last && !group_end) {
-        Map4 m = get_map(sh.own[0], lane);
-        for (int i = 1; i < kWarps; ++i) compose(m, get_map(sh.own[i], lane));
-        put_words(p.chain.maps + (chunk * nd + d) * kTileCh, lane, m.A, m.H);
-      }
-      if (enters) look_back(sh, p.chain, chunk, d, nd, warp, lane, h);
-      if (warp == kWarps - 1 && chunk < last && group_end) {
-        float hg[4] = {h[0], h[1], h[2], h[3]};
-        for (int i = 0; i < kWarps; ++i) advance(hg, sh.own[i], lane);
-        const float zero[4] = {0.f, 0.f, 0.f, 0.f};
-        put_words(p.chain.states + (chunk / kGroup * nd + d) * kTileCh, lane, zero, hg);
-      }
-    }
-    // in channel order: the backward may take other accesses than this call
-    if (p.carries != nullptr && warp == 0)
-      store_f32<kVec>(p.carries + (chunk * nd + d) * kTileCh, lane, kTileCh, make_float4(h[0], h[1], h[2], h[3]));
-    for (int i = 0; i < warp; ++i) advance(h, sh.own[i], lane);
-
-    uint64_t s2[2] = {f2_pack(h[0], h[1]), f2_pack(h[2], h[3])};
-    E *out = static_cast<E *>(p.out) + t0 * p.D + c0;
-#pragma unroll
-    for (int i = 0; i < kTok; ++i) {
-      if ((starts >> i) & 1) {
-        s2[0] = u[i][0];
-        s2[1] = u[i][1];
-      } else {
-        s2[0] = f2_fma(g[i][0], s2[0], u[i][0]);
-        s2[1] = f2_fma(g[i][1], s2[1], u[i][1]);
-      }
-      if (p.out != nullptr && i < valid) store4<E, kVec>(out + i * p.D, lane, left, s2[0], s2[1]);
-      if (((ends >> i) & 1) && p.final != nullptr)
-        store_f32<kVec>(p.final + p.s.row(sh.seqs.end[warp * kTok + i]) * p.D + c0, lane, left,
-                        make_float4(f2_lo(s2[0]), f2_hi(s2[0]), f2_lo(s2[1]), f2_hi(s2[1])));
-    }
-    if constexpr (kChain) return;
-    if (chunk == last) return;
-    // the state after the chunk, for the next one
-    h[0] = f2_lo(s2[0]), h[1] = f2_hi(s2[0]), h[2] = f2_lo(s2[1]), h[3] = f2_hi(s2[1]);
-    for (int i = warp + 1; i < kWarps; ++i) advance(h, sh.own[i], lane);
-    __syncthreads();
-  }
 }
 
 // ---- backward ------------------------------------------------------------------
@@ -725,63 +465,20 @@ __global__ void __launch_bounds__(kThreads) recurrence_decode_kernel(const __gri
 }
 
 // ---- sizes and launches ----------------------------------------------------------
-inline int64_t tiles_of(int64_t D) { return (D + kTileCh - 1) / kTileCh; }
-inline int64_t chunks_of(int64_t T) { return T > 0 ? (T + kChunkTok - 1) / kChunkTok : 1; }
-inline size_t words_bytes(int64_t T, int64_t D) {
-  const int64_t groups = (chunks_of(T) + kGroup - 1) / kGroup;
-  return static_cast<size_t>((chunks_of(T) + groups) * tiles_of(D) * kTileCh * 8);
-}
 inline size_t saved_bytes(int64_t T, int64_t D) {  // carries
   return static_cast<size_t>(chunks_of(T) * tiles_of(D) * kTileCh * 4);
-}
-
-// Inputs of up to this many chunks are walked by one CTA per 128 channels.
-constexpr int64_t kSerialChunks = 4;
-constexpr int64_t kSerialSeqs = 1024;  // each CTA checks all of cu_seqlens then
-
-inline bool serial(const Seqs &s) {
-  return chunks_of(s.T) <= kSerialChunks && (s.cu == nullptr || s.N <= kSerialSeqs);
-}
-
-inline cudaError_t launch_init(Header *hdr, Chain &ch, const Seqs &s, int64_t D, cudaStream_t stream) {
-  uint64_t *words = reinterpret_cast<uint64_t *>(hdr + 1);
-  ch.maps = words;
-  ch.states = words + chunks_of(s.T) * tiles_of(D) * kTileCh;
-  const int64_t n = static_cast<int64_t>(words_bytes(s.T, D) / 16);
-  const int64_t blocks = min(int64_t{148 * 2}, (n + 1023) / 1024);
-  recurrence_init_kernel<<<static_cast<unsigned>(max(blocks, int64_t{1})), 1024, 0, stream>>>(
-      hdr, reinterpret_cast<ulonglong2 *>(words), n, s);
-  return cudaGetLastError();
-}
-
-template <typename E, bool kVec, bool kPack>
-cudaError_t launch_forward_t(Forward p, void *workspace, cudaStream_t stream) {
-  const int64_t nd = tiles_of(p.D);
-  if (serial(p.s)) {
-    recurrence_forward_kernel<E, kVec, kPack, false><<<static_cast<unsigned>(nd), kThreads, 0, stream>>>(p);
-    return cudaGetLastError();
-  }
-  p.hdr = static_cast<Header *>(workspace);
-  if (cudaError_t e = launch_init(p.hdr, p.chain, p.s, p.D, stream)) return e;
-  recurrence_forward_kernel<E, kVec, kPack, true>
-      <<<static_cast<unsigned>(chunks_of(p.s.T) * nd), kThreads, 0, stream>>>(p);
-  return cudaGetLastError();
-}
-
-template <typename E>
-cudaError_t launch_forward_e(const Forward &p, bool vec, void *workspace, cudaStream_t stream) {
-  if (p.packed != nullptr)
-    return vec ? launch_forward_t<E, true, true>(p, workspace, stream)
-               : launch_forward_t<E, false, true>(p, workspace, stream);
-  return vec ? launch_forward_t<E, true, false>(p, workspace, stream)
-             : launch_forward_t<E, false, false>(p, workspace, stream);
 }
 
 template <typename E, bool kVec, bool kPacked>
 cudaError_t launch_backward_t(Backward p, void *workspace, float *dA_log, float *ddt_bias, cudaStream_t stream) {
   const int64_t nd = tiles_of(p.D);
   p.hdr = static_cast<Header *>(workspace);
-  if (cudaError_t e = launch_init(p.hdr, p.chain, p.s, p.D, stream)) return e;
+  const Places w = places(workspace, p.s.T, p.D);
+  p.chain.maps = w.words;
+  p.chain.states = p.chain.maps + chunks_of(p.s.T) * nd * kTileCh;
+  const Prepared q{p.A_log, p.dt_bias, w.dt, w.c, p.D, nullptr, 0, kRows};
+  const int64_t words = (chunks_of(p.s.T) + (chunks_of(p.s.T) + kGroupLen - 1) / kGroupLen) * nd * kTileCh;
+  if (cudaError_t e = launch_init(p.hdr, w.words, words, p.s, q, stream)) return e;
   recurrence_backward_kernel<E, kVec, kPacked>
       <<<static_cast<unsigned>(chunks_of(p.s.T) * nd), kThreads, 0, stream>>>(p);
   if (cudaError_t e = cudaGetLastError()) return e;

@@ -37,8 +37,24 @@ bool bad_f32_alignment(std::initializer_list<const void *> ps) {
   return false;
 }
 
+// Whether rows can be fetched by TMA: 16-byte rows and bases.
+bool tma_rows(const void *p, int type, int64_t stride) {
+  return aligned(p, 16) && stride * type_size(type) % 16 == 0 && stride > 0;
+}
+
 gdn::rec::Seqs sequences(const int64_t *cu, int64_t N, int64_t T, const int32_t *slots, int64_t pool) {
   return gdn::rec::Seqs{cu, N, T, N > 0 ? T / N : 0, slots, pool};
+}
+
+int run_forward(int type, const gdn::rec::Forward &p, void *workspace, int sms, cudaStream_t s) {
+  const bool tma = p.s.T > 0 && p.s.T <= INT32_MAX && tma_rows(p.x, type, p.x_stride) &&
+                   tma_rows(p.a, type, p.a_stride) && tma_rows(p.b, type, p.b_stride) && p.D % 4 == 0 &&
+                   aligned(p.out, 8) && aligned(p.A_log, 8) && aligned(p.dt_bias, 8) && aligned(p.state, 8) &&
+                   aligned(p.final, 8);
+  const cudaError_t e = type == GDN_BF16   ? gdn::rec::launch_forward_e<__nv_bfloat16>(p, tma, workspace, sms, s)
+                        : type == GDN_FP16 ? gdn::rec::launch_forward_e<__half>(p, tma, workspace, sms, s)
+                                           : gdn::rec::launch_forward_e<float>(p, tma, workspace, sms, s);
+  return e == cudaSuccess ? GDN_OK : GDN_ERR_LAUNCH;
 }
 
 }  // namespace
@@ -47,7 +63,7 @@ extern "C" {
 
 size_t gdn_recurrence_workspace_bytes(int64_t total_tokens, int64_t channels) {
   if (!good_sizes(GDN_BF16, total_tokens, 1, channels)) return 0;
-  return sizeof(gdn::rec::Header) + gdn::rec::words_bytes(total_tokens, channels);
+  return (gdn::rec::places(nullptr, total_tokens, channels).bytes + 1023) / 1024 * 1024;
 }
 
 size_t gdn_recurrence_carry_bytes(int64_t total_tokens, int64_t channels) {
@@ -87,7 +103,8 @@ int gdn_recurrence_prefill(int type, const void *x, int64_t x_stride, const void
     return GDN_ERR_WORKSPACE;
   const size_t states = static_cast<size_t>(slots ? pool_slots : num_seqs) * channels * 4;
   if (state && state != final_state && overlap(state, states, final_state, states)) return GDN_ERR_ALIASING;
-  if (int st = check_device(nullptr)) return st;
+  int sms = 0;
+  if (int st = check_device(&sms)) return st;
   gdn::rec::Forward p{};
   p.x = x, p.a = a, p.b = b;
   p.x_stride = x_stride, p.a_stride = a_stride, p.b_stride = b_stride;
@@ -95,14 +112,7 @@ int gdn_recurrence_prefill(int type, const void *x, int64_t x_stride, const void
   p.s = sequences(cu_seqlens, num_seqs, total_tokens, slots, pool_slots);
   p.D = channels, p.zero_behind = zero_behind && cu_seqlens && total_tokens > 0;
   p.out = out, p.final = final_state, p.carries = carries, p.packed = static_cast<uint8_t *>(packed);
-  const bool vec = channels % 4 == 0 && vector_rows(x, type, x_stride) && vector_rows(a, type, a_stride) &&
-                   vector_rows(b, type, b_stride) && vector_rows(out, type, channels) && aligned(A_log, 16) &&
-                   aligned(dt_bias, 16) && (!state || aligned(state, 16)) && aligned(final_state, 16);
-  cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const cudaError_t e = type == GDN_BF16   ? gdn::rec::launch_forward_e<__nv_bfloat16>(p, vec, workspace, s)
-                        : type == GDN_FP16 ? gdn::rec::launch_forward_e<__half>(p, vec, workspace, s)
-                                           : gdn::rec::launch_forward_e<float>(p, vec, workspace, s);
-  return e == cudaSuccess ? GDN_OK : GDN_ERR_LAUNCH;
+  return run_forward(type, p, workspace, sms, static_cast<cudaStream_t>(stream));
 }
 
 int gdn_recurrence_backward(int type, const void *x, int64_t x_stride, const void *a, int64_t a_stride,
@@ -131,7 +141,8 @@ int gdn_recurrence_backward(int type, const void *x, int64_t x_stride, const voi
   if (d_state && ((state && overlap(state, states, d_state, states)) ||
                   (d_final_state && d_final_state != d_state && overlap(d_final_state, states, d_state, states))))
     return GDN_ERR_ALIASING;
-  if (int st = check_device(nullptr)) return st;
+  int sms = 0;
+  if (int st = check_device(&sms)) return st;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const gdn::rec::Seqs seqs = sequences(cu_seqlens, num_seqs, total_tokens, nullptr, 0);
   if (num_seqs == 0) {
@@ -154,10 +165,7 @@ int gdn_recurrence_backward(int type, const void *x, int64_t x_stride, const voi
     f.x = x, f.a = a, f.b = b;
     f.x_stride = x_stride, f.a_stride = a_stride, f.b_stride = b_stride;
     f.A_log = A_log, f.dt_bias = dt_bias, f.state = state, f.s = seqs, f.D = channels, f.carries = saved;
-    const cudaError_t e = type == GDN_BF16   ? gdn::rec::launch_forward_e<__nv_bfloat16>(f, vec, workspace, s)
-                          : type == GDN_FP16 ? gdn::rec::launch_forward_e<__half>(f, vec, workspace, s)
-                                             : gdn::rec::launch_forward_e<float>(f, vec, workspace, s);
-    if (e != cudaSuccess) return GDN_ERR_LAUNCH;
+    if (int st = run_forward(type, f, workspace, sms, s)) return st;
   }
   gdn::rec::Backward p{};
   p.x = x, p.a = a, p.b = b, p.d_out = d_out;

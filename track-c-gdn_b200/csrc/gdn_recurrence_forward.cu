@@ -1,0 +1,547 @@
+// gdn_recurrence_forward.cu -- prefill of the channelwise gated linear
+// recurrence (mathematics and look-back: gdn_recurrence.cu).
+#include <cuda.h>
+
+#include "gdn_recurrence_tile.cuh"
+
+namespace gdn {
+namespace rec {
+
+// Shape of a tile: 64 rows x 64 channels for 8 consumer warps, or with kPack
+// the 128 channels that share a scale for 16.  A lane has 2 channels of 8
+// consecutive rows.  A stage of shared memory holds one half (64 channels) as
+// planes of x, a and b, and afterwards, in place, what the first pass left: 16
+// bytes for each lane and row.
+constexpr int kTokW = 8;
+constexpr int kSlots = 8;
+constexpr int kRows = kTokW * kSlots;  // 64
+template <typename E, bool kTma, bool kPack>
+struct FwdShape {
+  static constexpr int kHalves = kPack ? 2 : 1;
+  static constexpr int kCh = 64 * kHalves;
+  static constexpr int kWorkers = kSlots * kHalves;       // consumer warps
+  static constexpr int kThreads = 32 * (kWorkers + 1 + 2 * kHalves);
+  static constexpr int kPlane = kRows * 64 * static_cast<int>(sizeof(E));
+  static constexpr int kHalfStage = kTma ? (sizeof(E) == 4 ? 3 : 4) * kPlane : kRows * 512;
+  static constexpr int kStage = kHalves * kHalfStage;
+  static constexpr int kStages = kHalfStage > 32768 ? 2 : 3;
+  static constexpr int kCtas = kPack ? 1 : 2;             // of an SM
+  // where a lane's 16 bytes of row i (of its 8) lie, from its slot's rows in
+  // the first plane: only rows that this warp alone reads are overwritten
+  static constexpr int kPerPlane = kTma ? (sizeof(E) == 4 ? 4 : 2) : kTokW;
+  static constexpr int kPlaneBytes = kTma ? kPlane : kRows * 512;
+};
+
+struct Forward {
+  CUtensorMap tx, ta, tb;  // kTma
+  const void *x, *a, *b;
+  int64_t x_stride, a_stride, b_stride;  // elements from one token to the next
+  const float *A_log, *dt_bias;
+  const float *state;  // rows of D, or null: zeros
+  Seqs s;
+  int64_t D;
+  void *out;       // [T, D], or null
+  float *final;    // rows of D, or null; may be `state`
+  float *carries;  // [T / 64][D up to 128s] states before every 64th row, or null
+  uint8_t *packed; // 8-bit x, a, b (kPack)
+  int zero_behind; // write zeros to out behind the last sequence
+  Header *hdr;     // kChain
+  uint64_t *maps, *states;  // kChain
+  const float *dt, *c;      // kChain: prepared
+  const int *first;
+};
+
+// What the consumers need of an ordinary tile: all rows belong to sequences that
+// neither start nor end there, and all 64 channels of each half exist.
+struct alignas(16) Tile {
+  int64_t at;  // element of out where the tile begins
+  int d;       // the tile's channels; -1: no more tiles
+  int plain;
+};
+
+template <typename Shape, bool kPack>
+struct FwdShared {
+  // maps of the slots' rows (A, A, H, H of a lane's channels); the chain warp
+  // replaces them by the states that enter the slots
+  float4 own[Shape::kStages][Shape::kHalves][kSlots][32];
+  float params[Shape::kStages][2][Shape::kCh];  // kChain: dt_bias and c of the tile's channels
+  Table<kRows> tables[Shape::kStages];
+  Tile tiles[Shape::kStages];
+  uint64_t full[Shape::kStages], ready[Shape::kStages], empty[Shape::kStages];
+  uint64_t mapped[Shape::kStages][Shape::kHalves];  // the slots' maps are there
+  uint64_t taken[Shape::kStages][Shape::kHalves];   // ... and have been read for the tile's
+  uint64_t pair[kPack ? kSlots : 1];
+  uint32_t amax[kPack ? 2 * kRows * 3 * 2 : 1];
+  int broken;
+};
+
+// Roles of the warps, joined by mbarriers alone:
+//   producer   takes tiles by ticket, fills the table, has the inputs copied
+//   consumers  first pass: gates; per row the state y from a zero start and the
+//              product P of the gates so far, left in shared memory; the map
+//              (P, y) of the slot, and the tile's, which is published.  Second
+//              pass, one tile later: out = y + P h, with h the state that
+//              enters the slot.
+//   chain      (two per half, for tiles in turn) looks back and hands each slot
+//              its state.  It has the time of two first passes for that, so
+//              that the look-back's latency costs the consumers nothing.
+// Without kChain (short inputs, one launch) a CTA walks all chunks of its
+// channels and the chain warp keeps the state.
+template <typename E, bool kTma, bool kPack, bool kChain>
+__global__ void __launch_bounds__(FwdShape<E, kTma, kPack>::kThreads, FwdShape<E, kTma, kPack>::kCtas)
+recurrence_forward_kernel(const __grid_constant__ Forward p) {
+  using S = FwdShape<E, kTma, kPack>;
+  constexpr bool kVec = kTma;
+  constexpr int kCh = S::kCh, kStages = S::kStages;
+  extern __shared__ __align__(1024) unsigned char smem[];
+  FwdShared<S, kPack> &sh = *reinterpret_cast<FwdShared<S, kPack> *>(smem + kStages * S::kStage);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int nt = static_cast<int>((p.D + kCh - 1) / kCh);
+
+  if constexpr (kChain) {
+    if (p.hdr->bad) return;
+  } else {
+    const int code = check_seqs(p.s);
+    if (code) {
+      if (tid == 0) set_device_status(code);
+      return;
+    }
+  }
+  if (tid == 0) {
+    sh.broken = 0;
+    for (int i = 0; i < kStages; ++i) {
+      mbar_init(smem_u32(&sh.full[i]), 1);
+      for (int w = 0; w < S::kHalves; ++w) {
+        mbar_init(smem_u32(&sh.mapped[i][w]), kSlots);
+        mbar_init(smem_u32(&sh.taken[i][w]), 1);
+      }
+      mbar_init(smem_u32(&sh.ready[i]), S::kHalves);
+      mbar_init(smem_u32(&sh.empty[i]), S::kWorkers);
+    }
+    if (kPack)
+      for (int i = 0; i < kSlots; ++i) mbar_init(smem_u32(&sh.pair[i]), 2);
+    mbar_init_fence();
+  }
+  __syncthreads();
+  const int64_t total = p.s.total();
+  const int64_t last = total > 0 ? (total - 1) / kRows : 0;
+
+  if (warp == S::kWorkers) {
+    // ---- producer ----
+    const int64_t tiles = ((p.s.T > 0 ? p.s.T - 1 : 0) / kRows + 1) * nt;
+    int64_t next = 0;  // !kChain: the next chunk
+    uint32_t ticket = 0;
+    if (kChain && lane == 0) ticket = atomicAdd(&p.hdr->ticket, 1u);
+    int k = 0, ends = 0;
+    while (true) {
+      int64_t chunk;
+      int d = blockIdx.x;
+      if constexpr (kChain) {
+        const int64_t t = __shfl_sync(0xffffffffu, ticket, 0);
+        if (lane == 0 && t < tiles) ticket = atomicAdd(&p.hdr->ticket, 1u);  // the next one, early
+        chunk = t < tiles ? t / nt : -1;
+        d = static_cast<int>(t % nt);
+      } else {
+        chunk = next * kRows < max(p.s.T, int64_t{1}) ? next : -1;
+        ++next;
+      }
+      const int64_t c0 = static_cast<int64_t>(d) * kCh, base = chunk * kRows;
+      if (chunk >= 0 && p.zero_behind) {
+        for (int64_t t = max(base, total); t < min(base + kRows, p.s.T); ++t)
+#pragma unroll
+          for (int w = 0; w < S::kHalves; ++w)
+            store2<E, kVec>(static_cast<E *>(p.out) + t * p.D + c0 + 64 * w, lane,
+                            static_cast<int>(min(p.D - c0 - 64 * w, int64_t{64})), 0);
+      }
+      if (chunk > last) continue;
+      const int s = k % kStages;
+      const bool go = k < kStages || wait_phase(smem_u32(&sh.empty[s]), ((k / kStages) - 1) & 1, &sh.broken);
+      if (!__all_sync(0xffffffffu, go)) break;
+      Table<kRows> &t = sh.tables[s];
+      const uint32_t full = smem_u32(&sh.full[s]);
+      if (chunk < 0) {
+        if (lane == 0) {
+          t.chunk = -1;
+          sh.tiles[s].d = -1;
+          mbar_arrive(full);
+        }
+        ++k;
+        if (++ends == 2) break;  // one for each chain warp
+        continue;
+      }
+      if (kChain && lane == 0) {
+        mbar_expect_tx(full, 2 * kCh * 4);
+        bulk_load(smem_u32(sh.params[s][0]), p.dt + c0, kCh * 4, full);
+        bulk_load(smem_u32(sh.params[s][1]), p.c + c0, kCh * 4, full);
+      }
+      if (kTma && lane == 0) {
+        mbar_expect_tx(full, S::kHalves * 3 * S::kPlane);
+#pragma unroll
+        for (int w = 0; w < S::kHalves; ++w) {
+          const uint32_t dst = smem_u32(smem + s * S::kStage + w * S::kHalfStage);
+          const int x = static_cast<int>(c0) + 64 * w, y = static_cast<int>(base);
+          tma_load_2d(dst, &p.tx, x, y, full);
+          tma_load_2d(dst + S::kPlane, &p.ta, x, y, full);
+          tma_load_2d(dst + 2 * S::kPlane, &p.tb, x, y, full);
+        }
+      }
+      fill_table<kRows>(p.s, t, base, chunk == last, lane, kChain ? p.first : nullptr, [&](int64_t n) {
+        if (p.final == nullptr) return;  // an empty sequence's final state is its initial state
+#pragma unroll
+        for (int w = 0; w < S::kHalves; ++w) {
+          const int left = static_cast<int>(min(p.D - c0 - 64 * w, int64_t{64}));
+          const int64_t row = p.s.row(n) * p.D + c0 + 64 * w;
+          store2_f32<kVec>(p.final + row, lane, left,
+                           p.state != nullptr ? load2_f32<kVec>(p.state + row, lane, left) : 0);
+        }
+      });
+      if (lane == 0) {
+        t.chunk = chunk;
+        t.d = d;
+        t.last = chunk == last;
+        t.valid = min(total - base, int64_t{kRows});
+        const bool edge = (t.starts[0] | t.starts[1] | t.ends[0] | t.ends[1]) != 0;
+        sh.tiles[s] = Tile{base * p.D + c0, d,
+                           !edge && base + kRows <= total && c0 + kCh <= p.D && p.out != nullptr};
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(full);
+      ++k;
+    }
+    // after a wait that ran out: no copy may be in flight when the CTA ends
+    if ((kTma || kChain) && *static_cast<volatile int *>(&sh.broken))
+      for (int i = max(k - kStages, 0); i < k - ends; ++i)
+        mbar_wait(smem_u32(&sh.full[i % kStages]), (i / kStages) & 1);
+    return;
+  }
+
+  if (warp > S::kWorkers) {
+    // ---- chain ----
+    const int half = (warp - S::kWorkers - 1) >> 1, odd = (warp - S::kWorkers - 1) & 1;
+    if (!kChain && odd) return;
+    uint64_t h = 0;
+    for (int k = odd;; k += kChain ? 2 : 1) {
+      const int s = k % kStages;
+      const uint32_t parity = (k / kStages) & 1;
+      if (!__all_sync(0xffffffffu, wait_phase(smem_u32(&sh.full[s]), parity, &sh.broken))) return;
+      const Table<kRows> &tab = sh.tables[s];
+      const int64_t chunk = tab.chunk;
+      if (chunk < 0) return;
+      const bool last_chunk = tab.last, enters = !(tab.starts[0] & 1);
+      const int64_t lane_ch = static_cast<int64_t>(tab.d) * kCh + 64 * half + 2 * lane;
+      const int64_t row_ch = static_cast<int64_t>(nt) * kCh;
+      const int64_t group = chunk / kGroupLen;
+      const int before = static_cast<int>(chunk % kGroupLen);
+      if constexpr (kChain) {
+        h = 0;
+        if (enters) {
+          Map2 q{f2_dup(1.f), 0};
+          const uint64_t *src = p.maps + (chunk - before) * row_ch + lane_ch;
+#pragma unroll 1
+          for (int j0 = 0; j0 < before; j0 += 8) {
+            Words2 w[8];
+            fetch_words2<8>(src + j0 * row_ch, row_ch, min(before - j0, 8), w, &sh.broken);
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+              if (j0 + j < before) q = compose2(q, w[j].map());
+          }
+          if (group > 0) {
+            Words2 w[1];
+            fetch_words2<1>(p.states + (group - 1) * row_ch + lane_ch, 0, 1, w, &sh.broken);
+            h = w[0].map().H;
+          }
+          h = apply2(q, h);
+        }
+      }
+      if (!__all_sync(0xffffffffu, wait_phase(smem_u32(&sh.mapped[s][half]), parity, &sh.broken) &&
+                                       wait_phase(smem_u32(&sh.taken[s][half]), parity, &sh.broken)))
+        return;
+      float4 *own = &sh.own[s][half][0][lane];
+      Map2 m[kSlots];
+#pragma unroll
+      for (int i = 0; i < kSlots; ++i) m[i] = get_map2(own + 32 * i, 0);
+      const uint64_t h_in = h;
+#pragma unroll
+      for (int i = 0; i < kSlots; ++i) {
+        *reinterpret_cast<uint64_t *>(own + 32 * i) = h;
+        h = apply2(m[i], h);
+      }
+      if (kChain && !last_chunk && before == kGroupLen - 1) put_words2(p.states + group * row_ch + lane_ch, 0, h);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_u32(&sh.ready[s]));
+      if (p.carries != nullptr)
+        store2_f32<kVec>(p.carries + chunk * ((p.D + 127) / 128 * 128) + lane_ch - 2 * lane, lane, 64, h_in);
+    }
+  }
+
+  // ---- consumers ----
+  const int slot = warp / S::kHalves, half = warp % S::kHalves;
+  const int row0 = slot * kTokW;
+  unsigned char *const stage0 = smem + half * S::kHalfStage + row0 * (S::kPlaneBytes / kRows);
+  Params2 par{};
+  int s = 0, s1 = 0, turn = 0;         // stages of this tile and the one before; whose turn to publish
+  uint32_t parity = 0, parity1 = 0;    // ... and the phases of their barriers
+  for (int k = 0;; ++k) {
+    if (!__all_sync(0xffffffffu, wait_phase(smem_u32(&sh.full[s]), parity, &sh.broken))) return;
+    const Tile tile = sh.tiles[s];
+    if (tile.d >= 0) {
+      // first pass
+      const Table<kRows> &tab = sh.tables[s];
+      const int64_t c0 = static_cast<int64_t>(tile.d) * kCh + 64 * half;
+      if (kChain) {
+        par = Params2{load2_f32<kVec>(sh.params[s][0] + 64 * half, lane, 64),
+                      load2_f32<kVec>(sh.params[s][1] + 64 * half, lane, 64)};
+      } else if (k == 0) {
+        par = load_params2<kVec>(p.A_log + c0, p.dt_bias + c0, lane, static_cast<int>(min(p.D - c0, int64_t{64})));
+      }
+      unsigned char *const stage = stage0 + s * S::kStage;
+      int valid = kTokW;
+      unsigned starts = 0;
+      if (!tile.plain) {
+        valid = static_cast<int>(max(int64_t{0}, min(int64_t{kTokW}, tab.valid - row0)));
+        starts = mask_bits(tab.starts, row0, kTokW);
+      }
+      Raw2<E> raw[3][kTokW];
+      if constexpr (kTma) {
+#pragma unroll
+        for (int w = 0; w < 3; ++w)
+#pragma unroll
+          for (int i = 0; i < kTokW; ++i)
+            raw[w][i].v =
+                reinterpret_cast<const decltype(Raw2<E>::v) *>(stage + w * S::kPlane + i * 64 * sizeof(E))[lane];
+        __syncwarp();  // the warp's rows are overwritten from here on
+      } else {
+        const int64_t t0 = tab.chunk * kRows + row0;
+        const int left = static_cast<int>(min(p.D - c0, int64_t{64}));
+#pragma unroll
+        for (int i = 0; i < kTokW; ++i) {
+          raw[0][i].v = raw[1][i].v = raw[2][i].v = {};
+          if (i < valid) {
+            raw[0][i] = load2<E, kVec>(static_cast<const E *>(p.x) + (t0 + i) * p.x_stride + c0, lane, left);
+            raw[1][i] = load2<E, kVec>(static_cast<const E *>(p.a) + (t0 + i) * p.a_stride + c0, lane, left);
+            raw[2][i] = load2<E, kVec>(static_cast<const E *>(p.b) + (t0 + i) * p.b_stride + c0, lane, left);
+          }
+        }
+      }
+      if constexpr (kPack) {
+        // the groups' largest magnitudes: each half by one warp, joined through shared memory
+        uint32_t *amax = sh.amax + (k & 1) * kRows * 6 + row0 * 6;
+#pragma unroll
+        for (int w = 0; w < 3; ++w)
+#pragma unroll
+          for (int i = 0; i < kTokW; ++i) {
+            const uint64_t v = raw[w][i].pair();
+            const uint32_t m = __reduce_max_sync(0xffffffffu, abs_max_bits(v, v));
+            if (lane == 0) amax[(i * 3 + w) * 2 + half] = m;
+          }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&sh.pair[slot]));
+        if (!__all_sync(0xffffffffu, wait_phase(smem_u32(&sh.pair[slot]), k & 1, &sh.broken))) return;
+        const int64_t t0 = tab.chunk * kRows + row0;
+        const int left = static_cast<int>(min(p.D - c0, int64_t{64}));
+#pragma unroll
+        for (int w = 0; w < 3; ++w)
+#pragma unroll
+          for (int i = 0; i < kTokW; ++i) {
+            const uint32_t *m = amax + (i * 3 + w) * 2;
+            const uint32_t ex = group_exponent(max(m[0], m[1]), exp_cap<E>());
+            const uint64_t v = raw[w][i].pair();
+            const uint32_t q = quantise4(v, v, ex, exp_cap<E>());
+            if (i < valid) {
+              const int64_t t = w * p.s.T + t0 + i;
+              uint8_t *dst = p.packed + t * p.D + c0;
+              if constexpr (kVec) {
+                if (2 * lane < left) reinterpret_cast<uint16_t *>(dst)[lane] = static_cast<uint16_t>(q);
+              } else {
+                if (lane < left) dst[lane] = static_cast<uint8_t>(q);
+                if (lane + 32 < left) dst[lane + 32] = static_cast<uint8_t>(q >> 8);
+              }
+              if (lane == 0 && half == 0) p.packed[3 * p.s.T * p.D + t * nt + tile.d] = static_cast<uint8_t>(ex);
+            }
+          }
+      }
+      auto keep = [&](int i, uint64_t y, uint64_t P) {
+        *reinterpret_cast<ulonglong2 *>(stage + i / S::kPerPlane * S::kPlaneBytes + i % S::kPerPlane * 512 +
+                                        lane * 16) = make_ulonglong2(y, P);
+      };
+      uint64_t P = f2_dup(1.f), y = 0;
+      if (starts == 0 && valid == kTokW) {
+#pragma unroll
+        for (int i = 0; i < kTokW; ++i) {
+          uint64_t g, u;
+          gate_pair(raw[0][i].pair(), raw[1][i].pair(), raw[2][i].pair(), par.dt, par.c, g, u);
+          P = f2_mul(P, g);
+          y = f2_fma(g, y, u);
+          keep(i, y, P);
+        }
+      } else {
+#pragma unroll 1
+        for (int i = 0; i < kTokW; ++i) {
+          Raw2<E> r[3] = {raw[0][0], raw[1][0], raw[2][0]};
+#pragma unroll
+          for (int j = 1; j < kTokW; ++j)
+            if (i == j) r[0] = raw[0][j], r[1] = raw[1][j], r[2] = raw[2][j];
+          uint64_t g, u;
+          gate_pair(r[0].pair(), r[1].pair(), r[2].pair(), par.dt, par.c, g, u);
+          if (i >= valid) g = f2_dup(1.f), u = 0;
+          if ((starts >> i) & 1) {  // y is the state itself from here on
+            y = p.state != nullptr
+                    ? load2_f32<kVec>(p.state + p.s.row(tab.start[row0 + i]) * p.D + c0, lane,
+                                      static_cast<int>(min(p.D - c0, int64_t{64})))
+                    : 0;
+            P = f2_dup(-1.f);
+          }
+          P = f2_mul(P, g);
+          y = f2_fma(g, y, u);
+          keep(i, y, P);
+        }
+      }
+      put_map2(&sh.own[s][half][slot][0], lane, Map2{P, y});
+      __syncwarp();
+      const uint32_t mapped = smem_u32(&sh.mapped[s][half]);
+      if (lane == 0) mbar_arrive(mapped);
+      if (slot == turn) {
+        // the tile's map is published by the consumers, each warp in its turn,
+        // so that it does not wait for the look-back of the tile before
+        if (kChain && !tab.last && tab.chunk % kGroupLen != kGroupLen - 1) {
+          if (!__all_sync(0xffffffffu, wait_phase(mapped, parity, &sh.broken))) return;
+          Map2 all = get_map2(&sh.own[s][half][0][0], lane);
+#pragma unroll
+          for (int i = 1; i < kSlots; ++i) all = compose2(all, get_map2(&sh.own[s][half][i][0], lane));
+          put_words2(p.maps + (tab.chunk * nt + tile.d) * kCh + 64 * half + 2 * lane, all.A, all.H);
+          __syncwarp();
+        }
+        if (lane == 0) mbar_arrive(smem_u32(&sh.taken[s][half]));
+      }
+      turn = turn + 1 == kSlots ? 0 : turn + 1;
+    }
+    if (k > 0) {
+      // second pass, over the tile before
+      if (!__all_sync(0xffffffffu, wait_phase(smem_u32(&sh.ready[s1]), parity1, &sh.broken))) return;
+      const unsigned char *const src = stage0 + s1 * S::kStage + lane * 16;
+      const uint64_t h = *reinterpret_cast<const uint64_t *>(&sh.own[s1][half][slot][lane]);
+      auto kept = [&](int i) {
+        return *reinterpret_cast<const ulonglong2 *>(src + i / S::kPerPlane * S::kPlaneBytes + i % S::kPerPlane * 512);
+      };
+      const Tile before = sh.tiles[s1];
+      E *out = static_cast<E *>(p.out) + before.at + row0 * p.D + 64 * half;
+      if (before.plain) {
+#pragma unroll
+        for (int i = 0; i < kTokW; ++i) {
+          const ulonglong2 v = kept(i);
+          store2<E, kVec>(out, lane, 64, f2_fma(v.y, h, v.x));
+          out += p.D;
+        }
+      } else {
+        const Table<kRows> &tab = sh.tables[s1];
+        const int64_t c0 = static_cast<int64_t>(before.d) * kCh + 64 * half;
+        const int left = static_cast<int>(min(p.D - c0, int64_t{64}));
+        const int valid = static_cast<int>(max(int64_t{0}, min(int64_t{kTokW}, tab.valid - row0)));
+        const unsigned starts = mask_bits(tab.starts, row0, kTokW), ends = mask_bits(tab.ends, row0, kTokW);
+        const int first = starts ? __ffs(starts) - 1 : kTokW;
+#pragma unroll
+        for (int i = 0; i < kTokW; ++i) {
+          const ulonglong2 v = kept(i);
+          const uint64_t r = i < first ? f2_fma(v.y, h, v.x) : v.x;
+          if (p.out != nullptr && i < valid) store2<E, kVec>(out + i * p.D, lane, left, r);
+          if (((ends >> i) & 1) && p.final != nullptr)
+            store2_f32<kVec>(p.final + p.s.row(tab.end[row0 + i]) * p.D + c0, lane, left, r);
+        }
+      }
+      if (kTma) fence_async_smem();  // this stage was written here; the next copy into it comes after
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_u32(&sh.empty[s1]));
+    }
+    if (tile.d < 0) return;
+    s1 = s;
+    parity1 = parity;
+    if (++s == kStages) s = 0, parity ^= 1;
+  }
+}
+
+// ---- launch ---------------------------------------------------------------------
+template <typename E>
+bool make_row_map(CUtensorMap *m, const void *base, int64_t channels, int64_t rows, int64_t stride, int box_x,
+                  int box_y) {
+  PFN_cuTensorMapEncodeTiled_v12000 enc = tensor_map_encoder();
+  if (enc == nullptr) return false;
+  const cuuint64_t dims[2] = {static_cast<cuuint64_t>(channels), static_cast<cuuint64_t>(rows)};
+  const cuuint64_t strides[1] = {static_cast<cuuint64_t>(stride) * sizeof(E)};
+  const cuuint32_t box[2] = {static_cast<cuuint32_t>(box_x), static_cast<cuuint32_t>(box_y)};
+  const cuuint32_t estr[2] = {1, 1};
+  const CUtensorMapDataType type = std::is_same<E, float>::value     ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                                   : std::is_same<E, __half>::value  ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                                   : std::is_same<E, uint8_t>::value ? CU_TENSOR_MAP_DATA_TYPE_UINT8
+                                                                     : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+  return enc(m, type, 2, const_cast<void *>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+             CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// The workspace: header, prepared parameters and first sequences, words (as
+// many as the widest tiles need).
+struct Places {
+  float *dt, *c;
+  int *first;
+  uint64_t *words;
+  size_t bytes;
+};
+inline int64_t tiles_of(int64_t D) { return (D + 127) / 128; }
+inline int64_t chunks_of(int64_t T) { return T > 0 ? (T + kRows - 1) / kRows : 1; }
+inline Places places(void *workspace, int64_t T, int64_t D) {
+  const int64_t width = tiles_of(D) * 128, chunks = chunks_of(T);
+  const size_t first = sizeof(Header) + 8 * width, words = first + (4 * (chunks + 1) + 15) / 16 * 16;
+  char *w = static_cast<char *>(workspace);
+  return Places{reinterpret_cast<float *>(w + sizeof(Header)), reinterpret_cast<float *>(w + sizeof(Header) + 4 * width),
+                reinterpret_cast<int *>(w + first), reinterpret_cast<uint64_t *>(w + words),
+                words + 8 * (chunks + (chunks + kGroupLen - 1) / kGroupLen) * width};
+}
+
+// Inputs of up to this many chunks are walked by one CTA per 64 or 128 channels.
+constexpr int64_t kSerialChunks = 4;
+constexpr int64_t kSerialSeqs = 1024;  // each CTA checks all of cu_seqlens then
+
+template <typename E, bool kTma, bool kPack>
+cudaError_t launch_forward_t(Forward p, void *workspace, int sms, cudaStream_t stream) {
+  using S = FwdShape<E, kTma, kPack>;
+  const int64_t nt = (p.D + S::kCh - 1) / S::kCh, chunks = (max(p.s.T, int64_t{1}) - 1) / kRows + 1;
+  constexpr int smem = S::kStages * S::kStage + static_cast<int>(sizeof(FwdShared<S, kPack>));
+  static_assert(smem * S::kCtas <= 227 * 1024 - 1024 * (S::kCtas - 1), "CTAs of an SM share 228 KiB");
+  if constexpr (kTma) {
+    if (!make_row_map<E>(&p.tx, p.x, p.D, p.s.T, p.x_stride, 64, kRows) ||
+        !make_row_map<E>(&p.ta, p.a, p.D, p.s.T, p.a_stride, 64, kRows) ||
+        !make_row_map<E>(&p.tb, p.b, p.D, p.s.T, p.b_stride, 64, kRows))
+      return cudaErrorInvalidValue;
+  }
+  const bool serial = chunks <= kSerialChunks && (p.s.cu == nullptr || p.s.N <= kSerialSeqs);
+  auto kernel = serial ? recurrence_forward_kernel<E, kTma, kPack, false>
+                       : recurrence_forward_kernel<E, kTma, kPack, true>;
+  if (cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem)) return e;
+  int64_t blocks = nt;
+  if (!serial) {
+    p.hdr = static_cast<Header *>(workspace);
+    const Places w = places(workspace, p.s.T, p.D);
+    p.maps = w.words;
+    p.states = p.maps + chunks * nt * S::kCh;
+    p.dt = w.dt, p.c = w.c;
+    p.first = p.s.cu != nullptr ? w.first : nullptr;
+    const int64_t words = (chunks + (chunks + kGroupLen - 1) / kGroupLen) * nt * S::kCh;
+    const Prepared q{p.A_log, p.dt_bias, w.dt, w.c, p.D, p.s.cu != nullptr ? w.first : nullptr, chunks, kRows};
+    if (cudaError_t e = launch_init(p.hdr, p.maps, words, p.s, q, stream)) return e;
+    blocks = min(chunks * nt, int64_t{sms} * S::kCtas);
+  }
+  kernel<<<static_cast<unsigned>(blocks), S::kThreads, smem, stream>>>(p);
+  return cudaGetLastError();
+}
+
+template <typename E>
+cudaError_t launch_forward_e(const Forward &p, bool tma, void *workspace, int sms, cudaStream_t stream) {
+  if (p.packed != nullptr)
+    return tma ? launch_forward_t<E, true, true>(p, workspace, sms, stream)
+               : launch_forward_t<E, false, true>(p, workspace, sms, stream);
+  return tma ? launch_forward_t<E, true, false>(p, workspace, sms, stream)
+             : launch_forward_t<E, false, false>(p, workspace, sms, stream);
+}
+
+}  // namespace rec
+}  // namespace gdn

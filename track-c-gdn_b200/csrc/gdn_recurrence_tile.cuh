@@ -1,0 +1,342 @@
+// gdn_recurrence_tile.cuh -- what the recurrence's forward and backward share
+// beyond the arithmetic: sequences and their tables of starts and ends, pairs of
+// channels, affine maps, and the words that chunks hand to one another.
+#pragma once
+#include <type_traits>
+
+#include "gdn_recurrence.cuh"
+
+namespace gdn {
+namespace rec {
+
+constexpr int kGroupLen = 8;  // chunks joined through one published state
+
+// Sequences that start or end in a tile.
+template <int kRows>
+struct Table {
+  int64_t chunk;  // -1: no more tiles
+  int64_t valid;  // rows of the tile that belong to a sequence
+  int d;
+  int last;       // the last chunk
+  uint32_t starts[kRows / 32], ends[kRows / 32];
+  int start[kRows], end[kRows];  // the sequence, or -1
+};
+
+struct Seqs {
+  const int64_t *cu;  // [N + 1], or null: N sequences of S tokens each
+  int64_t N, T, S;
+  const int32_t *slots;  // state row of a sequence, or null: its number
+  int64_t pool;
+  __device__ __forceinline__ int64_t at(int64_t n) const { return cu != nullptr ? cu[n] : n * S; }
+  __device__ __forceinline__ int64_t row(int64_t n) const { return slots != nullptr ? slots[n] : n; }
+  __device__ __forceinline__ int64_t total() const { return cu != nullptr ? cu[N] : T; }
+};
+
+struct Header {
+  uint32_t ticket;
+  uint32_t bad;  // cu_seqlens or slots are not valid: write nothing
+  uint32_t pad[254];
+};
+static_assert(sizeof(Header) == 1024, "words start 1024 bytes into the workspace");
+
+// Checks cu_seqlens and slots with all threads of a CTA; returns the device
+// status code of what is wrong, or 0.
+__device__ __forceinline__ int check_seqs(const Seqs &s) {
+  int bad_cu = 0, bad_slot = 0;
+  if (s.cu != nullptr) {
+    if (threadIdx.x == 0) bad_cu = s.cu[0] != 0 || s.cu[s.N] > s.T;
+    for (int64_t n = threadIdx.x; n < s.N; n += blockDim.x) bad_cu |= s.cu[n] > s.cu[n + 1];
+  }
+  if (s.slots != nullptr)
+    for (int64_t n = threadIdx.x; n < s.N; n += blockDim.x)
+      bad_slot |= s.slots[n] < 0 || s.slots[n] >= s.pool;
+  bad_cu = __syncthreads_or(bad_cu);
+  bad_slot = __syncthreads_or(bad_slot);
+  return bad_cu ? kDevStatusBadSeqlens : bad_slot ? kDevStatusBadSlot : 0;
+}
+
+// What the init kernel prepares besides: dt_bias and -exp(A_log) log2(e) of all
+// channels (zeros up to a multiple of 128), and the first sequence that starts
+// at or behind each chunk's first row.
+struct Prepared {
+  const float *A_log, *dt_bias;
+  float *dt, *c;    // [D up to 128s] each
+  int64_t D;
+  int *first;       // [chunks + 1], or null
+  int64_t chunks, rows;
+};
+
+// Empties the words, prepares, and checks the sequences, before the tiles run.
+__global__ void __launch_bounds__(1024) recurrence_init_kernel(Header *hdr, ulonglong2 *words, int64_t n,
+                                                               const Seqs s, const Prepared q) {
+  const ulonglong2 e = make_ulonglong2(kEmptyWord, kEmptyWord);
+  for (int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; i < n;
+       i += static_cast<int64_t>(gridDim.x) * blockDim.x)
+    words[i] = e;
+  const int64_t me = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x;
+  for (int64_t c = me; c < (q.D + 127) / 128 * 128; c += static_cast<int64_t>(gridDim.x) * blockDim.x) {
+    q.dt[c] = c < q.D ? q.dt_bias[c] : 0.f;
+    q.c[c] = c < q.D ? -expf(q.A_log[c]) * kLog2e : 0.f;
+  }
+  if (q.first != nullptr) {
+    // every block searches in cu_seqlens, which may be wrong: the searches stay
+    // in [0, N] whatever it holds
+    for (int64_t k = me; k <= q.chunks; k += static_cast<int64_t>(gridDim.x) * blockDim.x) {
+      int64_t lo = 0, hi = s.N;
+      while (lo < hi) {
+        const int64_t mid = (lo + hi) / 2;
+        if (s.cu[mid] < k * q.rows)
+          lo = mid + 1;
+        else
+          hi = mid;
+      }
+      q.first[k] = static_cast<int>(lo);
+    }
+  }
+  if (blockIdx.x == 0) {
+    const int code = check_seqs(s);
+    if (threadIdx.x == 0) {
+      hdr->ticket = 0;
+      hdr->bad = code != 0;
+      if (code) set_device_status(code);
+    }
+  }
+}
+
+// First n in [0, N] with at(n) >= v (N if none), by all lanes of a warp.
+__device__ __forceinline__ int64_t first_at_or_after(const Seqs &s, int64_t v, int lane) {
+  if (s.cu == nullptr) return s.S > 0 ? min((v + s.S - 1) / s.S, s.N) : 0;
+  int64_t lo = 0, hi = s.N;
+  while (lo < hi) {
+    const int64_t step = (hi - lo + 31) / 32, i = lo + (lane + 1) * step - 1;
+    const int64_t k = __popc(__ballot_sync(0xffffffffu, i < hi && s.cu[i] < v));
+    hi = min(hi, lo + (k + 1) * step - 1);
+    lo += k * step;
+  }
+  return lo;
+}
+
+// Fills the table of the rows [base, base + kRows) with one warp.  on_empty(n)
+// is called by the whole warp for each sequence without tokens that lies there
+// (the last chunk also has those behind the last token).
+// `first`: where the chunks' first sequences were prepared, else they are
+// searched for.
+template <int kRows, typename F>
+__device__ __forceinline__ void fill_table(const Seqs &s, Table<kRows> &t, int64_t base, bool last, int lane,
+                                           const int *first, F on_empty) {
+#pragma unroll
+  for (int i = 0; i < kRows; i += 32) t.start[i + lane] = t.end[i + lane] = -1;
+  const int64_t lo = first != nullptr ? first[base / kRows] : first_at_or_after(s, base, lane);
+  const int64_t hi = last               ? s.N
+                     : first != nullptr ? first[base / kRows + 1]
+                                        : first_at_or_after(s, base + kRows, lane);
+  __syncwarp();
+  for (int64_t n0 = max(lo - 1, int64_t{0}); n0 < hi; n0 += 32) {
+    const int64_t n = n0 + lane;
+    bool empty = false;
+    if (n < hi) {
+      const int64_t from = s.at(n), to = s.at(n + 1);
+      empty = from == to && n >= lo;
+      if (from < to) {
+        if (from >= base && from < base + kRows) t.start[from - base] = static_cast<int>(n);
+        if (to > base && to <= base + kRows) t.end[to - 1 - base] = static_cast<int>(n);
+      }
+    }
+    unsigned m = __ballot_sync(0xffffffffu, empty);
+    while (m) {
+      on_empty(n0 + __ffs(m) - 1);
+      m &= m - 1;
+    }
+  }
+  __syncwarp();
+#pragma unroll
+  for (int i = 0; i < kRows / 32; ++i) {
+    const unsigned a = __ballot_sync(0xffffffffu, t.start[i * 32 + lane] >= 0);
+    const unsigned b = __ballot_sync(0xffffffffu, t.end[i * 32 + lane] >= 0);
+    if (lane == 0) t.starts[i] = a, t.ends[i] = b;
+  }
+}
+// the bits of rows [row, row + n) of a table's mask, n <= 16 and within one word
+__device__ __forceinline__ unsigned mask_bits(const uint32_t *words, int row, int n) {
+  return (words[row >> 5] >> (row & 31)) & ((1u << n) - 1u);
+}
+
+inline cudaError_t launch_init(Header *hdr, uint64_t *words, int64_t n, const Seqs &s, const Prepared &q,
+                               cudaStream_t stream) {
+  const int64_t blocks = min(int64_t{148 * 2}, (n / 2 + 1023) / 1024);
+  recurrence_init_kernel<<<static_cast<unsigned>(max(blocks, int64_t{1})), 1024, 0, stream>>>(
+      hdr, reinterpret_cast<ulonglong2 *>(words), n / 2, s, q);
+  return cudaGetLastError();
+}
+
+// ---- two channels of a lane -----------------------------------------------------
+// With kVec neighbours (one access), else lane and lane + 32 of 64 channels.
+template <typename E>
+struct Raw2;
+template <>
+struct Raw2<__nv_bfloat16> {
+  uint32_t v;
+  __device__ __forceinline__ uint64_t pair() const { return f2_pack(bf16_lo(v), bf16_hi(v)); }
+};
+template <>
+struct Raw2<__half> {
+  uint32_t v;
+  __device__ __forceinline__ uint64_t pair() const {
+    const float2 a = __half22float2(*reinterpret_cast<const __half2 *>(&v));
+    return f2_pack(a.x, a.y);
+  }
+};
+template <>
+struct Raw2<float> {
+  float2 v;
+  __device__ __forceinline__ uint64_t pair() const { return f2_pack(v.x, v.y); }
+};
+
+template <typename E, bool kVec>
+__device__ __forceinline__ Raw2<E> load2(const E *p, int lane, int left) {
+  Raw2<E> r;
+  r.v = {};
+  if constexpr (kVec) {
+    if (2 * lane < left) r.v = __ldg(reinterpret_cast<const decltype(r.v) *>(p) + lane);
+  } else {
+    E e[2] = {E(0.f), E(0.f)};
+    if (lane < left) e[0] = p[lane];
+    if (lane + 32 < left) e[1] = p[lane + 32];
+    memcpy(&r.v, e, sizeof(r.v));
+  }
+  return r;
+}
+template <typename E, bool kVec>
+__device__ __forceinline__ void store2(E *p, int lane, int left, uint64_t a) {
+  using V = decltype(Raw2<E>::v);
+  V v;
+  // the one rounding of a result: to nearest even
+  if constexpr (std::is_same<E, float>::value) {
+    v = make_float2(f2_lo(a), f2_hi(a));
+  } else if constexpr (std::is_same<E, __half>::value) {
+    const __half2 h = __floats2half2_rn(f2_lo(a), f2_hi(a));
+    v = *reinterpret_cast<const uint32_t *>(&h);
+  } else {
+    v = pack_bf16x2(f2_lo(a), f2_hi(a));
+  }
+  if constexpr (kVec) {
+    if (2 * lane < left) reinterpret_cast<V *>(p)[lane] = v;
+  } else {
+    E e[2];
+    memcpy(e, &v, sizeof(v));
+    if (lane < left) p[lane] = e[0];
+    if (lane + 32 < left) p[lane + 32] = e[1];
+  }
+}
+// fp32 rows (states, parameters); plain loads, since a state may be updated in place
+template <bool kVec>
+__device__ __forceinline__ uint64_t load2_f32(const float *p, int lane, int left) {
+  if constexpr (kVec) {
+    const float2 v = 2 * lane < left ? reinterpret_cast<const float2 *>(p)[lane] : make_float2(0.f, 0.f);
+    return f2_pack(v.x, v.y);
+  } else {
+    return f2_pack(lane < left ? p[lane] : 0.f, lane + 32 < left ? p[lane + 32] : 0.f);
+  }
+}
+template <bool kVec>
+__device__ __forceinline__ void store2_f32(float *p, int lane, int left, uint64_t a) {
+  if constexpr (kVec) {
+    if (2 * lane < left) reinterpret_cast<float2 *>(p)[lane] = make_float2(f2_lo(a), f2_hi(a));
+  } else {
+    if (lane < left) p[lane] = f2_lo(a);
+    if (lane + 32 < left) p[lane + 32] = f2_hi(a);
+  }
+}
+
+struct Params2 {
+  uint64_t dt, c;  // dt_bias; -exp(A_log) log2(e)
+};
+template <bool kVec>
+__device__ __forceinline__ Params2 load_params2(const float *A_log, const float *dt_bias, int lane, int left) {
+  const uint64_t a = load2_f32<kVec>(A_log, lane, left);
+  return Params2{load2_f32<kVec>(dt_bias, lane, left),
+                 f2_pack(-expf(f2_lo(a)) * kLog2e, -expf(f2_hi(a)) * kLog2e)};
+}
+
+// ---- affine maps of two channels ---------------------------------------------------
+struct Map2 {
+  uint64_t A, H;
+};
+__device__ __forceinline__ uint64_t apply2(const Map2 &m, uint64_t h) {
+  return f2_pack(apply(f2_lo(m.A), f2_lo(m.H), f2_lo(h)), apply(f2_hi(m.A), f2_hi(m.H), f2_hi(h)));
+}
+// `then` after `first`
+__device__ __forceinline__ Map2 compose2(const Map2 &first, const Map2 &then) {
+  const uint64_t A = f2_mul(then.A, first.A);
+  return Map2{f2_pack(restarts(f2_lo(then.A)) ? f2_lo(then.A) : f2_lo(A),
+                      restarts(f2_hi(then.A)) ? f2_hi(then.A) : f2_hi(A)),
+              apply2(then, first.H)};
+}
+// in shared memory, a lane's two side by side as (A, A, H, H)
+__device__ __forceinline__ void put_map2(float4 *row, int lane, const Map2 &m) {
+  row[lane] = make_float4(f2_lo(m.A), f2_hi(m.A), f2_lo(m.H), f2_hi(m.H));
+}
+__device__ __forceinline__ Map2 get_map2(const float4 *row, int lane) {
+  const float4 v = row[lane];
+  return Map2{f2_pack(v.x, v.y), f2_pack(v.z, v.w)};
+}
+
+// ---- words of two channels -----------------------------------------------------------
+__device__ __forceinline__ void put_words2(uint64_t *p, uint64_t lo, uint64_t hi) {
+  const uint64_t a = keep_apart(f2_pack(f2_lo(lo), f2_lo(hi))), b = keep_apart(f2_pack(f2_hi(lo), f2_hi(hi)));
+  asm volatile("st.relaxed.gpu.global.v2.b64 [%0], {%1, %2};" ::"l"(p), "l"(a), "l"(b) : "memory");
+}
+struct Words2 {
+  uint64_t a, b;
+  __device__ __forceinline__ bool there() const { return a != kEmptyWord && b != kEmptyWord; }
+  __device__ __forceinline__ Map2 map() const {
+    return Map2{f2_pack(f2_lo(a), f2_lo(b)), f2_pack(f2_hi(a), f2_hi(b))};
+  }
+};
+__device__ __forceinline__ Words2 try_words2(const uint64_t *p) {
+  Words2 w;
+  asm volatile("ld.relaxed.gpu.global.v2.b64 {%0, %1}, [%2];" : "=l"(w.a), "=l"(w.b) : "l"(p) : "memory");
+  return w;
+}
+// Fetches n <= 8 pairs of words, `stride` words apart, and waits (bounded) until
+// all lanes have theirs.  All that are missing are asked for again together:
+// one after the other each would cost a round trip to L2.  A wait that runs out
+// records device status 2 and goes on with zeros, as do all later waits of the
+// CTA.
+template <int kMost>
+__device__ __forceinline__ void fetch_words2(const uint64_t *src, int64_t stride, int n, Words2 (&w)[kMost],
+                                             volatile int *broken) {
+#pragma unroll
+  for (int j = 0; j < kMost; ++j) w[j] = j < n ? try_words2(src + j * stride) : Words2{0, 0};
+  const long long limit = wait_limit_cycles();
+  long long t0 = 0;
+  while (true) {
+    bool missing = false;
+#pragma unroll
+    for (int j = 0; j < kMost; ++j) missing |= !w[j].there();
+    if (!__any_sync(0xffffffffu, missing)) return;
+    if (t0 == 0) t0 = clock64();
+    if (__any_sync(0xffffffffu, *broken || clock64() - t0 > limit)) {
+      if (!*broken) set_device_status(kDevStatusWaitTimeout);
+      *broken = 1;
+#pragma unroll
+      for (int j = 0; j < kMost; ++j)
+        if (!w[j].there()) w[j] = Words2{0, 0};
+      return;
+    }
+#pragma unroll
+    for (int j = 0; j < kMost; ++j)
+      if (!w[j].there()) w[j] = try_words2(src + j * stride);
+  }
+}
+
+// Expects `bytes` more of asynchronous copies in the barrier's phase.
+__device__ __forceinline__ void mbar_expect_tx(uint32_t mbar, uint32_t bytes) {
+  asm volatile("mbarrier.expect_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(mbar), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void mbar_arrive(uint32_t mbar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(mbar) : "memory");
+}
+
+}  // namespace rec
+}  // namespace gdn
