@@ -8,10 +8,13 @@ evaluation, also of composed affine maps, is covered):
   exp by one base-2 exponential: its argument is rounded (a relative error of
     2 u in the argument is |argument| 2 u in the result) and it is accurate to
     2^-22 = 4 u
-  softplus: e = exp(-|z|) as above with z itself rounded once, the logarithm's
-    polynomial 3 u, sum 1 u; relative to softplus at most (3 |z| + 8) u
-  lg = -exp(A_log) softplus: exp(A_log) 4 u and two products: (3 |z| + 15) u
-  g = exp(lg): |lg| (3 |z| + 15) u + 4 u
+  w = (a + dt_bias) log2(e) as one fused a log2(e) + fl(dt_bias log2(e)): off by
+    log2(e) u (|a| + 2 |dt_bias| + |z|), which moves softplus by at most its
+    slope times that, and the slope is at most softplus itself
+  softplus: besides, the exponential 4 u, the logarithm's polynomial 3 u, sum 1 u:
+    (|a| + 2 |dt_bias| + |z| + 8) u
+  lg = -exp(A_log) softplus: exp(A_log) 4 u and two products: 15 for the 8
+  g = exp(lg): |lg| times lg's and 4 u
   sigmoid: (2 |b| + 8) u; u_t = sigmoid(b) x one more
   a state: the product and sum of its update, and as much again where maps
     are composed: 3 u of the sum's absolute parts
@@ -44,7 +47,8 @@ class Gates:
         self.g = self.lg.exp()
         self.beta = torch.sigmoid(b)
         self.u = self.beta * x
-        self.rel_lg = (3 * self.z.abs() + 15) * U
+        self.moved = a.abs() + 2 * dt_bias.double().abs() + self.z.abs()
+        self.rel_lg = (self.moved + 15) * U
         self.rel_g = self.lg.abs() * self.rel_lg + 4 * U
         self.rel_beta = (2 * b.abs() + 8) * U
         self.rel_u = self.rel_beta + U
@@ -133,7 +137,7 @@ def backward(x, state, A_log, a, dt_bias, b, cu, d_out, d_final, eight=False):
             R, mag = k.g[t] * v, k.g[t] * mag
         d_state[n], d_state_err[n] = R, r + 2 * U * mag
     sig = torch.sigmoid(k.z)
-    rel_sig = (3 * k.z.abs() + 10) * U
+    rel_sig = (k.moved + 10) * U
     slope = k.beta * (1 - k.beta)
     rel_slope = 2 * k.rel_beta + 2 * U
     dx = k.beta * dh

@@ -196,7 +196,7 @@ recurrence_backward_kernel(const __grid_constant__ Backward p) {
   const int nd = static_cast<int>((p.D + kTileCh - 1) / kTileCh);
   if (tid == 0) {
     sh.broken = 0;
-    sh.ticket = p.hdr->bad ? -1 : static_cast<int>(atomicAdd(&p.hdr->ticket, 1u));
+    sh.ticket = p.hdr->bad ? -1 : static_cast<int>(atomicAdd(&p.hdr->stream[0].ticket, 1u));
   }
   __syncthreads();
   if (sh.ticket < 0) return;
@@ -338,22 +338,20 @@ recurrence_backward_kernel(const __grid_constant__ Backward p) {
         const uint64_t dh = f2_add(o[i][k], R2[k]);
         R2[k] = f2_mul(g[i][k], dh);
         // beta and beta (1 - beta) from e = exp(-|b|): r = 1 / (1 + e), e r
-        const uint64_t eb = exp_neg_abs(b[k]), db1 = f2_add(eb, f2_dup(1.f));
+        const uint64_t eb = ex2_neg_abs(f2_mul(b[k], f2_dup(kLog2e))), db1 = f2_add(eb, f2_dup(1.f));
         const uint64_t rb = f2_pack(rcp(f2_lo(db1)), rcp(f2_hi(db1))), erb = f2_mul(eb, rb);
         const uint64_t beta = f2_pack(f2_lo(b[k]) >= 0.f ? f2_lo(rb) : f2_lo(erb),
                                       f2_hi(b[k]) >= 0.f ? f2_hi(rb) : f2_hi(erb));
         dx[k] = f2_mul(beta, dh);
         db[k] = f2_mul(f2_mul(x[k], dh), f2_mul(rb, erb));
-        const uint64_t z = f2_add(a[k], par.dt[k]), e = exp_neg_abs(z), d1 = f2_add(e, f2_dup(1.f));
+        const uint64_t z = f2_fma(a[k], f2_dup(kLog2e), par.dt[k]), e = ex2_neg_abs(z), d1 = f2_add(e, f2_dup(1.f));
         const uint64_t rz = f2_pack(rcp(f2_lo(d1)), rcp(f2_hi(d1))), erz = f2_mul(e, rz);
         const uint64_t sig = f2_pack(f2_lo(z) >= 0.f ? f2_lo(rz) : f2_lo(erz),
                                      f2_hi(z) >= 0.f ? f2_hi(rz) : f2_hi(erz));
-        // c dlg, with c = -exp(A_log) log2(e): ln 2 times it is -exp(A_log) dlg
-        const uint64_t cd = f2_mul(par.c[k], f2_mul(u[i][k], dh));
-        const uint64_t cdl = f2_mul(cd, f2_dup(kLn2));
-        da[k] = f2_mul(cdl, sig);
+        const uint64_t cd = f2_mul(par.c[k], f2_mul(u[i][k], dh));  // -exp(A_log) dlg
+        da[k] = f2_mul(cd, sig);
         sum_da[k] = f2_add(sum_da[k], da[k]);
-        sum_lg[k] = f2_fma(cdl, softplus_from(z, e), sum_lg[k]);
+        sum_lg[k] = f2_fma(cd, softplus2(z, e), sum_lg[k]);  // dlg lg log2(e)
       }
       const int64_t at = (t0 + i) * p.D + c0;
       store4<E, kVec>(static_cast<E *>(p.dx) + at, lane, left, dx[0], dx[1]);
@@ -364,6 +362,8 @@ recurrence_backward_kernel(const __grid_constant__ Backward p) {
                         make_float4(f2_lo(R2[0]), f2_hi(R2[0]), f2_lo(R2[1]), f2_hi(R2[1])));
     }
   }
+  sum_lg[0] = f2_mul(sum_lg[0], f2_dup(kLn2));
+  sum_lg[1] = f2_mul(sum_lg[1], f2_dup(kLn2));
   // the chunk's part of the parameters' gradients, over the warps in order
   __syncthreads();
   put_map(sh.own[warp], lane,
@@ -476,7 +476,7 @@ cudaError_t launch_backward_t(Backward p, void *workspace, float *dA_log, float 
   const Places w = places(workspace, p.s.T, p.D);
   p.chain.maps = w.words;
   p.chain.states = p.chain.maps + chunks_of(p.s.T) * nd * kTileCh;
-  const Prepared q{p.A_log, p.dt_bias, w.dt, w.c, p.D, nullptr, 0, kRows};
+  const Prepared q{p.A_log, p.dt_bias, w.dt, w.c, p.D, nullptr, chunks_of(p.s.T), kRows, 1};
   const int64_t words = (chunks_of(p.s.T) + (chunks_of(p.s.T) + kGroupLen - 1) / kGroupLen) * nd * kTileCh;
   if (cudaError_t e = launch_init(p.hdr, w.words, words, p.s, q, stream)) return e;
   recurrence_backward_kernel<E, kVec, kPacked>

@@ -161,43 +161,41 @@ __device__ __forceinline__ float rcp(float x) {
   return y;
 }
 
-// log1p(e) for e in [0, 1], both halves of a pair: e P(e) with the polynomial
-// P of degree 8 of least relative error (weighted least squares iterated to
-// the minimax, 3e-8; with its coefficients and steps in fp32 1.8e-7).  A
-// logarithm of 1 + e would lose the relative error where e is small, which is
-// where a gate remembers longest.
-__device__ __forceinline__ uint64_t log1p_poly(uint64_t e) {
-  uint64_t p = f2_dup(0.005232691299170256f);
-  p = f2_fma(p, e, f2_dup(-0.029505226761102676f));
-  p = f2_fma(p, e, f2_dup(0.07822593301534653f));
-  p = f2_fma(p, e, f2_dup(-0.13663244247436523f));
-  p = f2_fma(p, e, f2_dup(0.19106006622314453f));
-  p = f2_fma(p, e, f2_dup(-0.2484298199415207f));
-  p = f2_fma(p, e, f2_dup(0.3331909775733948f));
-  p = f2_fma(p, e, f2_dup(-0.4999949336051941f));
-  p = f2_fma(p, e, f2_dup(0.9999999403953552f));
-  return p;
-}
-
-// e = exp(-|z|) of both halves.
-__device__ __forceinline__ uint64_t exp_neg_abs(uint64_t z) {
-  return f2_pack(ex2(-kLog2e * fabsf(f2_lo(z))), ex2(-kLog2e * fabsf(f2_hi(z))));
-}
-// softplus(z) = max(z, 0) + log1p(exp(-|z|)), given e = exp(-|z|); NaN stays NaN (through e).
-__device__ __forceinline__ uint64_t softplus_from(uint64_t z, uint64_t e) {
-  return f2_fma(log1p_poly(e), e, f2_pack(fmaxf(f2_lo(z), 0.f), fmaxf(f2_hi(z), 0.f)));
-}
+// The gates are evaluated in base 2: with w = (a + dt_bias) log2(e) and
+// e = 2^-|w|, softplus(z) log2(e) = max(w, 0) + log2(1 + e), so that
+// g = 2^(-exp(A_log) softplus(z) log2(e)).
 __device__ __forceinline__ uint64_t ex2_pair(uint64_t x) { return f2_pack(ex2(f2_lo(x)), ex2(f2_hi(x))); }
+__device__ __forceinline__ uint64_t ex2_neg_abs(uint64_t x) {
+  return f2_pack(ex2(-fabsf(f2_lo(x))), ex2(-fabsf(f2_hi(x))));
+}
+// log2(1 + e) for e in [0, 1], added to max(w, 0): e Q(e), with the polynomial Q
+// of degree 8 of least relative error for log1p(e) / e (weighted least squares
+// iterated to the minimax, 3e-8; 1.8e-7 with its coefficients and steps in
+// fp32), times log2(e).  A logarithm of 1 + e would lose the relative error
+// where e is small, which is where a gate remembers longest.  NaN stays NaN
+// (through e).
+__device__ __forceinline__ uint64_t softplus2(uint64_t w, uint64_t e) {
+  uint64_t q = f2_dup(0.00754917785525322f);
+  q = f2_fma(q, e, f2_dup(-0.042567044496536255f));
+  q = f2_fma(q, e, f2_dup(0.11285616457462311f));
+  q = f2_fma(q, e, f2_dup(-0.19711895287036896f));
+  q = f2_fma(q, e, f2_dup(0.27564141154289246f));
+  q = f2_fma(q, e, f2_dup(-0.35840848088264465f));
+  q = f2_fma(q, e, f2_dup(0.480692982673645f));
+  q = f2_fma(q, e, f2_dup(-0.7213402390480042f));
+  q = f2_fma(q, e, f2_dup(1.442694902420044f));
+  return f2_fma(q, e, f2_pack(fmaxf(f2_lo(w), 0.f), fmaxf(f2_hi(w), 0.f)));
+}
 
 // 1 / (1 + exp(-b)): exp(-b) may be infinite, its reciprocal is then 0.
 __device__ __forceinline__ uint64_t sigmoid_pair(uint64_t b) {
-  const uint64_t e = ex2_pair(f2_mul(b, f2_dup(-kLog2e)));
-  const uint64_t d = f2_add(e, f2_dup(1.f));
+  const uint64_t d = f2_add(ex2_pair(f2_mul(b, f2_dup(-kLog2e))), f2_dup(1.f));
   return f2_pack(rcp(f2_lo(d)), rcp(f2_hi(d)));
 }
 
-// Per-lane channel constants: dt_bias, and c = -exp(A_log) log2(e), so that
-// g = 2^(c softplus(z)).
+// A channel's constants: dt = dt_bias log2(e), c = -exp(A_log).
+__device__ __forceinline__ float param_dt(float dt_bias) { return dt_bias * kLog2e; }
+__device__ __forceinline__ float param_c(float A_log) { return -expf(A_log); }
 struct Params {
   uint64_t dt[2], c[2];
 };
@@ -205,18 +203,18 @@ template <bool kVec>
 __device__ __forceinline__ Params load_params(const float *A_log, const float *dt_bias, int lane, int left) {
   const float4 a = load_f32<kVec>(A_log, lane, left), d = load_f32<kVec>(dt_bias, lane, left);
   Params p;
-  p.dt[0] = f2_pack(d.x, d.y);
-  p.dt[1] = f2_pack(d.z, d.w);
-  p.c[0] = f2_pack(-expf(a.x) * kLog2e, -expf(a.y) * kLog2e);
-  p.c[1] = f2_pack(-expf(a.z) * kLog2e, -expf(a.w) * kLog2e);
+  p.dt[0] = f2_pack(param_dt(d.x), param_dt(d.y));
+  p.dt[1] = f2_pack(param_dt(d.z), param_dt(d.w));
+  p.c[0] = f2_pack(param_c(a.x), param_c(a.y));
+  p.c[1] = f2_pack(param_c(a.z), param_c(a.w));
   return p;
 }
 
 // g and u = sigmoid(b) x of one channel pair.
 __device__ __forceinline__ void gate_pair(uint64_t x, uint64_t a, uint64_t b, uint64_t dt, uint64_t c,
                                           uint64_t &g, uint64_t &u) {
-  const uint64_t z = f2_add(a, dt);
-  g = ex2_pair(f2_mul(c, softplus_from(z, exp_neg_abs(z))));
+  const uint64_t w = f2_fma(a, f2_dup(kLog2e), dt);
+  g = ex2_pair(f2_mul(c, softplus2(w, ex2_neg_abs(w))));
   u = f2_mul(sigmoid_pair(b), x);
 }
 

@@ -64,7 +64,7 @@ struct FwdShared {
   // maps of the slots' rows (A, A, H, H of a lane's channels); the chain warp
   // replaces them by the states that enter the slots
   float4 own[Shape::kStages][Shape::kHalves][kSlots][32];
-  float params[Shape::kStages][2][Shape::kCh];  // kChain: dt_bias and c of the tile's channels
+  float params[Shape::kStages][2][Shape::kCh];  // kChain: dt and c of the tile's channels
   Table<kRows> tables[Shape::kStages];
   Tile tiles[Shape::kStages];
   uint64_t full[Shape::kStages], ready[Shape::kStages], empty[Shape::kStages];
@@ -125,28 +125,48 @@ recurrence_forward_kernel(const __grid_constant__ Forward p) {
   __syncthreads();
   const int64_t total = p.s.total();
   const int64_t last = total > 0 ? (total - 1) / kRows : 0;
+  const int group_len = kChain ? p.hdr->group : 1;  // 1 or kGroupLen
+  uint64_t *const states = group_len == 1 ? p.maps : p.states;  // no maps are published then
 
   if (warp == S::kWorkers) {
     // ---- producer ----
-    const int64_t tiles = ((p.s.T > 0 ? p.s.T - 1 : 0) / kRows + 1) * nt;
     int64_t next = 0;  // !kChain: the next chunk
+    // kChain: the stream that tickets are taken from, and those left after it
+    int stream = 0, left_streams = 0;
+    Stream st{};
     uint32_t ticket = 0;
-    if (kChain && lane == 0) ticket = atomicAdd(&p.hdr->ticket, 1u);
+    if constexpr (kChain) {
+      left_streams = p.hdr->streams;
+      stream = blockIdx.x % left_streams;
+      st = p.hdr->stream[stream];
+      if (lane == 0) ticket = atomicAdd(&p.hdr->stream[stream].ticket, 1u);
+    }
     int k = 0, ends = 0;
     while (true) {
-      int64_t chunk;
+      int64_t chunk = -1;
       int d = blockIdx.x;
+      bool only_map = false;
       if constexpr (kChain) {
         const int64_t t = __shfl_sync(0xffffffffu, ticket, 0);
-        if (lane == 0 && t < tiles) ticket = atomicAdd(&p.hdr->ticket, 1u);  // the next one, early
-        chunk = t < tiles ? t / nt : -1;
-        d = static_cast<int>(t % nt);
+        if (left_streams > 0) {
+          const int64_t tiles = (st.to - st.from + st.only_map) * nt;
+          if (t < tiles) {
+            if (lane == 0) ticket = atomicAdd(&p.hdr->stream[stream].ticket, 1u);  // the next one, early
+            chunk = st.from - st.only_map + t / nt;
+            only_map = chunk < st.from;
+            d = static_cast<int>(t % nt);
+          } else if (--left_streams > 0) {
+            stream = stream + 1 == p.hdr->streams ? 0 : stream + 1;
+            st = p.hdr->stream[stream];
+            if (lane == 0) ticket = atomicAdd(&p.hdr->stream[stream].ticket, 1u);
+            continue;
+          }
+        }
       } else {
-        chunk = next * kRows < max(p.s.T, int64_t{1}) ? next : -1;
-        ++next;
+        if (next * kRows < max(p.s.T, int64_t{1})) chunk = next++;
       }
       const int64_t c0 = static_cast<int64_t>(d) * kCh, base = chunk * kRows;
-      if (chunk >= 0 && p.zero_behind) {
+      if (chunk >= 0 && p.zero_behind && !only_map) {
         for (int64_t t = max(base, total); t < min(base + kRows, p.s.T); ++t)
 #pragma unroll
           for (int w = 0; w < S::kHalves; ++w)
@@ -185,8 +205,8 @@ recurrence_forward_kernel(const __grid_constant__ Forward p) {
           tma_load_2d(dst + 2 * S::kPlane, &p.tb, x, y, full);
         }
       }
-      fill_table<kRows>(p.s, t, base, chunk == last, lane, kChain ? p.first : nullptr, [&](int64_t n) {
-        if (p.final == nullptr) return;  // an empty sequence's final state is its initial state
+      const bool inside = fill_table<kRows>(p.s, t, base, chunk == last, lane, kChain ? p.first : nullptr, [&](int64_t n) {
+        if (p.final == nullptr || only_map) return;  // an empty sequence's final state is its initial state
 #pragma unroll
         for (int w = 0; w < S::kHalves; ++w) {
           const int left = static_cast<int>(min(p.D - c0 - 64 * w, int64_t{64}));
@@ -199,10 +219,10 @@ recurrence_forward_kernel(const __grid_constant__ Forward p) {
         t.chunk = chunk;
         t.d = d;
         t.last = chunk == last;
+        t.only_map = only_map;
         t.valid = min(total - base, int64_t{kRows});
-        const bool edge = (t.starts[0] | t.starts[1] | t.ends[0] | t.ends[1]) != 0;
-        sh.tiles[s] = Tile{base * p.D + c0, d,
-                           !edge && base + kRows <= total && c0 + kCh <= p.D && p.out != nullptr};
+        const bool plain = inside && !only_map && base + kRows <= total && c0 + kCh <= p.D && p.out != nullptr;
+        sh.tiles[s] = Tile{base * p.D + c0, d, plain ? 1 : 0};
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(full);
@@ -230,11 +250,13 @@ recurrence_forward_kernel(const __grid_constant__ Forward p) {
       const bool last_chunk = tab.last, enters = !(tab.starts[0] & 1);
       const int64_t lane_ch = static_cast<int64_t>(tab.d) * kCh + 64 * half + 2 * lane;
       const int64_t row_ch = static_cast<int64_t>(nt) * kCh;
-      const int64_t group = chunk / kGroupLen;
-      const int before = static_cast<int>(chunk % kGroupLen);
+      const int64_t group = group_len == 1 ? chunk : chunk / kGroupLen;
+      const int place = group_len == 1 ? 0 : static_cast<int>(chunk % kGroupLen);
+      const bool from_state = tab.reach > place;  // the sequence started before the group did
+      const int before = from_state ? place : static_cast<int>(tab.reach);
       if constexpr (kChain) {
         h = 0;
-        if (enters) {
+        if (enters && !tab.only_map) {
           Map2 q{f2_dup(1.f), 0};
           const uint64_t *src = p.maps + (chunk - before) * row_ch + lane_ch;
 #pragma unroll 1
@@ -245,9 +267,9 @@ recurrence_forward_kernel(const __grid_constant__ Forward p) {
             for (int j = 0; j < 8; ++j)
               if (j0 + j < before) q = compose2(q, w[j].map());
           }
-          if (group > 0) {
+          if (from_state) {
             Words2 w[1];
-            fetch_words2<1>(p.states + (group - 1) * row_ch + lane_ch, 0, 1, w, &sh.broken);
+            fetch_words2<1>(states + (group - 1) * row_ch + lane_ch, 0, 1, w, &sh.broken);
             h = w[0].map().H;
           }
           h = apply2(q, h);
@@ -266,10 +288,11 @@ recurrence_forward_kernel(const __grid_constant__ Forward p) {
         *reinterpret_cast<uint64_t *>(own + 32 * i) = h;
         h = apply2(m[i], h);
       }
-      if (kChain && !last_chunk && before == kGroupLen - 1) put_words2(p.states + group * row_ch + lane_ch, 0, h);
+      if (kChain && !last_chunk && !tab.only_map && place == group_len - 1)
+        put_words2(states + group * row_ch + lane_ch, 0, h);
       __syncwarp();
       if (lane == 0) mbar_arrive(smem_u32(&sh.ready[s]));
-      if (p.carries != nullptr)
+      if (p.carries != nullptr && !tab.only_map)
         store2_f32<kVec>(p.carries + chunk * ((p.D + 127) / 128 * 128) + lane_ch - 2 * lane, lane, 64, h_in);
     }
   }
@@ -403,12 +426,17 @@ recurrence_forward_kernel(const __grid_constant__ Forward p) {
       if (slot == turn) {
         // the tile's map is published by the consumers, each warp in its turn,
         // so that it does not wait for the look-back of the tile before
-        if (kChain && !tab.last && tab.chunk % kGroupLen != kGroupLen - 1) {
+        const bool group_end = group_len == 1 || tab.chunk % kGroupLen == kGroupLen - 1;
+        if (kChain && !tab.last && (!group_end || tab.only_map)) {
           if (!__all_sync(0xffffffffu, wait_phase(mapped, parity, &sh.broken))) return;
           Map2 all = get_map2(&sh.own[s][half][0][0], lane);
 #pragma unroll
           for (int i = 1; i < kSlots; ++i) all = compose2(all, get_map2(&sh.own[s][half][i][0], lane));
-          put_words2(p.maps + (tab.chunk * nt + tile.d) * kCh + 64 * half + 2 * lane, all.A, all.H);
+          const int64_t at = tile.d * kCh + 64 * half + 2 * lane;
+          if (group_end)  // only_map: a sequence starts here, so the map is the state after it
+            put_words2(states + (group_len == 1 ? tab.chunk : tab.chunk / kGroupLen) * nt * kCh + at, 0, all.H);
+          else
+            put_words2(p.maps + tab.chunk * nt * kCh + at, all.A, all.H);
           __syncwarp();
         }
         if (lane == 0) mbar_arrive(smem_u32(&sh.taken[s][half]));
@@ -432,7 +460,7 @@ recurrence_forward_kernel(const __grid_constant__ Forward p) {
           store2<E, kVec>(out, lane, 64, f2_fma(v.y, h, v.x));
           out += p.D;
         }
-      } else {
+      } else if (!sh.tables[s1].only_map) {
         const Table<kRows> &tab = sh.tables[s1];
         const int64_t c0 = static_cast<int64_t>(before.d) * kCh + 64 * half;
         const int left = static_cast<int>(min(p.D - c0, int64_t{64}));
@@ -490,11 +518,17 @@ inline int64_t tiles_of(int64_t D) { return (D + 127) / 128; }
 inline int64_t chunks_of(int64_t T) { return T > 0 ? (T + kRows - 1) / kRows : 1; }
 inline Places places(void *workspace, int64_t T, int64_t D) {
   const int64_t width = tiles_of(D) * 128, chunks = chunks_of(T);
-  const size_t first = sizeof(Header) + 8 * width, words = first + (4 * (chunks + 1) + 15) / 16 * 16;
+  const size_t first = kHeaderBytes + 8 * width, words = first + (4 * (chunks + 1) + 15) / 16 * 16;
   char *w = static_cast<char *>(workspace);
-  return Places{reinterpret_cast<float *>(w + sizeof(Header)), reinterpret_cast<float *>(w + sizeof(Header) + 4 * width),
+  return Places{reinterpret_cast<float *>(w + kHeaderBytes), reinterpret_cast<float *>(w + kHeaderBytes + 4 * width),
                 reinterpret_cast<int *>(w + first), reinterpret_cast<uint64_t *>(w + words),
                 words + 8 * (chunks + (chunks + kGroupLen - 1) / kGroupLen) * width};
+}
+
+// Streams for nt tiles of channels on `ctas` CTAs: about as many CTAs to a stream
+// as it has tiles of channels, so that the chunk before is done or nearly so.
+inline int streams_for(int64_t nt, int64_t ctas) {
+  return static_cast<int>(max(int64_t{1}, min(int64_t{kStreams}, ctas / nt)));
 }
 
 // Inputs of up to this many chunks are walked by one CTA per 64 or 128 channels.
@@ -524,9 +558,10 @@ cudaError_t launch_forward_t(Forward p, void *workspace, int sms, cudaStream_t s
     p.maps = w.words;
     p.states = p.maps + chunks * nt * S::kCh;
     p.dt = w.dt, p.c = w.c;
-    p.first = p.s.cu != nullptr ? w.first : nullptr;
+    p.first = w.first;
     const int64_t words = (chunks + (chunks + kGroupLen - 1) / kGroupLen) * nt * S::kCh;
-    const Prepared q{p.A_log, p.dt_bias, w.dt, w.c, p.D, p.s.cu != nullptr ? w.first : nullptr, chunks, kRows};
+    const Prepared q{p.A_log,     p.dt_bias, w.dt,  w.c, p.D, w.first, chunks, kRows,
+                     streams_for(nt, int64_t{sms} * S::kCtas)};
     if (cudaError_t e = launch_init(p.hdr, p.maps, words, p.s, q, stream)) return e;
     blocks = min(chunks * nt, int64_t{sms} * S::kCtas);
   }

@@ -9,15 +9,22 @@
 namespace gdn {
 namespace rec {
 
-constexpr int kGroupLen = 8;  // chunks joined through one published state
+// Chunks joined through one published state: 8 where one sequence (or a few) has
+// to be worked on by all CTAs at once -- a state then travels one link of about
+// 0.75 us for 8 chunks (65536 x 1024 bf16: 185 us; groups of 4: 214, 16: 212,
+// 2: 380) -- and 1 where the streams leave about one chunk of each in work,
+// whose predecessor is done: then a state per chunk is all that is published.
+constexpr int kGroupLen = 8;
 
 // Sequences that start or end in a tile.
 template <int kRows>
 struct Table {
   int64_t chunk;  // -1: no more tiles
   int64_t valid;  // rows of the tile that belong to a sequence
+  int64_t reach;  // chunks between this one and where the sequence of its first row starts
   int d;
   int last;       // the last chunk
+  int only_map;   // nothing but the tile's map is wanted
   uint32_t starts[kRows / 32], ends[kRows / 32];
   int start[kRows], end[kRows];  // the sequence, or -1
 };
@@ -32,12 +39,27 @@ struct Seqs {
   __device__ __forceinline__ int64_t total() const { return cu != nullptr ? cu[N] : T; }
 };
 
-struct Header {
+// The chunks are worked on as up to kStreams streams side by side, each a run of
+// consecutive chunks that begins where a sequence does, so that a chunk's
+// predecessor has usually long been finished when its turn comes; one sequence
+// alone is one stream.  A stream's first chunk `from` may follow one in which
+// the sequence starts: that chunk belongs to the stream before, but its map is
+// needed at once, and is worked out once more by the stream (only_map).
+constexpr int kStreams = 32;
+struct Stream {
+  int64_t from, to;  // chunks [from, to)
   uint32_t ticket;
-  uint32_t bad;  // cu_seqlens or slots are not valid: write nothing
-  uint32_t pad[254];
+  int only_map;      // 1: the stream starts with the map of chunk from - 1
 };
-static_assert(sizeof(Header) == 1024, "words start 1024 bytes into the workspace");
+struct Header {
+  uint32_t bad;      // cu_seqlens or slots are not valid: write nothing
+  int streams;
+  int group;         // chunks joined through one published state
+  uint32_t pad;
+  Stream stream[kStreams];
+};
+static_assert(sizeof(Header) <= 1024, "what follows starts 1024 bytes into the workspace");
+constexpr size_t kHeaderBytes = 1024;
 
 // Checks cu_seqlens and slots with all threads of a CTA; returns the device
 // status code of what is wrong, or 0.
@@ -55,8 +77,22 @@ __device__ __forceinline__ int check_seqs(const Seqs &s) {
   return bad_cu ? kDevStatusBadSeqlens : bad_slot ? kDevStatusBadSlot : 0;
 }
 
-// What the init kernel prepares besides: dt_bias and -exp(A_log) log2(e) of all
-// channels (zeros up to a multiple of 128), and the first sequence that starts
+// First n in [0, N] with at(n) >= v (N if none), by one thread.  Stays in [0, N]
+// whatever cu_seqlens holds.
+__device__ __forceinline__ int64_t first_by_halves(const Seqs &s, int64_t v) {
+  if (s.cu == nullptr) return s.S > 0 ? min((v + s.S - 1) / s.S, s.N) : 0;
+  int64_t lo = 0, hi = s.N;
+  while (lo < hi) {
+    const int64_t mid = (lo + hi) / 2;
+    if (s.cu[mid] < v)
+      lo = mid + 1;
+    else
+      hi = mid;
+  }
+  return lo;
+}
+
+// What the init kernel prepares besides: the parameters of all channels (zeros up to a multiple of 128), and the first sequence that starts
 // at or behind each chunk's first row.
 struct Prepared {
   const float *A_log, *dt_bias;
@@ -64,6 +100,7 @@ struct Prepared {
   int64_t D;
   int *first;       // [chunks + 1], or null
   int64_t chunks, rows;
+  int streams;      // as many as wanted, at most kStreams
 };
 
 // Empties the words, prepares, and checks the sequences, before the tiles run.
@@ -75,28 +112,39 @@ __global__ void __launch_bounds__(1024) recurrence_init_kernel(Header *hdr, ulon
     words[i] = e;
   const int64_t me = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x;
   for (int64_t c = me; c < (q.D + 127) / 128 * 128; c += static_cast<int64_t>(gridDim.x) * blockDim.x) {
-    q.dt[c] = c < q.D ? q.dt_bias[c] : 0.f;
-    q.c[c] = c < q.D ? -expf(q.A_log[c]) * kLog2e : 0.f;
+    q.dt[c] = c < q.D ? param_dt(q.dt_bias[c]) : 0.f;
+    q.c[c] = c < q.D ? param_c(q.A_log[c]) : 0.f;
   }
   if (q.first != nullptr) {
-    // every block searches in cu_seqlens, which may be wrong: the searches stay
-    // in [0, N] whatever it holds
-    for (int64_t k = me; k <= q.chunks; k += static_cast<int64_t>(gridDim.x) * blockDim.x) {
-      int64_t lo = 0, hi = s.N;
-      while (lo < hi) {
-        const int64_t mid = (lo + hi) / 2;
-        if (s.cu[mid] < k * q.rows)
-          lo = mid + 1;
-        else
-          hi = mid;
-      }
-      q.first[k] = static_cast<int>(lo);
-    }
+    for (int64_t k = me; k <= q.chunks; k += static_cast<int64_t>(gridDim.x) * blockDim.x)
+      q.first[k] = static_cast<int>(first_by_halves(s, k * q.rows));
   }
   if (blockIdx.x == 0) {
     const int code = check_seqs(s);
-    if (threadIdx.x == 0) {
-      hdr->ticket = 0;
+    __shared__ int64_t from[kStreams];
+    __shared__ int only_map[kStreams];
+    const int i = threadIdx.x;
+    if (i < q.streams) {
+      // the first chunk that begins with a sequence's start or after it, from
+      // an even cut on
+      const int64_t n = first_by_halves(s, q.chunks * i / q.streams * q.rows);
+      from[i] = i == 0 ? 0 : n < s.N ? (s.at(n) + q.rows - 1) / q.rows : q.chunks;
+      // does the sequence of its first row start in the chunk before?
+      const int64_t row = from[i] * q.rows, m = first_by_halves(s, row);
+      only_map[i] = i > 0 && !(m < s.N && s.at(m) == row);
+    }
+    __syncthreads();
+    if (i == 0) {
+      int n = 1;
+      hdr->stream[0] = Stream{0, q.chunks, 0, 0};
+      for (int j = 1; j < q.streams; ++j)
+        if (from[j] > from[j - 1] && from[j] < q.chunks) {
+          hdr->stream[n - 1].to = from[j];
+          hdr->stream[n] = Stream{from[j], q.chunks, 0, only_map[j]};
+          ++n;
+        }
+      hdr->streams = n;
+      hdr->group = 2 * n > q.streams && q.streams > 1 ? 1 : kGroupLen;
       hdr->bad = code != 0;
       if (code) set_device_status(code);
     }
@@ -116,17 +164,23 @@ __device__ __forceinline__ int64_t first_at_or_after(const Seqs &s, int64_t v, i
   return lo;
 }
 
-// Fills the table of the rows [base, base + kRows) with one warp.  on_empty(n)
-// is called by the whole warp for each sequence without tokens that lies there
-// (the last chunk also has those behind the last token).
-// `first`: where the chunks' first sequences were prepared, else they are
-// searched for.
+// Fills the table of the rows [base, base + kRows) with one warp; returns whether
+// no sequence starts or ends there.  on_empty(n) is called by the whole warp for
+// each sequence without tokens that lies there (the last chunk also has those
+// behind the last token).  `first`: where the chunks' first sequences were
+// prepared, else they are searched for.
 template <int kRows, typename F>
-__device__ __forceinline__ void fill_table(const Seqs &s, Table<kRows> &t, int64_t base, bool last, int lane,
+__device__ __forceinline__ bool fill_table(const Seqs &s, Table<kRows> &t, int64_t base, bool last, int lane,
                                            const int *first, F on_empty) {
+  const int64_t lo = first != nullptr ? first[base / kRows] : first_at_or_after(s, base, lane);
+  // the sequence that covers the first row, if it does not start there
+  if (lane == 0) t.reach = lo > 0 ? base / kRows - s.at(lo - 1) / kRows : 0;
+  if (!last && s.at(lo) > base + kRows) {
+    if (lane < kRows / 32) t.starts[lane] = t.ends[lane] = 0;
+    return true;
+  }
 #pragma unroll
   for (int i = 0; i < kRows; i += 32) t.start[i + lane] = t.end[i + lane] = -1;
-  const int64_t lo = first != nullptr ? first[base / kRows] : first_at_or_after(s, base, lane);
   const int64_t hi = last               ? s.N
                      : first != nullptr ? first[base / kRows + 1]
                                         : first_at_or_after(s, base + kRows, lane);
@@ -155,6 +209,7 @@ __device__ __forceinline__ void fill_table(const Seqs &s, Table<kRows> &t, int64
     const unsigned b = __ballot_sync(0xffffffffu, t.end[i * 32 + lane] >= 0);
     if (lane == 0) t.starts[i] = a, t.ends[i] = b;
   }
+  return false;
 }
 // the bits of rows [row, row + n) of a table's mask, n <= 16 and within one word
 __device__ __forceinline__ unsigned mask_bits(const uint32_t *words, int row, int n) {
@@ -249,13 +304,12 @@ __device__ __forceinline__ void store2_f32(float *p, int lane, int left, uint64_
 }
 
 struct Params2 {
-  uint64_t dt, c;  // dt_bias; -exp(A_log) log2(e)
+  uint64_t dt, c;
 };
 template <bool kVec>
 __device__ __forceinline__ Params2 load_params2(const float *A_log, const float *dt_bias, int lane, int left) {
-  const uint64_t a = load2_f32<kVec>(A_log, lane, left);
-  return Params2{load2_f32<kVec>(dt_bias, lane, left),
-                 f2_pack(-expf(f2_lo(a)) * kLog2e, -expf(f2_hi(a)) * kLog2e)};
+  const uint64_t a = load2_f32<kVec>(A_log, lane, left), d = load2_f32<kVec>(dt_bias, lane, left);
+  return Params2{f2_pack(param_dt(f2_lo(d)), param_dt(f2_hi(d))), f2_pack(param_c(f2_lo(a)), param_c(f2_hi(a)))};
 }
 
 // ---- affine maps of two channels ---------------------------------------------------
