@@ -319,25 +319,22 @@ __device__ __forceinline__ float group_scale(uint32_t E) { return __uint_as_floa
 __device__ __forceinline__ float group_inverse(uint32_t E) {  // 2^(127 - E); 0 for a non-finite group
   return E == kExpNonFinite ? 0.f : __uint_as_float((254u - E) << 23);
 }
-// q of four values as four bytes.  v inv is exact and below 2^7 in magnitude
+// q of two (four) values as bytes.  v inv is exact and below 2^7 in magnitude
 // (2^7.01 in a capped group), so adding 1.5 2^23 rounds it to an integer, half
 // to even, in the sum's low byte.
-__device__ __forceinline__ uint32_t quantise4(uint64_t a, uint64_t b, uint32_t E, uint32_t cap) {
+__device__ __forceinline__ uint32_t quantise2(uint64_t a, uint32_t E, uint32_t cap) {
   if (E == kExpNonFinite) return 0u;  // 0 times infinity reads back as NaN
-  const uint64_t inv = f2_dup(group_inverse(E)), magic = f2_dup(12582912.f);
+  const uint64_t magic = f2_dup(12582912.f);
   if (E == cap) {
-    float f[4] = {f2_lo(a), f2_hi(a), f2_lo(b), f2_hi(b)};
-#pragma unroll
-    for (int j = 0; j < 4; ++j) f[j] = fminf(fmaxf(f[j] * group_inverse(E), -127.f), 127.f);
-    a = f2_add(f2_pack(f[0], f[1]), magic);
-    b = f2_add(f2_pack(f[2], f[3]), magic);
+    const float lim = 127.f, inv = group_inverse(E);
+    a = f2_add(f2_pack(fminf(fmaxf(f2_lo(a) * inv, -lim), lim), fminf(fmaxf(f2_hi(a) * inv, -lim), lim)), magic);
   } else {
-    a = f2_fma(a, inv, magic);
-    b = f2_fma(b, inv, magic);
+    a = f2_fma(a, f2_dup(group_inverse(E)), magic);
   }
-  const uint32_t lo = __byte_perm(static_cast<uint32_t>(a), static_cast<uint32_t>(a >> 32), 0x0040);
-  const uint32_t hi = __byte_perm(static_cast<uint32_t>(b), static_cast<uint32_t>(b >> 32), 0x0040);
-  return __byte_perm(lo, hi, 0x5410);
+  return __byte_perm(static_cast<uint32_t>(a), static_cast<uint32_t>(a >> 32), 0x0040);
+}
+__device__ __forceinline__ uint32_t quantise4(uint64_t a, uint64_t b, uint32_t E, uint32_t cap) {
+  return __byte_perm(quantise2(a, E, cap), quantise2(b, E, cap), 0x5410);
 }
 // The values that four bytes stand for.  A byte q + 128 put into the mantissa
 // of 2^23 is the fp32 number 2^23 + 128 + q: a byte permute and an addition

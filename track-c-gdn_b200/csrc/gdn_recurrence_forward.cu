@@ -71,7 +71,7 @@ struct FwdShared {
   uint64_t mapped[Shape::kStages][Shape::kHalves];  // the slots' maps are there
   uint64_t taken[Shape::kStages][Shape::kHalves];   // ... and have been read for the tile's
   uint64_t pair[kPack ? kSlots : 1];
-  uint32_t amax[kPack ? 2 * kRows * 3 * 2 : 1];
+  uint32_t amax[kPack ? 2 * kSlots * 64 : 1];
   int broken;
 };
 
@@ -254,42 +254,48 @@ recurrence_forward_kernel(const __grid_constant__ Forward p) {
       const int place = group_len == 1 ? 0 : static_cast<int>(chunk % kGroupLen);
       const bool from_state = tab.reach > place;  // the sequence started before the group did
       const int before = from_state ? place : static_cast<int>(tab.reach);
+      // the words that are wanted, asked for before the first pass is done: maps
+      // of the chunks before, and the state that enters the first of them
+      const bool looks = kChain && enters && !tab.only_map;
+      Words2 w[kGroupLen];
+      auto src = [&](int j) {
+        return j < kGroupLen - 1 ? p.maps + (chunk - before + j) * row_ch + lane_ch
+                                 : states + (group - 1) * row_ch + lane_ch;
+      };
       if constexpr (kChain) {
-        h = 0;
-        if (enters && !tab.only_map) {
-          Map2 q{f2_dup(1.f), 0};
-          const uint64_t *src = p.maps + (chunk - before) * row_ch + lane_ch;
-#pragma unroll 1
-          for (int j0 = 0; j0 < before; j0 += 8) {
-            Words2 w[8];
-            fetch_words2<8>(src + j0 * row_ch, row_ch, min(before - j0, 8), w, &sh.broken);
 #pragma unroll
-            for (int j = 0; j < 8; ++j)
-              if (j0 + j < before) q = compose2(q, w[j].map());
-          }
-          if (from_state) {
-            Words2 w[1];
-            fetch_words2<1>(states + (group - 1) * row_ch + lane_ch, 0, 1, w, &sh.broken);
-            h = w[0].map().H;
-          }
-          h = apply2(q, h);
-        }
+        for (int j = 0; j < kGroupLen; ++j)
+          w[j] = looks && (j < kGroupLen - 1 ? j < before : from_state) ? try_words2(src(j)) : Words2{0, 0};
       }
       if (!__all_sync(0xffffffffu, wait_phase(smem_u32(&sh.mapped[s][half]), parity, &sh.broken) &&
                                        wait_phase(smem_u32(&sh.taken[s][half]), parity, &sh.broken)))
         return;
       float4 *own = &sh.own[s][half][0][lane];
-      Map2 m[kSlots];
+      if constexpr (kChain) {
+        const bool publishes = !last_chunk && !tab.only_map && place == group_len - 1;
+        Map2 all = get_map2(own, 0);
+        if (publishes) {
 #pragma unroll
-      for (int i = 0; i < kSlots; ++i) m[i] = get_map2(own + 32 * i, 0);
+          for (int i = 1; i < kSlots; ++i) all = compose2(all, get_map2(own + 32 * i, 0));
+        }
+        h = 0;
+        if (looks) {
+          await_words2<kGroupLen>(w, src, &sh.broken);
+          if (from_state) h = w[kGroupLen - 1].map().H;
+#pragma unroll
+          for (int j = 0; j < kGroupLen - 1; ++j)
+            if (j < before) h = apply2(w[j].map(), h);
+        }
+        // first what others wait for
+        if (publishes) put_words2(states + group * row_ch + lane_ch, 0, apply2(all, h));
+      }
       const uint64_t h_in = h;
 #pragma unroll
       for (int i = 0; i < kSlots; ++i) {
+        const Map2 m = get_map2(own + 32 * i, 0);
         *reinterpret_cast<uint64_t *>(own + 32 * i) = h;
-        h = apply2(m[i], h);
+        h = apply2(m, h);
       }
-      if (kChain && !last_chunk && !tab.only_map && place == group_len - 1)
-        put_words2(states + group * row_ch + lane_ch, 0, h);
       __syncwarp();
       if (lane == 0) mbar_arrive(smem_u32(&sh.ready[s]));
       if (p.carries != nullptr && !tab.only_map)
@@ -347,41 +353,46 @@ recurrence_forward_kernel(const __grid_constant__ Forward p) {
         }
       }
       if constexpr (kPack) {
-        // the groups' largest magnitudes: each half by one warp, joined through shared memory
-        uint32_t *amax = sh.amax + (k & 1) * kRows * 6 + row0 * 6;
+        // The groups' largest magnitudes: each half by one warp, joined through
+        // shared memory.  Lane 8 w + i holds what belongs to row i of x, a or b.
+        uint32_t mine = 0;
 #pragma unroll
         for (int w = 0; w < 3; ++w)
 #pragma unroll
           for (int i = 0; i < kTokW; ++i) {
-            const uint64_t v = raw[w][i].pair();
-            const uint32_t m = __reduce_max_sync(0xffffffffu, abs_max_bits(v, v));
-            if (lane == 0) amax[(i * 3 + w) * 2 + half] = m;
+            const uint32_t m = __reduce_max_sync(0xffffffffu, raw[w][i].abs_max());
+            if (lane == kTokW * w + i) mine = m;
           }
+        uint32_t *amax = sh.amax + ((k & 1) * kSlots + slot) * 64;
+        amax[32 * half + lane] = mine;
         __syncwarp();
         if (lane == 0) mbar_arrive(smem_u32(&sh.pair[slot]));
         if (!__all_sync(0xffffffffu, wait_phase(smem_u32(&sh.pair[slot]), k & 1, &sh.broken))) return;
+        const uint32_t ex =
+            group_exponent(Raw2<E>::magnitude(max(mine, amax[32 * (half ^ 1) + lane])), exp_cap<E>());
         const int64_t t0 = tab.chunk * kRows + row0;
         const int left = static_cast<int>(min(p.D - c0, int64_t{64}));
+        if (half == 0 && lane < 3 * kTokW && lane % kTokW < valid)
+          p.packed[3 * p.s.T * p.D + (lane / kTokW * p.s.T + t0 + lane % kTokW) * nt + tile.d] =
+              static_cast<uint8_t>(ex);
 #pragma unroll
-        for (int w = 0; w < 3; ++w)
+        for (int w = 0; w < 3; ++w) {
+          uint8_t *dst = p.packed + (w * p.s.T + t0) * p.D + c0;
 #pragma unroll
           for (int i = 0; i < kTokW; ++i) {
-            const uint32_t *m = amax + (i * 3 + w) * 2;
-            const uint32_t ex = group_exponent(max(m[0], m[1]), exp_cap<E>());
             const uint64_t v = raw[w][i].pair();
-            const uint32_t q = quantise4(v, v, ex, exp_cap<E>());
+            const uint32_t q = quantise2(v, __shfl_sync(0xffffffffu, ex, kTokW * w + i), exp_cap<E>());
             if (i < valid) {
-              const int64_t t = w * p.s.T + t0 + i;
-              uint8_t *dst = p.packed + t * p.D + c0;
               if constexpr (kVec) {
                 if (2 * lane < left) reinterpret_cast<uint16_t *>(dst)[lane] = static_cast<uint16_t>(q);
               } else {
                 if (lane < left) dst[lane] = static_cast<uint8_t>(q);
                 if (lane + 32 < left) dst[lane + 32] = static_cast<uint8_t>(q >> 8);
               }
-              if (lane == 0 && half == 0) p.packed[3 * p.s.T * p.D + t * nt + tile.d] = static_cast<uint8_t>(ex);
             }
+            dst += p.D;
           }
+        }
       }
       auto keep = [&](int i, uint64_t y, uint64_t P) {
         *reinterpret_cast<ulonglong2 *>(stage + i / S::kPerPlane * S::kPlaneBytes + i % S::kPerPlane * 512 +

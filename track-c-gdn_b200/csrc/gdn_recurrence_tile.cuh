@@ -231,11 +231,19 @@ struct Raw2;
 template <>
 struct Raw2<__nv_bfloat16> {
   uint32_t v;
+  // the larger magnitude as bits whose order is that of the values, and those
+  // bits as an fp32's
+  __device__ __forceinline__ uint32_t abs_max() const { return max(v & 0x7fffu, (v >> 16) & 0x7fffu); }
+  __device__ static __forceinline__ uint32_t magnitude(uint32_t m) { return m << 16; }
   __device__ __forceinline__ uint64_t pair() const { return f2_pack(bf16_lo(v), bf16_hi(v)); }
 };
 template <>
 struct Raw2<__half> {
   uint32_t v;
+  __device__ __forceinline__ uint32_t abs_max() const { return max(v & 0x7fffu, (v >> 16) & 0x7fffu); }
+  __device__ static __forceinline__ uint32_t magnitude(uint32_t m) {
+    return __float_as_uint(__half2float(__ushort_as_half(static_cast<uint16_t>(m))));
+  }
   __device__ __forceinline__ uint64_t pair() const {
     const float2 a = __half22float2(*reinterpret_cast<const __half2 *>(&v));
     return f2_pack(a.x, a.y);
@@ -244,6 +252,10 @@ struct Raw2<__half> {
 template <>
 struct Raw2<float> {
   float2 v;
+  __device__ __forceinline__ uint32_t abs_max() const {
+    return max(__float_as_uint(v.x) & 0x7fffffffu, __float_as_uint(v.y) & 0x7fffffffu);
+  }
+  __device__ static __forceinline__ uint32_t magnitude(uint32_t m) { return m; }
   __device__ __forceinline__ uint64_t pair() const { return f2_pack(v.x, v.y); }
 };
 
@@ -352,16 +364,13 @@ __device__ __forceinline__ Words2 try_words2(const uint64_t *p) {
   asm volatile("ld.relaxed.gpu.global.v2.b64 {%0, %1}, [%2];" : "=l"(w.a), "=l"(w.b) : "l"(p) : "memory");
   return w;
 }
-// Fetches n <= 8 pairs of words, `stride` words apart, and waits (bounded) until
-// all lanes have theirs.  All that are missing are asked for again together:
-// one after the other each would cost a round trip to L2.  A wait that runs out
-// records device status 2 and goes on with zeros, as do all later waits of the
-// CTA.
-template <int kMost>
-__device__ __forceinline__ void fetch_words2(const uint64_t *src, int64_t stride, int n, Words2 (&w)[kMost],
-                                             volatile int *broken) {
-#pragma unroll
-  for (int j = 0; j < kMost; ++j) w[j] = j < n ? try_words2(src + j * stride) : Words2{0, 0};
+// Asks again for those of a lane's words that are wanted and missing, all at
+// once, until no lane of the warp misses any (bounded): one after the other each
+// would cost a round trip to L2.  `src` gives the address of word j.  A wait
+// that runs out records device status 2 and goes on with zeros, as do all later
+// waits of the CTA.
+template <int kMost, typename F>
+__device__ __forceinline__ void await_words2(Words2 (&w)[kMost], F src, volatile int *broken) {
   const long long limit = wait_limit_cycles();
   long long t0 = 0;
   while (true) {
@@ -380,7 +389,7 @@ __device__ __forceinline__ void fetch_words2(const uint64_t *src, int64_t stride
     }
 #pragma unroll
     for (int j = 0; j < kMost; ++j)
-      if (!w[j].there()) w[j] = try_words2(src + j * stride);
+      if (!w[j].there()) w[j] = try_words2(src(j));
   }
 }
 
