@@ -257,22 +257,31 @@ recurrence_forward_kernel(const __grid_constant__ Forward p) {
       // the words that are wanted, asked for before the first pass is done: maps
       // of the chunks before, and the state that enters the first of them
       const bool looks = kChain && enters && !tab.only_map;
+      const bool groups = kChain && group_len > 1;
       Words2 w[kGroupLen];
       auto src = [&](int j) {
-        return j < kGroupLen - 1 ? p.maps + (chunk - before + j) * row_ch + lane_ch
-                                 : states + (group - 1) * row_ch + lane_ch;
+        return j > 0 ? p.maps + (chunk - before + j - 1) * row_ch + lane_ch : states + (group - 1) * row_ch + lane_ch;
       };
       if constexpr (kChain) {
+        w[0] = looks && from_state ? try_words2(src(0)) : Words2{0, 0};
+        if (groups) {
 #pragma unroll
-        for (int j = 0; j < kGroupLen; ++j)
-          w[j] = looks && (j < kGroupLen - 1 ? j < before : from_state) ? try_words2(src(j)) : Words2{0, 0};
+          for (int j = 1; j < kGroupLen; ++j) w[j] = looks && j <= before ? try_words2(src(j)) : Words2{0, 0};
+        }
       }
       if (!__all_sync(0xffffffffu, wait_phase(smem_u32(&sh.mapped[s][half]), parity, &sh.broken) &&
                                        wait_phase(smem_u32(&sh.taken[s][half]), parity, &sh.broken)))
         return;
       float4 *own = &sh.own[s][half][0][lane];
-      if constexpr (kChain) {
-        const bool publishes = !last_chunk && !tab.only_map && place == group_len - 1;
+      const bool publishes = kChain && !last_chunk && !tab.only_map && place == group_len - 1;
+      if (kChain && !groups) {
+        h = 0;
+        if (looks && from_state) {
+          Words2 one[1] = {w[0]};
+          await_words2<1>(one, src, &sh.broken);
+          h = one[0].map().H;
+        }
+      } else if (kChain) {
         Map2 all = get_map2(own, 0);
         if (publishes) {
 #pragma unroll
@@ -281,10 +290,10 @@ recurrence_forward_kernel(const __grid_constant__ Forward p) {
         h = 0;
         if (looks) {
           await_words2<kGroupLen>(w, src, &sh.broken);
-          if (from_state) h = w[kGroupLen - 1].map().H;
+          if (from_state) h = w[0].map().H;
 #pragma unroll
-          for (int j = 0; j < kGroupLen - 1; ++j)
-            if (j < before) h = apply2(w[j].map(), h);
+          for (int j = 1; j < kGroupLen; ++j)
+            if (j <= before) h = apply2(w[j].map(), h);
         }
         // first what others wait for
         if (publishes) put_words2(states + group * row_ch + lane_ch, 0, apply2(all, h));
@@ -296,6 +305,7 @@ recurrence_forward_kernel(const __grid_constant__ Forward p) {
         *reinterpret_cast<uint64_t *>(own + 32 * i) = h;
         h = apply2(m, h);
       }
+      if (publishes && !groups) put_words2(states + group * row_ch + lane_ch, 0, h);
       __syncwarp();
       if (lane == 0) mbar_arrive(smem_u32(&sh.ready[s]));
       if (p.carries != nullptr && !tab.only_map)
