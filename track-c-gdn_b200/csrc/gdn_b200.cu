@@ -7,6 +7,7 @@
 #include "gdn_capi.cu"
 #include "gdn_prefill_noalloc.cu"
 #include "gdn_recurrence_forward.cu"
+#include "gdn_recurrence_backward.cu"
 #include "gdn_recurrence.cu"
 #include "gdn_checkpoint.cu"
 #include "gdn_recurrence_capi.cu"

@@ -340,6 +340,11 @@ __device__ __forceinline__ uint32_t quantise4(uint64_t a, uint64_t b, uint32_t E
 // of 2^23 is the fp32 number 2^23 + 128 + q: a byte permute and an addition
 // instead of a conversion, which would share the slow pipe with the gates'
 // exponentials.
+__device__ __forceinline__ uint64_t dequantise2(uint32_t q, uint32_t E) {
+  const uint32_t s = q ^ 0x8080u, m = 0x4b000000u;
+  const uint64_t v = f2_pack(__uint_as_float(__byte_perm(s, m, 0x7650)), __uint_as_float(__byte_perm(s, m, 0x7651)));
+  return f2_mul(f2_add(v, f2_dup(-8388736.f)), f2_dup(group_scale(E)));
+}
 __device__ __forceinline__ void dequantise4(uint32_t q, uint32_t E, uint64_t &a, uint64_t &b) {
   const uint64_t scale = f2_dup(group_scale(E)), off = f2_dup(-8388736.f);
   const uint32_t s = q ^ 0x80808080u, m = 0x4b000000u;

@@ -150,13 +150,13 @@ int gdn_recurrence_backward(int type, const void *x, int64_t x_stride, const voi
     const cudaError_t e1 = cudaMemsetAsync(ddt_bias, 0, channels * 4, s);
     return e0 == cudaSuccess && e1 == cudaSuccess ? GDN_OK : GDN_ERR_LAUNCH;
   }
-  const bool vec = channels % 4 == 0 &&
-                   (packed || (vector_rows(x, type, x_stride) && vector_rows(a, type, a_stride) &&
-                               vector_rows(b, type, b_stride))) &&
-                   vector_rows(d_out, type, d_out_stride) && vector_rows(dx, type, channels) &&
-                   vector_rows(da, type, channels) && vector_rows(db, type, channels) && aligned(A_log, 16) &&
-                   aligned(dt_bias, 16) && (!state || aligned(state, 16)) &&
-                   (!d_final_state || aligned(d_final_state, 16)) && (!d_state || aligned(d_state, 16));
+  const bool tma =
+      total_tokens > 0 && total_tokens <= INT32_MAX && channels % 4 == 0 &&
+      (packed ? channels % 16 == 0
+              : tma_rows(x, type, x_stride) && tma_rows(a, type, a_stride) && tma_rows(b, type, b_stride)) &&
+      tma_rows(d_out, type, d_out_stride) && aligned(dx, 8) && aligned(da, 8) && aligned(db, 8) &&
+      aligned(A_log, 8) && aligned(dt_bias, 8) && aligned(state, 8) && aligned(d_final_state, 8) &&
+      aligned(d_state, 8);
   char *extra = static_cast<char *>(workspace) + gdn_recurrence_workspace_bytes(total_tokens, channels);
   float *saved = reinterpret_cast<float *>(extra);
   if (!carries) {
@@ -177,9 +177,9 @@ int gdn_recurrence_backward(int type, const void *x, int64_t x_stride, const voi
   p.dx = dx, p.da = da, p.db = db, p.d_state = d_state;
   p.partials = reinterpret_cast<float2 *>(extra + gdn::rec::saved_bytes(total_tokens, channels));
   const cudaError_t e =
-      type == GDN_BF16   ? gdn::rec::launch_backward_e<__nv_bfloat16>(p, vec, workspace, dA_log, ddt_bias, s)
-      : type == GDN_FP16 ? gdn::rec::launch_backward_e<__half>(p, vec, workspace, dA_log, ddt_bias, s)
-                         : gdn::rec::launch_backward_e<float>(p, vec, workspace, dA_log, ddt_bias, s);
+      type == GDN_BF16   ? gdn::rec::launch_backward_e<__nv_bfloat16>(p, tma, workspace, sms, dA_log, ddt_bias, s)
+      : type == GDN_FP16 ? gdn::rec::launch_backward_e<__half>(p, tma, workspace, sms, dA_log, ddt_bias, s)
+                         : gdn::rec::launch_backward_e<float>(p, tma, workspace, sms, dA_log, ddt_bias, s);
   return e == cudaSuccess ? GDN_OK : GDN_ERR_LAUNCH;
 }
 

@@ -1,7 +1,5 @@
 // gdn_recurrence_forward.cu -- prefill of the channelwise gated linear
 // recurrence (mathematics and look-back: gdn_recurrence.cu).
-#include <cuda.h>
-
 #include "gdn_recurrence_tile.cuh"
 
 namespace gdn {
@@ -12,9 +10,6 @@ namespace rec {
 // consecutive rows.  A stage of shared memory holds one half (64 channels) as
 // planes of x, a and b, and afterwards, in place, what the first pass left: 16
 // bytes for each lane and row.
-constexpr int kTokW = 8;
-constexpr int kSlots = 8;
-constexpr int kRows = kTokW * kSlots;  // 64
 template <typename E, bool kTma, bool kPack>
 struct FwdShape {
   static constexpr int kHalves = kPack ? 2 : 1;
@@ -49,14 +44,6 @@ struct Forward {
   uint64_t *maps, *states;  // kChain
   const float *dt, *c;      // kChain: prepared
   const int *first;
-};
-
-// What the consumers need of an ordinary tile: all rows belong to sequences that
-// neither start nor end there, and all 64 channels of each half exist.
-struct alignas(16) Tile {
-  int64_t at;  // element of out where the tile begins
-  int d;       // the tile's channels; -1: no more tiles
-  int plain;
 };
 
 template <typename Shape, bool kPack>
@@ -509,49 +496,6 @@ recurrence_forward_kernel(const __grid_constant__ Forward p) {
 }
 
 // ---- launch ---------------------------------------------------------------------
-template <typename E>
-bool make_row_map(CUtensorMap *m, const void *base, int64_t channels, int64_t rows, int64_t stride, int box_x,
-                  int box_y) {
-  PFN_cuTensorMapEncodeTiled_v12000 enc = tensor_map_encoder();
-  if (enc == nullptr) return false;
-  const cuuint64_t dims[2] = {static_cast<cuuint64_t>(channels), static_cast<cuuint64_t>(rows)};
-  const cuuint64_t strides[1] = {static_cast<cuuint64_t>(stride) * sizeof(E)};
-  const cuuint32_t box[2] = {static_cast<cuuint32_t>(box_x), static_cast<cuuint32_t>(box_y)};
-  const cuuint32_t estr[2] = {1, 1};
-  const CUtensorMapDataType type = std::is_same<E, float>::value     ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
-                                   : std::is_same<E, __half>::value  ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
-                                   : std::is_same<E, uint8_t>::value ? CU_TENSOR_MAP_DATA_TYPE_UINT8
-                                                                     : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
-  return enc(m, type, 2, const_cast<void *>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-             CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
-}
-
-// The workspace: header, prepared parameters and first sequences, words (as
-// many as the widest tiles need).
-struct Places {
-  float *dt, *c;
-  int *first;
-  uint64_t *words;
-  size_t bytes;
-};
-inline int64_t tiles_of(int64_t D) { return (D + 127) / 128; }
-inline int64_t chunks_of(int64_t T) { return T > 0 ? (T + kRows - 1) / kRows : 1; }
-inline Places places(void *workspace, int64_t T, int64_t D) {
-  const int64_t width = tiles_of(D) * 128, chunks = chunks_of(T);
-  const size_t first = kHeaderBytes + 8 * width, words = first + (4 * (chunks + 1) + 15) / 16 * 16;
-  char *w = static_cast<char *>(workspace);
-  return Places{reinterpret_cast<float *>(w + kHeaderBytes), reinterpret_cast<float *>(w + kHeaderBytes + 4 * width),
-                reinterpret_cast<int *>(w + first), reinterpret_cast<uint64_t *>(w + words),
-                words + 8 * (chunks + (chunks + kGroupLen - 1) / kGroupLen) * width};
-}
-
-// Streams for nt tiles of channels on `ctas` CTAs: about as many CTAs to a stream
-// as it has tiles of channels, so that the chunk before is done or nearly so.
-inline int streams_for(int64_t nt, int64_t ctas) {
-  return static_cast<int>(max(int64_t{1}, min(int64_t{kStreams}, ctas / nt)));
-}
-
 // Inputs of up to this many chunks are walked by one CTA per 64 or 128 channels.
 constexpr int64_t kSerialChunks = 4;
 constexpr int64_t kSerialSeqs = 1024;  // each CTA checks all of cu_seqlens then
@@ -582,7 +526,7 @@ cudaError_t launch_forward_t(Forward p, void *workspace, int sms, cudaStream_t s
     p.first = w.first;
     const int64_t words = (chunks + (chunks + kGroupLen - 1) / kGroupLen) * nt * S::kCh;
     const Prepared q{p.A_log,     p.dt_bias, w.dt,  w.c, p.D, w.first, chunks, kRows,
-                     streams_for(nt, int64_t{sms} * S::kCtas)};
+                     streams_for(nt, int64_t{sms} * S::kCtas), false};
     if (cudaError_t e = launch_init(p.hdr, p.maps, words, p.s, q, stream)) return e;
     blocks = min(chunks * nt, int64_t{sms} * S::kCtas);
   }

@@ -2,6 +2,8 @@
 // beyond the arithmetic: sequences and their tables of starts and ends, pairs of
 // channels, affine maps, and the words that chunks hand to one another.
 #pragma once
+#include <cuda.h>
+
 #include <type_traits>
 
 #include "gdn_recurrence.cuh"
@@ -16,17 +18,30 @@ namespace rec {
 // whose predecessor is done: then a state per chunk is all that is published.
 constexpr int kGroupLen = 8;
 
+constexpr int kTokW = 8;
+constexpr int kSlots = 8;
+constexpr int kRows = kTokW * kSlots;  // 64
+
 // Sequences that start or end in a tile.
 template <int kRows>
 struct Table {
   int64_t chunk;  // -1: no more tiles
   int64_t valid;  // rows of the tile that belong to a sequence
-  int64_t reach;  // chunks between this one and where the sequence of its first row starts
+  int64_t reach;  // chunks from here to where the sequence of the first row starts
+  int64_t ahead;  // ... and to where that of the last row ends
   int d;
   int last;       // the last chunk
   int only_map;   // nothing but the tile's map is wanted
   uint32_t starts[kRows / 32], ends[kRows / 32];
   int start[kRows], end[kRows];  // the sequence, or -1
+};
+
+// What the consumers need of an ordinary tile: all rows belong to sequences that
+// neither start nor end there, and all 64 channels of each half exist.
+struct alignas(16) Tile {
+  int64_t at;  // element of out where the tile begins
+  int d;       // the tile's channels; -1: no more tiles
+  int plain;
 };
 
 struct Seqs {
@@ -40,16 +55,16 @@ struct Seqs {
 };
 
 // The chunks are worked on as up to kStreams streams side by side, each a run of
-// consecutive chunks that begins where a sequence does, so that a chunk's
-// predecessor has usually long been finished when its turn comes; one sequence
-// alone is one stream.  A stream's first chunk `from` may follow one in which
-// the sequence starts: that chunk belongs to the stream before, but its map is
-// needed at once, and is worked out once more by the stream (only_map).
+// consecutive chunks cut where a sequence starts, so that a chunk's predecessor
+// in the chain has usually long been finished when its turn comes; one sequence
+// alone is one stream.  The cut may go through a chunk: that chunk belongs to
+// the stream that ends with it, but its map is needed by the other from the
+// start, and is worked out there once more (only_map).
 constexpr int kStreams = 32;
 struct Stream {
   int64_t from, to;  // chunks [from, to)
   uint32_t ticket;
-  int only_map;      // 1: the stream starts with the map of chunk from - 1
+  int only_map;      // 1: starts with the map of chunk from - 1 (backwards: to)
 };
 struct Header {
   uint32_t bad;      // cu_seqlens or slots are not valid: write nothing
@@ -101,6 +116,7 @@ struct Prepared {
   int *first;       // [chunks + 1], or null
   int64_t chunks, rows;
   int streams;      // as many as wanted, at most kStreams
+  bool backwards;   // the chain runs from the last chunk to the first
 };
 
 // Empties the words, prepares, and checks the sequences, before the tiles run.
@@ -125,22 +141,29 @@ __global__ void __launch_bounds__(1024) recurrence_init_kernel(Header *hdr, ulon
     __shared__ int only_map[kStreams];
     const int i = threadIdx.x;
     if (i < q.streams) {
-      // the first chunk that begins with a sequence's start or after it, from
-      // an even cut on
+      // from an even cut on, where the next sequence starts: forwards the first
+      // chunk that begins there or after it, backwards the last one to end there
+      // or before it is the first of its stream
       const int64_t n = first_by_halves(s, q.chunks * i / q.streams * q.rows);
-      from[i] = i == 0 ? 0 : n < s.N ? (s.at(n) + q.rows - 1) / q.rows : q.chunks;
-      // does the sequence of its first row start in the chunk before?
-      const int64_t row = from[i] * q.rows, m = first_by_halves(s, row);
-      only_map[i] = i > 0 && !(m < s.N && s.at(m) == row);
+      const int64_t row = n < s.N ? s.at(n) : q.chunks * q.rows;
+      from[i] = i == 0 ? 0 : (q.backwards ? row : row + q.rows - 1) / q.rows;
+      // backwards: the chunk that the cut goes through belongs to the stream
+      // above, and the one below needs its map.  Forwards: the same of the chunk
+      // before, unless a sequence starts with the first row itself
+      const int64_t first = from[i] * q.rows, m = first_by_halves(s, first);
+      only_map[i] = i > 0 && (q.backwards ? row % q.rows != 0 : !(m < s.N && s.at(m) == first));
     }
     __syncthreads();
     if (i == 0) {
       int n = 1;
+      int64_t prev = 0;
       hdr->stream[0] = Stream{0, q.chunks, 0, 0};
       for (int j = 1; j < q.streams; ++j)
-        if (from[j] > from[j - 1] && from[j] < q.chunks) {
+        if (from[j] > prev && from[j] < q.chunks) {
+          prev = from[j];
           hdr->stream[n - 1].to = from[j];
-          hdr->stream[n] = Stream{from[j], q.chunks, 0, only_map[j]};
+          if (q.backwards) hdr->stream[n - 1].only_map = only_map[j];
+          hdr->stream[n] = Stream{from[j], q.chunks, 0, q.backwards ? 0 : only_map[j]};
           ++n;
         }
       hdr->streams = n;
@@ -175,7 +198,9 @@ __device__ __forceinline__ bool fill_table(const Seqs &s, Table<kRows> &t, int64
   const int64_t lo = first != nullptr ? first[base / kRows] : first_at_or_after(s, base, lane);
   // the sequence that covers the first row, if it does not start there
   if (lane == 0) t.reach = lo > 0 ? base / kRows - s.at(lo - 1) / kRows : 0;
-  if (!last && s.at(lo) > base + kRows) {
+  const int64_t next = lo < s.N ? s.at(lo) : s.total();
+  if (!last && next > base + kRows) {
+    if (lane == 0) t.ahead = (next - 1) / kRows - base / kRows;
     if (lane < kRows / 32) t.starts[lane] = t.ends[lane] = 0;
     return true;
   }
@@ -184,6 +209,7 @@ __device__ __forceinline__ bool fill_table(const Seqs &s, Table<kRows> &t, int64
   const int64_t hi = last               ? s.N
                      : first != nullptr ? first[base / kRows + 1]
                                         : first_at_or_after(s, base + kRows, lane);
+  if (lane == 0) t.ahead = last ? 0 : (s.at(hi) - 1) / kRows - base / kRows;
   __syncwarp();
   for (int64_t n0 = max(lo - 1, int64_t{0}); n0 < hi; n0 += 32) {
     const int64_t n = n0 + lane;
@@ -399,6 +425,50 @@ __device__ __forceinline__ void mbar_expect_tx(uint32_t mbar, uint32_t bytes) {
 }
 __device__ __forceinline__ void mbar_arrive(uint32_t mbar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(mbar) : "memory");
+}
+
+// ---- host ---------------------------------------------------------------------
+template <typename E>
+bool make_row_map(CUtensorMap *m, const void *base, int64_t channels, int64_t rows, int64_t stride, int box_x,
+                  int box_y) {
+  PFN_cuTensorMapEncodeTiled_v12000 enc = tensor_map_encoder();
+  if (enc == nullptr) return false;
+  const cuuint64_t dims[2] = {static_cast<cuuint64_t>(channels), static_cast<cuuint64_t>(rows)};
+  const cuuint64_t strides[1] = {static_cast<cuuint64_t>(stride) * sizeof(E)};
+  const cuuint32_t box[2] = {static_cast<cuuint32_t>(box_x), static_cast<cuuint32_t>(box_y)};
+  const cuuint32_t estr[2] = {1, 1};
+  const CUtensorMapDataType type = std::is_same<E, float>::value     ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                                   : std::is_same<E, __half>::value  ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                                   : std::is_same<E, uint8_t>::value ? CU_TENSOR_MAP_DATA_TYPE_UINT8
+                                                                     : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+  return enc(m, type, 2, const_cast<void *>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+             CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// The workspace: header, prepared parameters and first sequences, words (as
+// many as the widest tiles need).
+struct Places {
+  float *dt, *c;
+  int *first;
+  uint64_t *words;
+  size_t bytes;
+};
+inline int64_t tiles_of(int64_t D) { return (D + 127) / 128; }
+inline int64_t chunks_of(int64_t T) { return T > 0 ? (T + kRows - 1) / kRows : 1; }
+inline Places places(void *workspace, int64_t T, int64_t D) {
+  const int64_t width = tiles_of(D) * 128, chunks = chunks_of(T);
+  const size_t first = kHeaderBytes + 8 * width, words = first + (4 * (chunks + 1) + 15) / 16 * 16;
+  char *w = static_cast<char *>(workspace);
+  return Places{reinterpret_cast<float *>(w + kHeaderBytes), reinterpret_cast<float *>(w + kHeaderBytes + 4 * width),
+                reinterpret_cast<int *>(w + first), reinterpret_cast<uint64_t *>(w + words),
+                words + 8 * (chunks + (chunks + kGroupLen - 1) / kGroupLen) * width};
+}
+
+// Streams for nt tiles of channels on `ctas` CTAs: about as many CTAs to a stream
+// as it has tiles of channels, so that the chunk before is done or nearly so.
+inline int streams_for(int64_t nt, int64_t ctas) {
+  return static_cast<int>(max(int64_t{1}, min(int64_t{kStreams}, ctas / nt)));
 }
 
 }  // namespace rec
