@@ -456,6 +456,49 @@ def test_two_streams_at_once(gdn):
             assert torch.equal(p[0], q[0]) and torch.equal(p[1], q[1])
 
 
+def test_calls_from_a_thread_that_has_not_used_cuda(gdn):
+    """As autograd's threads are: with all memory from torch's cache nothing
+    before the call makes the device's context current there."""
+    import threading
+    import cases
+    from gpu_util import prefill_args
+
+    d = dev(inputs([600], 128, BF16, 71))
+    d_out = torch.randn(600, 128, device="cuda").to(BF16)
+    want = gdn.recurrence.backward(*d, None, d_out)
+    out, final = gdn.recurrence.run(*d)
+    out2, final2 = torch.empty_like(out), torch.empty_like(final)
+    ws = gdn.recurrence.alloc_workspace(600, 128, "cuda")
+    g = {k: torch.empty_like(v) for k, v in want.items()}
+    bws = gdn.recurrence.alloc_backward_workspace(600, 128, "cuda")
+    p = prefill_args(cases.prefill_inputs(seed=3, lens=[100, 30], with_state=True))
+    p_out, p_final = gdn.prefill.run(*p, None)
+    p_out2, p_final2 = torch.empty_like(p_out), torch.empty_like(p_final)
+    pws = gdn.prefill.alloc_workspace(130, 2, "cuda")
+    stream = torch.cuda.current_stream().cuda_stream
+    errors = []
+
+    def call(f):
+        try:
+            f()
+        except Exception as e:      # noqa: BLE001  (reported by the test's own thread)
+            errors.append(e)
+
+    for f in (lambda: gdn.recurrence.run_into(*d, None, out2, final2, ws, stream=stream),
+              lambda: gdn.recurrence.backward_into(*d, None, d_out, None, g["dx"], g["da"], g["db"], g["dA_log"],
+                                                   g["ddt_bias"], g["d_state"], bws, stream=stream),
+              lambda: gdn.prefill.prefill_into(*p, None, p_out2, p_final2, pws, stream=stream)):
+        t = threading.Thread(target=call, args=(f,))
+        t.start()
+        t.join()
+    assert not errors, errors
+    torch.cuda.synchronize()
+    assert torch.equal(out, out2) and torch.equal(final, final2)
+    assert torch.equal(p_out, p_out2) and torch.equal(p_final, p_final2)
+    for k, v in want.items():
+        assert torch.equal(v, g[k]), k
+
+
 def test_captured_training_step_with_new_lengths_on_replay(gdn):
     """Forward and backward in a graph; replays see other values and other
     cu_seqlens, fewer rows among them."""

@@ -59,11 +59,13 @@ bool overlap(const void *a, size_t na, const void *b, size_t nb) {
   return x < y + nb && y < x + na;
 }
 
-// Current device must be sm_100 (B200 family); cached per device ordinal.
+// Current device must be sm_100 (B200 family); cached per device ordinal.  Makes
+// its context current for the calling thread: a thread that has not used CUDA
+// yet (autograd's, for one) has none, and tensor maps cannot be encoded then.
 int check_device(int *num_sms) {
   static int cached_dev = -1, cached_ok = 0, cached_sms = 0;
   int dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess) return GDN_ERR_DEVICE;
+  if (cudaGetDevice(&dev) != cudaSuccess || cudaSetDevice(dev) != cudaSuccess) return GDN_ERR_DEVICE;
   if (dev != cached_dev) {
     cudaDeviceProp prop;
     if (cudaGetDeviceProperties(&prop, dev) != cudaSuccess) return GDN_ERR_DEVICE;
