@@ -10,10 +10,12 @@
 // the forward.  The state that enters a chunk was saved; R goes through the
 // chain.  Consumers, first pass: the slot's map of the state (P, y) and of R
 // (P, Q with Q = sum of P_i d_out_i: one ascending sweep gives both).  Second
-// pass, one tile later: gates once more, half a slot (4 rows) at a time, first
+// pass, once the chain warp has what enters: gates once more, half a slot (4 rows) at a time, first
 // upwards for the states, then downwards for the gradients.  Evaluating the
 // gates twice costs exponentials but no memory: keeping them would take 16
-// bytes a value beside the 8 of the inputs.
+// bytes a value beside the 8 of the inputs.  The second pass is not put off by
+// a tile as in the forward: with the two stages that fit the next tile's copy
+// would then wait for it (303 against NEW us, 8 x 4096 x 2048 bf16).
 #include "gdn_recurrence_tile.cuh"
 
 namespace gdn {
@@ -340,8 +342,8 @@ recurrence_backward_kernel(const __grid_constant__ Backward p) {
                                                   static_cast<int>(min(p.D - c0, int64_t{64})))
                                 : 0;
   };
-  int s = 0, s1 = 0, turn = 0;
-  uint32_t parity = 0, parity1 = 0;
+  int s = 0, turn = 0;
+  uint32_t parity = 0;
   for (int k = 0;; ++k) {
     if (!__all_sync(0xffffffffu, wait_phase(smem_u32(&sh.full[s]), parity, &sh.broken))) return;
     const Tile tile = sh.tiles[s];
@@ -410,19 +412,14 @@ recurrence_backward_kernel(const __grid_constant__ Backward p) {
         if (lane == 0) mbar_arrive(smem_u32(&sh.taken[s]));
       }
       turn = turn + 1 == kSlots ? 0 : turn + 1;
-    }
-    if (k > 0) {
-      // second pass, over the tile before
-      if (!__all_sync(0xffffffffu, wait_phase(smem_u32(&sh.ready[s1]), parity1, &sh.broken))) return;
-      const Table<kRows> &tab = sh.tables[s1];
-      const Tile before = sh.tiles[s1];
+
+      // second pass
+      if (!__all_sync(0xffffffffu, wait_phase(smem_u32(&sh.ready[s]), parity, &sh.broken))) return;
       if (!tab.only_map) {
-        const int64_t c0 = static_cast<int64_t>(before.d) * 64;
-        const Params2 par{load2_f32<kVec>(sh.params[s1][0], lane, 64), load2_f32<kVec>(sh.params[s1][1], lane, 64)};
-        const float4 in4 = sh.own[s1][warp][lane], mid4 = sh.mid[s1][warp][lane];
+        const float4 in4 = sh.own[s][warp][lane], mid4 = sh.mid[s][warp][lane];
         const uint64_t h_in = f2_pack(in4.x, in4.y);
         uint64_t R = f2_pack(in4.z, in4.w), sum_lg = 0, sum_da = 0;
-        const int64_t at = before.at + row0 * p.D;
+        const int64_t at = tile.at + row0 * p.D;
         constexpr int kHalf = kTokW / 2;
         auto half = [&](int i0, bool edge, int valid, unsigned starts, unsigned ends, int left) {
           uint64_t g[kHalf], o[kHalf], beta[kHalf], xs[kHalf], ca[kHalf], cl[kHalf];
@@ -434,7 +431,7 @@ recurrence_backward_kernel(const __grid_constant__ Backward p) {
 #pragma unroll
           for (int j = 0; j < kHalf; ++j) {
             uint64_t in[3];
-            load(s1, before, i0 + j, in, o[j]);
+            load(s, tile, i0 + j, in, o[j]);
             if (edge && ((starts >> (i0 + j)) & 1)) h = initial(tab, c0, i0 + j);
             // beta and beta (1 - beta) from e = exp(-|b|): r = 1 / (1 + e), e r
             const uint64_t eb = ex2_neg_abs(f2_mul(in[2], f2_dup(kLog2e))), db1 = f2_add(eb, f2_dup(1.f));
@@ -470,7 +467,7 @@ recurrence_backward_kernel(const __grid_constant__ Backward p) {
               store2_f32<kVec>(p.d_state + tab.start[row0 + i] * p.D + c0, lane, left, R);
           }
         };
-        if (before.plain) {
+        if (tile.plain) {
           half(kHalf, false, kTokW, 0, 0, 64);
           half(0, false, kTokW, 0, 0, 64);
         } else {
@@ -481,15 +478,13 @@ recurrence_backward_kernel(const __grid_constant__ Backward p) {
           for (int i0 = kHalf; i0 >= 0; i0 -= kHalf) half(i0, true, valid, starts, ends, left);
         }
         constexpr float kLn2 = 0.6931471805599453f;
-        sh.own[s1][warp][lane] =
+        sh.own[s][warp][lane] =
             make_float4(f2_lo(sum_lg) * kLn2, f2_hi(sum_lg) * kLn2, f2_lo(sum_da), f2_hi(sum_da));
       }
       __syncwarp();
-      if (lane == 0) mbar_arrive(smem_u32(&sh.empty[s1]));
+      if (lane == 0) mbar_arrive(smem_u32(&sh.empty[s]));
     }
     if (tile.d < 0) return;
-    s1 = s;
-    parity1 = parity;
     if (++s == kStages) s = 0, parity ^= 1;
   }
 }
