@@ -139,11 +139,12 @@ def backward(x, state, A_log, a, dt_bias, b, cu, d_out, d_final, eight=False):
     sig = torch.sigmoid(k.z)
     rel_sig = (k.moved + 10) * U
     slope = k.beta * (1 - k.beta)
-    rel_slope = 2 * k.rel_beta + 2 * U
     dx = k.beta * dh
     dx_err = dx.abs() * (k.rel_beta + U) + k.beta * dh_err
     db = k.x * dh * slope
-    db_err = db.abs() * (rel_slope + 3 * U) + (k.x * slope).abs() * dh_err
+    # beta - beta^2 in one rounding from the rounded beta: its error is beta's
+    # times |1 - 2 beta| <= 1, also where 1 - beta is small
+    db_err = (k.x * dh).abs() * k.beta * k.rel_beta + db.abs() * 4 * U + (k.x * slope).abs() * dh_err
     dlg = k.g * prev * dh
     dlg_err = dlg.abs() * (k.rel_g + 3 * U) + k.g * (dh.abs() * prev_err + prev.abs() * dh_err)
     da = -k.A * dlg * sig

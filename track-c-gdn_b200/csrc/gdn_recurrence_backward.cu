@@ -9,13 +9,10 @@
 // One pass over the tiles from the last chunk to the first, with the roles of
 // the forward.  The state that enters a chunk was saved; R goes through the
 // chain.  Consumers, first pass: the slot's map of the state (P, y) and of R
-// (P, Q with Q = sum of P_i d_out_i: one ascending sweep gives both).  Second
-// pass, once the chain warp has what enters: gates once more, half a slot (4 rows) at a time, first
-// upwards for the states, then downwards for the gradients.  Evaluating the
-// gates twice costs exponentials but no memory: keeping them would take 16
-// bytes a value beside the 8 of the inputs.  The second pass is not put off by
-// a tile as in the forward: with the two stages that fit the next tile's copy
-// would then wait for it (303 against NEW us, 8 x 4096 x 2048 bf16).
+// (P, Q with Q = sum of P_i d_out_i: one ascending sweep gives both); softplus
+// and beta stay in shared memory.  Second pass, when the chain warp has what
+// enters: half a slot (4 rows) at a time, first upwards for the states, then
+// downwards for the gradients.
 #include "gdn_recurrence_tile.cuh"
 
 namespace gdn {
@@ -26,9 +23,11 @@ struct BwdShape {
   static constexpr int kThreads = 32 * (kSlots + 2);
   static constexpr int kPlane = kRows * 64 * static_cast<int>(sizeof(E));      // d_out; x, a, b
   static constexpr int kInPlane = kPacked ? kRows * 64 : kPlane;
-  static constexpr int kStage = kTma ? kPlane + 3 * kInPlane : 0;
+  static constexpr int kStage = kTma ? kPlane + 3 * kInPlane : kSlots * 512;
   static constexpr int kStages = 2;
   static constexpr int kCtas = kStage > 49152 ? 1 : 2;
+  // where a warp leaves its sums: the stage's first plane, in its own rows
+  static constexpr int kSlotBytes = kTma ? kPlane / kSlots : 512;
 };
 
 struct Backward {
@@ -52,12 +51,12 @@ struct Backward {
 
 template <typename Shape, bool kPacked>
 struct BwdShared {
-  // A slot's P and y, its Q, and P and y of its first half.  The chain warp
-  // replaces P, y by the state and the R that enter, and the consumers at the
-  // end by their sums for the parameters' gradients.
-  float4 own[Shape::kStages][kSlots][32];
-  float2 rev[Shape::kStages][kSlots][32];
-  float4 mid[Shape::kStages][kSlots][32];
+  // A slot's P and y, and its Q.  The chain warp replaces P, y by the state and
+  // the R that enter.
+  float4 own[kSlots][32];
+  float2 rev[kSlots][32];
+  // what the first pass leaves to the second: softplus(z) log2(e) and beta
+  ulonglong2 kept[kSlots][kTokW][32];
   float params[Shape::kStages][2][64];
   uint8_t scales[kPacked ? Shape::kStages : 1][3][kRows];
   Table<kRows> tables[Shape::kStages];
@@ -110,10 +109,11 @@ recurrence_backward_kernel(const __grid_constant__ Backward p) {
       if (!__all_sync(0xffffffffu, wait_phase(smem_u32(&sh.empty[s]), (i / kStages) & 1, &sh.broken))) return false;
       const Table<kRows> &t = sh.tables[s];
       if (!t.only_map) {
-        float4 v = sh.own[s][0][lane];
+        const unsigned char *sums = smem + s * S::kStage + lane * 16;
+        float4 v = *reinterpret_cast<const float4 *>(sums);
 #pragma unroll
         for (int j = 1; j < kSlots; ++j) {
-          const float4 w = sh.own[s][j][lane];
+          const float4 w = *reinterpret_cast<const float4 *>(sums + j * S::kSlotBytes);
           v.x += w.x, v.y += w.y, v.z += w.z, v.w += w.w;
         }
         float2 *dst = p.partials + t.chunk * groups128 * 128 + t.d * 64;
@@ -165,11 +165,12 @@ recurrence_backward_kernel(const __grid_constant__ Backward p) {
           sh.tiles[s].d = -1;
           mbar_arrive(full);
         }
-        if (k > 0) finish(k - 1);
+        for (int i = max(k - kStages + 1, 0); i < k; ++i)
+          if (!finish(i)) break;
         break;
       }
       if (lane == 0) {
-        mbar_expect_tx(full, 2 * 64 * 4 + S::kStage);
+        mbar_expect_tx(full, 2 * 64 * 4 + (kTma ? S::kStage : 0));
         bulk_load(smem_u32(sh.params[s][0]), p.dt + c0, 64 * 4, full);
         bulk_load(smem_u32(sh.params[s][1]), p.c + c0, 64 * 4, full);
         if constexpr (kTma) {
@@ -247,8 +248,8 @@ recurrence_backward_kernel(const __grid_constant__ Backward p) {
       if (!__all_sync(0xffffffffu, wait_phase(smem_u32(&sh.mapped[s]), parity, &sh.broken) &&
                                        wait_phase(smem_u32(&sh.taken[s]), parity, &sh.broken)))
         return;
-      float4 *own = &sh.own[s][0][lane];
-      const float2 *rev = &sh.rev[s][0][lane];
+      float4 *own = &sh.own[0][lane];
+      const float2 *rev = &sh.rev[0][lane];
       const uint32_t ends[2] = {tab.ends[0], tab.ends[1]}, starts[2] = {tab.starts[0], tab.starts[1]};
       const bool publishes = chunk > 0 && !tab.only_map && place == group_len - 1;
       uint64_t R = 0;
@@ -344,19 +345,23 @@ recurrence_backward_kernel(const __grid_constant__ Backward p) {
   };
   int s = 0, turn = 0;
   uint32_t parity = 0;
-  for (int k = 0;; ++k) {
+  while (true) {
     if (!__all_sync(0xffffffffu, wait_phase(smem_u32(&sh.full[s]), parity, &sh.broken))) return;
     const Tile tile = sh.tiles[s];
-    if (tile.d >= 0) {
+    if (tile.d < 0) return;
+    {
       // first pass
       const Table<kRows> &tab = sh.tables[s];
       const int64_t c0 = static_cast<int64_t>(tile.d) * 64;
       const Params2 par{load2_f32<kVec>(sh.params[s][0], lane, 64), load2_f32<kVec>(sh.params[s][1], lane, 64)};
-      uint64_t P = f2_dup(1.f), y = 0, Q = 0;
+      uint64_t P = f2_dup(1.f), y = 0, Q = 0, P_mid = 0, y_mid = 0;  // _mid: after half the slot
       auto row = [&](int i, bool edge, int valid, unsigned starts, unsigned ends, bool &ended) {
-        uint64_t in[3], o, g, u;
+        uint64_t in[3], o;
         load(s, tile, i, in, o);
-        gate_pair(in[0], in[1], in[2], par.dt, par.c, g, u);
+        const uint64_t w = f2_fma(in[1], f2_dup(kLog2e), par.dt), sp = softplus2(w, ex2_neg_abs(w));
+        const uint64_t beta = sigmoid_pair(in[2]);
+        sh.kept[warp][i][lane] = make_ulonglong2(sp, beta);
+        uint64_t g = ex2_pair(f2_mul(par.c, sp)), u = f2_mul(beta, in[0]);
         if (edge) {
           if (i >= valid) g = f2_dup(1.f), u = 0, o = 0;
           if ((starts >> i) & 1) y = initial(tab, c0, i);
@@ -372,8 +377,7 @@ recurrence_backward_kernel(const __grid_constant__ Backward p) {
           }
           Q = f2_fma(P, o, Q);
         }
-        if (i == kTokW / 2 - 1)
-          sh.mid[s][warp][lane] = make_float4(f2_lo(P), f2_hi(P), f2_lo(y), f2_hi(y));
+        if (i == kTokW / 2 - 1) P_mid = P, y_mid = y;
       };
       bool ended = false;
       if (tile.plain) {
@@ -385,8 +389,8 @@ recurrence_backward_kernel(const __grid_constant__ Backward p) {
 #pragma unroll 1
         for (int i = 0; i < kTokW; ++i) row(i, true, valid, starts, ends, ended);
       }
-      sh.own[s][warp][lane] = make_float4(f2_lo(P), f2_hi(P), f2_lo(y), f2_hi(y));
-      sh.rev[s][warp][lane] = make_float2(f2_lo(Q), f2_hi(Q));
+      sh.own[warp][lane] = make_float4(f2_lo(P), f2_hi(P), f2_lo(y), f2_hi(y));
+      sh.rev[warp][lane] = make_float2(f2_lo(Q), f2_hi(Q));
       __syncwarp();
       const uint32_t mapped = smem_u32(&sh.mapped[s]);
       if (lane == 0) mbar_arrive(mapped);
@@ -395,8 +399,8 @@ recurrence_backward_kernel(const __grid_constant__ Backward p) {
         if (tab.chunk > 0 && (!group_end || tab.only_map)) {
           if (!__all_sync(0xffffffffu, wait_phase(mapped, parity, &sh.broken))) return;
           auto map = [&](int i) {
-            const float4 v = sh.own[s][i][lane];
-            const float2 q = sh.rev[s][i][lane];
+            const float4 v = sh.own[i][lane];
+            const float2 q = sh.rev[i][lane];
             return Map2{mask_bits(tab.ends, i * kTokW, kTokW) ? f2_dup(-1.f) : f2_pack(v.x, v.y), f2_pack(q.x, q.y)};
           };
           Map2 all = map(kSlots - 1);
@@ -416,7 +420,7 @@ recurrence_backward_kernel(const __grid_constant__ Backward p) {
       // second pass
       if (!__all_sync(0xffffffffu, wait_phase(smem_u32(&sh.ready[s]), parity, &sh.broken))) return;
       if (!tab.only_map) {
-        const float4 in4 = sh.own[s][warp][lane], mid4 = sh.mid[s][warp][lane];
+        const float4 in4 = sh.own[warp][lane];
         const uint64_t h_in = f2_pack(in4.x, in4.y);
         uint64_t R = f2_pack(in4.z, in4.w), sum_lg = 0, sum_da = 0;
         const int64_t at = tile.at + row0 * p.D;
@@ -425,23 +429,22 @@ recurrence_backward_kernel(const __grid_constant__ Backward p) {
           uint64_t g[kHalf], o[kHalf], beta[kHalf], xs[kHalf], ca[kHalf], cl[kHalf];
           uint64_t h = h_in;
           if (i0 > 0) {  // the state in the middle of the slot
-            h = f2_pack(mid4.z, mid4.w);
-            if (!edge || !(starts & ((1u << kHalf) - 1u))) h = f2_fma(f2_pack(mid4.x, mid4.y), h_in, h);
+            h = y_mid;
+            if (!edge || !(starts & ((1u << kHalf) - 1u))) h = f2_fma(P_mid, h_in, h);
           }
 #pragma unroll
           for (int j = 0; j < kHalf; ++j) {
             uint64_t in[3];
             load(s, tile, i0 + j, in, o[j]);
             if (edge && ((starts >> (i0 + j)) & 1)) h = initial(tab, c0, i0 + j);
-            // beta and beta (1 - beta) from e = exp(-|b|): r = 1 / (1 + e), e r
-            const uint64_t eb = ex2_neg_abs(f2_mul(in[2], f2_dup(kLog2e))), db1 = f2_add(eb, f2_dup(1.f));
-            const uint64_t rb = f2_pack(rcp(f2_lo(db1)), rcp(f2_hi(db1))), erb = f2_mul(eb, rb);
-            beta[j] = f2_pack(f2_lo(in[2]) >= 0.f ? f2_lo(rb) : f2_lo(erb), f2_hi(in[2]) >= 0.f ? f2_hi(rb) : f2_hi(erb));
-            xs[j] = f2_mul(in[0], f2_mul(rb, erb));
+            const ulonglong2 kept = sh.kept[warp][i0 + j][lane];
+            const uint64_t sp = kept.x;
+            beta[j] = kept.y;
+            xs[j] = f2_mul(in[0], f2_fma(f2_mul(beta[j], f2_dup(-1.f)), beta[j], beta[j]));  // x beta (1 - beta)
+            // sigmoid(z) from e = exp(-|z|): r = 1 / (1 + e) or e r
             const uint64_t w = f2_fma(in[1], f2_dup(kLog2e), par.dt), e = ex2_neg_abs(w), d1 = f2_add(e, f2_dup(1.f));
             const uint64_t rz = f2_pack(rcp(f2_lo(d1)), rcp(f2_hi(d1))), erz = f2_mul(e, rz);
             const uint64_t sig = f2_pack(f2_lo(w) >= 0.f ? f2_lo(rz) : f2_lo(erz), f2_hi(w) >= 0.f ? f2_hi(rz) : f2_hi(erz));
-            const uint64_t sp = softplus2(w, e);
             g[j] = ex2_pair(f2_mul(par.c, sp));
             const uint64_t gh = f2_mul(g[j], h), cgh = f2_mul(par.c, gh);  // -exp(A_log) g h_{t-1}
             h = f2_fma(g[j], h, f2_mul(beta[j], in[0]));
@@ -478,13 +481,14 @@ recurrence_backward_kernel(const __grid_constant__ Backward p) {
           for (int i0 = kHalf; i0 >= 0; i0 -= kHalf) half(i0, true, valid, starts, ends, left);
         }
         constexpr float kLn2 = 0.6931471805599453f;
-        sh.own[s][warp][lane] =
+        __syncwarp();  // all lanes have read the warp's rows
+        *reinterpret_cast<float4 *>(smem + s * S::kStage + warp * S::kSlotBytes + lane * 16) =
             make_float4(f2_lo(sum_lg) * kLn2, f2_hi(sum_lg) * kLn2, f2_lo(sum_da), f2_hi(sum_da));
+        if (kTma) fence_async_smem();  // the next copy into this stage comes after
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(smem_u32(&sh.empty[s]));
     }
-    if (tile.d < 0) return;
     if (++s == kStages) s = 0, parity ^= 1;
   }
 }
