@@ -322,6 +322,10 @@ __device__ __forceinline__ float group_inverse(uint32_t E) {  // 2^(127 - E); 0 
 // q of two (four) values as bytes.  v inv is exact and below 2^7 in magnitude
 // (2^7.01 in a capped group), so adding 1.5 2^23 rounds it to an integer, half
 // to even, in the sum's low byte.
+__device__ __forceinline__ uint32_t quantise2(uint64_t a, float inv) {  // E below the cap
+  a = f2_fma(a, f2_dup(inv), f2_dup(12582912.f));
+  return __byte_perm(static_cast<uint32_t>(a), static_cast<uint32_t>(a >> 32), 0x0040);
+}
 __device__ __forceinline__ uint32_t quantise2(uint64_t a, uint32_t E, uint32_t cap) {
   if (E == kExpNonFinite) return 0u;  // 0 times infinity reads back as NaN
   const uint64_t magic = f2_dup(12582912.f);

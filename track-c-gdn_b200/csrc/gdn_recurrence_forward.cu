@@ -59,6 +59,7 @@ struct FwdShared {
   uint64_t taken[Shape::kStages][Shape::kHalves];   // ... and have been read for the tile's
   uint64_t pair[kPack ? kSlots : 1];
   uint32_t amax[kPack ? 2 * kSlots * 64 : 1];
+  alignas(16) float inverse[kPack ? Shape::kWorkers : 1][32];
   int broken;
 };
 
@@ -328,15 +329,15 @@ recurrence_forward_kernel(const __grid_constant__ Forward p) {
         starts = mask_bits(tab.starts, row0, kTokW);
       }
       Raw2<E> raw[3][kTokW];
-      if constexpr (kTma) {
-#pragma unroll
-        for (int w = 0; w < 3; ++w)
+      auto fetch = [&](int w) {  // the lane's 8 rows of x, a or b
+        if constexpr (kTma) {
 #pragma unroll
           for (int i = 0; i < kTokW; ++i)
             raw[w][i].v =
                 reinterpret_cast<const decltype(Raw2<E>::v) *>(stage + w * S::kPlane + i * 64 * sizeof(E))[lane];
-        __syncwarp();  // the warp's rows are overwritten from here on
-      } else {
+        }
+      };
+      if constexpr (!kTma) {
         const int64_t t0 = tab.chunk * kRows + row0;
         const int left = static_cast<int>(min(p.D - c0, int64_t{64}));
 #pragma unroll
@@ -352,19 +353,23 @@ recurrence_forward_kernel(const __grid_constant__ Forward p) {
       if constexpr (kPack) {
         // The groups' largest magnitudes: each half by one warp, joined through
         // shared memory.  Lane 8 w + i holds what belongs to row i of x, a or b.
+        // The values are fetched anew for each use, not kept: registers are scarcer.
         uint32_t mine = 0;
 #pragma unroll
-        for (int w = 0; w < 3; ++w)
+        for (int w = 0; w < 3; ++w) {
+          fetch(w);
 #pragma unroll
           for (int i = 0; i < kTokW; ++i) {
             const uint32_t m = __reduce_max_sync(0xffffffffu, raw[w][i].abs_max());
             if (lane == kTokW * w + i) mine = m;
           }
+        }
         uint32_t *amax = sh.amax + ((k & 1) * kSlots + slot) * 64;
         amax[32 * half + lane] = mine;
         __syncwarp();
         if (lane == 0) mbar_arrive(smem_u32(&sh.pair[slot]));
         if (!__all_sync(0xffffffffu, wait_phase(smem_u32(&sh.pair[slot]), k & 1, &sh.broken))) return;
+        asm volatile("" ::: "memory");
         const uint32_t ex =
             group_exponent(Raw2<E>::magnitude(max(mine, amax[32 * (half ^ 1) + lane])), exp_cap<E>());
         const int64_t t0 = tab.chunk * kRows + row0;
@@ -372,14 +377,47 @@ recurrence_forward_kernel(const __grid_constant__ Forward p) {
         if (half == 0 && lane < 3 * kTokW && lane % kTokW < valid)
           p.packed[3 * p.s.T * p.D + (lane / kTokW * p.s.T + t0 + lane % kTokW) * nt + tile.d] =
               static_cast<uint8_t>(ex);
+        if (tile.plain && __all_sync(0xffffffffu, ex < exp_cap<E>())) {
+          // ordinary groups: one multiplication by the inverse scales, which
+          // the lanes hand around through shared memory
+          float *inv = sh.inverse[warp];
+          if (lane < 3 * kTokW) inv[lane] = group_inverse(ex);
+          __syncwarp();
 #pragma unroll
-        for (int w = 0; w < 3; ++w) {
-          uint8_t *dst = p.packed + (w * p.s.T + t0) * p.D + c0;
+          for (int w = 0; w < 3; ++w) {
+            uint16_t *dst = reinterpret_cast<uint16_t *>(p.packed + (w * p.s.T + t0) * p.D + c0) + lane;
+            fetch(w);
+            float f[kTokW];
 #pragma unroll
-          for (int i = 0; i < kTokW; ++i) {
-            const uint64_t v = raw[w][i].pair();
-            const uint32_t q = quantise2(v, __shfl_sync(0xffffffffu, ex, kTokW * w + i), exp_cap<E>());
-            if (i < valid) {
+            for (int i = 0; i < kTokW; i += 4)
+              *reinterpret_cast<float4 *>(f + i) = *reinterpret_cast<const float4 *>(inv + kTokW * w + i);
+#pragma unroll
+            for (int i = 0; i < kTokW; ++i) {
+              const uint32_t q = quantise2(raw[w][i].pair(), f[i]);
+              if constexpr (kVec) {
+                *dst = static_cast<uint16_t>(q);
+              } else {
+                reinterpret_cast<uint8_t *>(dst - lane)[lane] = static_cast<uint8_t>(q);
+                reinterpret_cast<uint8_t *>(dst - lane)[lane + 32] = static_cast<uint8_t>(q >> 8);
+              }
+              dst = reinterpret_cast<uint16_t *>(reinterpret_cast<uint8_t *>(dst) + p.D);
+            }
+          }
+        } else {
+#pragma unroll 1
+          for (int w = 0; w < 3; ++w) {
+            uint8_t *dst = p.packed + (w * p.s.T + t0) * p.D + c0;
+#pragma unroll 1
+            for (int i = 0; i < valid; ++i, dst += p.D) {
+              Raw2<E> r;
+              if constexpr (kTma) {
+                r.v = reinterpret_cast<const decltype(r.v) *>(stage + w * S::kPlane + i * 64 * sizeof(E))[lane];
+              } else {
+                const void *src = w == 0 ? p.x : w == 1 ? p.a : p.b;
+                const int64_t stride = w == 0 ? p.x_stride : w == 1 ? p.a_stride : p.b_stride;
+                r = load2<E, kVec>(static_cast<const E *>(src) + (t0 + i) * stride + c0, lane, left);
+              }
+              const uint32_t q = quantise2(r.pair(), __shfl_sync(0xffffffffu, ex, kTokW * w + i), exp_cap<E>());
               if constexpr (kVec) {
                 if (2 * lane < left) reinterpret_cast<uint16_t *>(dst)[lane] = static_cast<uint16_t>(q);
               } else {
@@ -387,10 +425,13 @@ recurrence_forward_kernel(const __grid_constant__ Forward p) {
                 if (lane + 32 < left) dst[lane + 32] = static_cast<uint8_t>(q >> 8);
               }
             }
-            dst += p.D;
           }
         }
       }
+      asm volatile("" ::: "memory");
+#pragma unroll
+      for (int w = 0; w < 3; ++w) fetch(w);
+      __syncwarp();  // the warp's rows are overwritten from here on
       auto keep = [&](int i, uint64_t y, uint64_t P) {
         *reinterpret_cast<ulonglong2 *>(stage + i / S::kPerPlane * S::kPlaneBytes + i % S::kPerPlane * 512 +
                                         lane * 16) = make_ulonglong2(y, P);

@@ -259,14 +259,22 @@ struct Raw2<__nv_bfloat16> {
   uint32_t v;
   // the larger magnitude as bits whose order is that of the values, and those
   // bits as an fp32's
-  __device__ __forceinline__ uint32_t abs_max() const { return max(v & 0x7fffu, (v >> 16) & 0x7fffu); }
+  __device__ __forceinline__ uint32_t abs_max() const {  // in both halves
+    const __nv_bfloat162 a = *reinterpret_cast<const __nv_bfloat162 *>(&v);
+    const __nv_bfloat162 m = __hmax2_nan(__habs2(a), __habs2(__lowhigh2highlow(a)));
+    return *reinterpret_cast<const uint32_t *>(&m);
+  }
   __device__ static __forceinline__ uint32_t magnitude(uint32_t m) { return m << 16; }
   __device__ __forceinline__ uint64_t pair() const { return f2_pack(bf16_lo(v), bf16_hi(v)); }
 };
 template <>
 struct Raw2<__half> {
   uint32_t v;
-  __device__ __forceinline__ uint32_t abs_max() const { return max(v & 0x7fffu, (v >> 16) & 0x7fffu); }
+  __device__ __forceinline__ uint32_t abs_max() const {  // in both halves
+    const __half2 a = *reinterpret_cast<const __half2 *>(&v);
+    const __half2 m = __hmax2_nan(__habs2(a), __habs2(__lowhigh2highlow(a)));
+    return *reinterpret_cast<const uint32_t *>(&m);
+  }
   __device__ static __forceinline__ uint32_t magnitude(uint32_t m) {
     return __float_as_uint(__half2float(__ushort_as_half(static_cast<uint16_t>(m))));
   }
