@@ -1,120 +1,132 @@
 // gdn_checkpoint.cu -- activations to int8 groups and back (format in
 // gdn_recurrence.cuh: 128 values of a row share one power of two).
 //
-// A warp takes kPackRows groups at once, loads them all before it works on the
-// first, finds each group's largest magnitude with one warp reduction on the
-// fp32 bits, and writes a byte per value and a byte per group.  Bound by HBM:
-// 3 bytes a value each way for 2-byte types.
+// A warp takes kItems groups of one tensor, loads them all before it works on
+// the first, finds each group's largest magnitude with one warp reduction, and
+// writes a byte a value and a byte a group: 3 bytes a value each way for 2-byte
+// types, bound by HBM.  Where a tensor's groups follow one another in memory
+// (full groups, rows without gaps) a group's place is its number; elsewhere it
+// takes two 32-bit divisions a group.
 #include "gdn_recurrence.cuh"
 
 namespace gdn {
 namespace rec {
 
 constexpr int kPackTensors = 4;  // tensors of one launch
-constexpr int kPackRows = 4;
+constexpr int kItems = 8;
 
 struct PackTensor {
-  const void *data;  // pack: the input; unpack: unused
-  void *out;         // unpack: the output [rows, cols]
+  void *data;        // pack: the input; unpack: the output [rows, cols]
   uint8_t *values;   // [rows, cols] int8
   uint8_t *scales;   // [rows, groups]
-  int64_t inner, outer_stride, inner_stride;  // row r lies at r / inner, r % inner
-  int64_t cols, groups;
-  int64_t first;     // number of the tensor's first group in the launch
+  int64_t outer_stride, inner_stride;  // row r lies at r / inner, r % inner
+  int64_t cols;
+  uint32_t inner, groups, items;
+  uint32_t first;    // the tensor's first warp in the launch
+  int flat;          // groups follow one another
 };
 struct Pack {
   PackTensor t[kPackTensors];
   int count;
-  int64_t items;
 };
 
-// The tensor that group `item` belongs to (an index, so that the launch
-// argument is not copied).
-__device__ __forceinline__ int tensor_of(const Pack &p, int64_t item) {
+// A group's elements, from the start of the data (as it lies) and of the values.
+struct Place {
+  int64_t data, values;
+  int left;  // values of the row from there on
+};
+__device__ __forceinline__ Place place_of(const PackTensor &t, uint32_t item, bool unpack) {
+  if (t.flat) return Place{static_cast<int64_t>(item) * kGroupValues, static_cast<int64_t>(item) * kGroupValues, kGroupValues};
+  const uint32_t row = item / t.groups, c0 = (item - row * t.groups) * kGroupValues;
+  const int64_t values = row * t.cols + c0;
+  const uint32_t outer = row / t.inner;
+  return Place{unpack ? values : outer * t.outer_stride + (row - outer * t.inner) * t.inner_stride + c0, values,
+               static_cast<int>(min(t.cols - c0, int64_t{kGroupValues}))};
+}
+__device__ __forceinline__ int tensor_of(const Pack &p, uint32_t warp) {
   int k = 0;
 #pragma unroll
-  for (int i = 1; i < kPackTensors; ++i) k = i < p.count && item >= p.t[i].first ? i : k;
+  for (int i = 1; i < kPackTensors; ++i) k = i < p.count && warp >= p.t[i].first ? i : k;
   return k;
 }
 
 template <typename E, bool kVec>
 __global__ void __launch_bounds__(kThreads) checkpoint_pack_kernel(const __grid_constant__ Pack p) {
   const int lane = threadIdx.x & 31;
-  const int64_t item0 = (static_cast<int64_t>(blockIdx.x) * kWarps + (threadIdx.x >> 5)) * kPackRows;
-  Raw<E> raw[kPackRows];
-  int left[kPackRows];
+  const uint32_t warp = blockIdx.x * kWarps + (threadIdx.x >> 5);
+  const PackTensor &t = p.t[tensor_of(p, warp)];
+  const uint32_t item0 = (warp - t.first) * kItems;
+  if (item0 >= t.items) return;
+  const int n = static_cast<int>(min(t.items - item0, uint32_t{kItems}));
+  Raw<E> raw[kItems];
 #pragma unroll
-  for (int i = 0; i < kPackRows; ++i) {
+  for (int i = 0; i < kItems; ++i) {
     raw[i] = {};
-    left[i] = 0;
-    if (item0 + i < p.items) {
-      const PackTensor &t = p.t[tensor_of(p, item0 + i)];
-      const int64_t n = item0 + i - t.first, row = n / t.groups, c0 = n % t.groups * kGroupValues;
-      left[i] = static_cast<int>(min(t.cols - c0, int64_t{kGroupValues}));
-      raw[i] = load4<E, kVec>(static_cast<const E *>(t.data) + row / t.inner * t.outer_stride +
-                                  row % t.inner * t.inner_stride + c0, lane, left[i]);
+    if (i < n) {
+      const Place at = place_of(t, item0 + i, false);
+      raw[i] = load4<E, kVec>(static_cast<const E *>(t.data) + at.data, lane, at.left);
     }
   }
+  uint32_t mine = 0;  // lane i: the exponent of group i
 #pragma unroll
-  for (int i = 0; i < kPackRows; ++i) {
-    if (item0 + i >= p.items) break;
-    const PackTensor &t = p.t[tensor_of(p, item0 + i)];
-    const int64_t n = item0 + i - t.first, row = n / t.groups, c0 = n % t.groups * kGroupValues;
+  for (int i = 0; i < kItems; ++i) {
+    if (i >= n) break;
+    const Place at = place_of(t, item0 + i, false);
     uint64_t a, b;
     raw[i].pairs(a, b);
     const uint32_t ex = group_exponent(__reduce_max_sync(0xffffffffu, abs_max_bits(a, b)), exp_cap<E>());
     const uint32_t q = quantise4(a, b, ex, exp_cap<E>());
-    uint8_t *dst = t.values + row * t.cols + c0;
+    uint8_t *dst = t.values + at.values;
     if constexpr (kVec) {
-      if (4 * lane < left[i]) reinterpret_cast<uint32_t *>(dst)[lane] = q;
+      if (4 * lane < at.left) reinterpret_cast<uint32_t *>(dst)[lane] = q;
     } else {
 #pragma unroll
       for (int j = 0; j < 4; ++j)
-        if (lane + 32 * j < left[i]) dst[lane + 32 * j] = static_cast<uint8_t>(q >> (8 * j));
+        if (lane + 32 * j < at.left) dst[lane + 32 * j] = static_cast<uint8_t>(q >> (8 * j));
     }
-    if (lane == 0) t.scales[n] = static_cast<uint8_t>(ex);
+    mine = lane == i ? ex : mine;
   }
+  if (lane < n) t.scales[item0 + lane] = static_cast<uint8_t>(mine);
 }
 
 template <typename E, bool kVec>
 __global__ void __launch_bounds__(kThreads) checkpoint_unpack_kernel(const __grid_constant__ Pack p) {
   const int lane = threadIdx.x & 31;
-  const int64_t item0 = (static_cast<int64_t>(blockIdx.x) * kWarps + (threadIdx.x >> 5)) * kPackRows;
-  uint32_t q[kPackRows], ex[kPackRows];
+  const uint32_t warp = blockIdx.x * kWarps + (threadIdx.x >> 5);
+  const PackTensor &t = p.t[tensor_of(p, warp)];
+  const uint32_t item0 = (warp - t.first) * kItems;
+  if (item0 >= t.items) return;
+  const int n = static_cast<int>(min(t.items - item0, uint32_t{kItems}));
+  const uint32_t mine = lane < n ? __ldg(t.scales + item0 + lane) : 0;
+  uint32_t q[kItems];
 #pragma unroll
-  for (int i = 0; i < kPackRows; ++i) {
-    q[i] = ex[i] = 0;
-    if (item0 + i < p.items) {
-      const PackTensor &t = p.t[tensor_of(p, item0 + i)];
-      const int64_t n = item0 + i - t.first, row = n / t.groups, c0 = n % t.groups * kGroupValues;
-      const int left = static_cast<int>(min(t.cols - c0, int64_t{kGroupValues}));
-      const uint8_t *src = t.values + row * t.cols + c0;
-      ex[i] = __ldg(t.scales + n);
+  for (int i = 0; i < kItems; ++i) {
+    q[i] = 0;
+    if (i < n) {
+      const Place at = place_of(t, item0 + i, true);
+      const uint8_t *src = t.values + at.values;
       if constexpr (kVec) {
-        if (4 * lane < left) q[i] = __ldg(reinterpret_cast<const uint32_t *>(src) + lane);
+        if (4 * lane < at.left) q[i] = __ldg(reinterpret_cast<const uint32_t *>(src) + lane);
       } else {
 #pragma unroll
         for (int j = 0; j < 4; ++j)
-          if (lane + 32 * j < left) q[i] |= static_cast<uint32_t>(src[lane + 32 * j]) << (8 * j);
+          if (lane + 32 * j < at.left) q[i] |= static_cast<uint32_t>(src[lane + 32 * j]) << (8 * j);
       }
     }
   }
 #pragma unroll
-  for (int i = 0; i < kPackRows; ++i) {
-    if (item0 + i >= p.items) break;
-    const PackTensor &t = p.t[tensor_of(p, item0 + i)];
-    const int64_t n = item0 + i - t.first, row = n / t.groups, c0 = n % t.groups * kGroupValues;
+  for (int i = 0; i < kItems; ++i) {
+    if (i >= n) break;
+    const Place at = place_of(t, item0 + i, true);
     uint64_t a, b;
-    dequantise4(q[i], ex[i], a, b);
-    store4<E, kVec>(static_cast<E *>(t.out) + row * t.cols + c0, lane,
-                    static_cast<int>(min(t.cols - c0, int64_t{kGroupValues})), a, b);
+    dequantise4(q[i], __shfl_sync(0xffffffffu, mine, i), a, b);
+    store4<E, kVec>(static_cast<E *>(t.data) + at.data, lane, at.left, a, b);
   }
 }
 
 template <typename E>
-cudaError_t launch_checkpoint_e(const Pack &p, bool vec, bool unpack, cudaStream_t stream) {
-  const int64_t per_block = kWarps * kPackRows;
-  const unsigned blocks = static_cast<unsigned>((p.items + per_block - 1) / per_block);
+cudaError_t launch_checkpoint_e(const Pack &p, uint32_t warps, bool vec, bool unpack, cudaStream_t stream) {
+  const unsigned blocks = (warps + kWarps - 1) / kWarps;
   auto kernel = unpack ? (vec ? checkpoint_unpack_kernel<E, true> : checkpoint_unpack_kernel<E, false>)
                        : (vec ? checkpoint_pack_kernel<E, true> : checkpoint_pack_kernel<E, false>);
   kernel<<<blocks, kThreads, 0, stream>>>(p);

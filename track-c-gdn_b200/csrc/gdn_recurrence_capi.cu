@@ -225,33 +225,41 @@ namespace {
 int checkpoint_call(int type, const gdn_checkpoint_tensor *tensors, int count, bool unpack, void *stream) {
   if (!known_type(type) || count < 0 || count > GDN_CHECKPOINT_MAX_TENSORS) return GDN_ERR_BAD_SIZE;
   if (count > 0 && !tensors) return GDN_ERR_NULL_POINTER;
+  using gdn::rec::kGroupValues;
   gdn::rec::Pack p{};
   bool vec = true;
+  int64_t warps = 0;
   for (int i = 0; i < count; ++i) {
     const gdn_checkpoint_tensor &t = tensors[i];
-    if (t.rows < 0 || t.cols < 0 || t.inner < 1 || t.rows > (int64_t{1} << 40) || t.cols > (int64_t{1} << 24))
+    if (t.rows < 0 || t.cols < 0 || t.inner < 1 || t.rows > INT32_MAX || t.inner > INT32_MAX ||
+        t.cols > (int64_t{1} << 24))
       return GDN_ERR_BAD_SIZE;
     if (t.rows == 0 || t.cols == 0) continue;
     if (!t.data || !t.values || !t.scales) return GDN_ERR_NULL_POINTER;
     if (!aligned(t.data, type_size(type))) return GDN_ERR_MISALIGNED;
-    gdn::rec::PackTensor &k = p.t[p.count];
-    k.data = t.data, k.out = t.data;
+    const int64_t groups = (t.cols + kGroupValues - 1) / kGroupValues, items = t.rows * groups;
+    if (items > INT32_MAX) return GDN_ERR_BAD_SIZE;
+    gdn::rec::PackTensor &k = p.t[p.count++];
+    k.data = t.data;
     k.values = static_cast<uint8_t *>(t.values), k.scales = static_cast<uint8_t *>(t.scales);
-    k.inner = t.inner, k.outer_stride = t.outer_stride, k.inner_stride = t.inner_stride;
-    k.cols = t.cols, k.groups = (t.cols + gdn::rec::kGroupValues - 1) / gdn::rec::kGroupValues;
-    k.first = p.items;
-    p.items += t.rows * k.groups;
-    ++p.count;
+    k.inner = static_cast<uint32_t>(t.inner), k.outer_stride = t.outer_stride, k.inner_stride = t.inner_stride;
+    k.cols = t.cols, k.groups = static_cast<uint32_t>(groups), k.items = static_cast<uint32_t>(items);
+    k.first = static_cast<uint32_t>(warps);
+    warps += (items + gdn::rec::kItems - 1) / gdn::rec::kItems;
+    const bool dense = unpack || t.rows == 1 ||
+                       ((t.inner == 1 || t.inner_stride == t.cols) && t.outer_stride == t.inner * t.cols);
+    k.flat = t.cols % kGroupValues == 0 && dense;
     vec = vec && t.cols % 4 == 0 && aligned(t.data, 4 * type_size(type)) && aligned(t.values, 4) &&
           (unpack || (t.outer_stride % 4 == 0 && t.inner_stride % 4 == 0));
   }
-  if (p.items == 0) return GDN_OK;
-  if (p.items > int64_t{INT32_MAX}) return GDN_ERR_BAD_SIZE;
+  if (warps == 0) return GDN_OK;
+  if (warps > INT32_MAX) return GDN_ERR_BAD_SIZE;
   if (int st = check_device(nullptr)) return st;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const cudaError_t e = type == GDN_BF16   ? gdn::rec::launch_checkpoint_e<__nv_bfloat16>(p, vec, unpack, s)
-                        : type == GDN_FP16 ? gdn::rec::launch_checkpoint_e<__half>(p, vec, unpack, s)
-                                           : gdn::rec::launch_checkpoint_e<float>(p, vec, unpack, s);
+  const uint32_t w = static_cast<uint32_t>(warps);
+  const cudaError_t e = type == GDN_BF16   ? gdn::rec::launch_checkpoint_e<__nv_bfloat16>(p, w, vec, unpack, s)
+                        : type == GDN_FP16 ? gdn::rec::launch_checkpoint_e<__half>(p, w, vec, unpack, s)
+                                           : gdn::rec::launch_checkpoint_e<float>(p, w, vec, unpack, s);
   return e == cudaSuccess ? GDN_OK : GDN_ERR_LAUNCH;
 }
 
