@@ -50,6 +50,30 @@ __device__ __forceinline__ int tensor_of(const Pack &p, uint32_t warp) {
   return k;
 }
 
+// The largest magnitude of a lane's four values, as bits whose order is that of
+// the values (16 bits, twice, for 2-byte types), and those bits as an fp32's.
+__device__ __forceinline__ uint32_t lane_max(const Raw<__nv_bfloat16> &r) {
+  const __nv_bfloat162 a = *reinterpret_cast<const __nv_bfloat162 *>(&r.v.x);
+  const __nv_bfloat162 b = *reinterpret_cast<const __nv_bfloat162 *>(&r.v.y);
+  const __nv_bfloat162 m = __hmax2_nan(__habs2(a), __habs2(b)), n = __hmax2_nan(m, __lowhigh2highlow(m));
+  return *reinterpret_cast<const uint32_t *>(&n);
+}
+__device__ __forceinline__ uint32_t lane_max(const Raw<__half> &r) {
+  const __half2 a = *reinterpret_cast<const __half2 *>(&r.v.x), b = *reinterpret_cast<const __half2 *>(&r.v.y);
+  const __half2 m = __hmax2_nan(__habs2(a), __habs2(b)), n = __hmax2_nan(m, __lowhigh2highlow(m));
+  return *reinterpret_cast<const uint32_t *>(&n);
+}
+__device__ __forceinline__ uint32_t lane_max(const Raw<float> &r) {
+  return abs_max_bits(f2_pack(r.v.x, r.v.y), f2_pack(r.v.z, r.v.w));
+}
+template <typename E>
+__device__ __forceinline__ uint32_t magnitude(uint32_t m) {
+  if constexpr (std::is_same<E, float>::value) return m;
+  if constexpr (std::is_same<E, __half>::value)
+    return __float_as_uint(__half2float(__ushort_as_half(static_cast<uint16_t>(m))));
+  return m << 16;
+}
+
 template <typename E, bool kVec>
 __global__ void __launch_bounds__(kThreads) checkpoint_pack_kernel(const __grid_constant__ Pack p) {
   const int lane = threadIdx.x & 31;
@@ -59,6 +83,39 @@ __global__ void __launch_bounds__(kThreads) checkpoint_pack_kernel(const __grid_
   if (item0 >= t.items) return;
   const int n = static_cast<int>(min(t.items - item0, uint32_t{kItems}));
   Raw<E> raw[kItems];
+  if (kVec && t.flat && n == kItems) {
+    // groups one after the other; lane i works out the scale of group i
+    const E *src = static_cast<const E *>(t.data) + static_cast<int64_t>(item0) * kGroupValues;
+    uint32_t *dst = reinterpret_cast<uint32_t *>(t.values + static_cast<int64_t>(item0) * kGroupValues) + lane;
+#pragma unroll
+    for (int i = 0; i < kItems; ++i) raw[i] = load4<E, kVec>(src + i * kGroupValues, lane, kGroupValues);
+    uint32_t top = 0;
+#pragma unroll
+    for (int i = 0; i < kItems; ++i) {
+      const uint32_t m = __reduce_max_sync(0xffffffffu, lane_max(raw[i]));
+      top = lane == i ? m : top;
+    }
+    const uint32_t ex = group_exponent(magnitude<E>(top), exp_cap<E>());
+    if (lane < kItems) t.scales[item0 + lane] = static_cast<uint8_t>(ex);
+    if (__all_sync(0xffffffffu, ex < exp_cap<E>())) {
+      const float inv = group_inverse(ex);
+#pragma unroll
+      for (int i = 0; i < kItems; ++i) {
+        uint64_t a, b;
+        raw[i].pairs(a, b);
+        const float f = __shfl_sync(0xffffffffu, inv, i);
+        dst[i * (kGroupValues / 4)] = __byte_perm(quantise2(a, f), quantise2(b, f), 0x5410);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < kItems; ++i) {
+        uint64_t a, b;
+        raw[i].pairs(a, b);
+        dst[i * (kGroupValues / 4)] = quantise4(a, b, __shfl_sync(0xffffffffu, ex, i), exp_cap<E>());
+      }
+    }
+    return;
+  }
 #pragma unroll
   for (int i = 0; i < kItems; ++i) {
     raw[i] = {};
@@ -98,6 +155,38 @@ __global__ void __launch_bounds__(kThreads) checkpoint_unpack_kernel(const __gri
   if (item0 >= t.items) return;
   const int n = static_cast<int>(min(t.items - item0, uint32_t{kItems}));
   const uint32_t mine = lane < n ? __ldg(t.scales + item0 + lane) : 0;
+  if (kVec && t.flat && n == kItems) {
+    // groups one after the other: 8 values a lane, two groups a load
+    const uint2 *src = reinterpret_cast<const uint2 *>(t.values + static_cast<int64_t>(item0) * kGroupValues) + lane;
+    E *dst = static_cast<E *>(t.data) + static_cast<int64_t>(item0) * kGroupValues + 8 * lane;
+    uint2 v[kItems / 2];
+#pragma unroll
+    for (int i = 0; i < kItems / 2; ++i) v[i] = __ldg(src + 32 * i);
+#pragma unroll
+    for (int i = 0; i < kItems / 2; ++i) {
+      uint64_t a, b, c, d;
+      const uint32_t ex = __shfl_sync(0xffffffffu, mine, 2 * i + (lane >> 4));
+      dequantise4(v[i].x, ex, a, b);
+      dequantise4(v[i].y, ex, c, d);
+      E *at = dst + 2 * i * kGroupValues;
+      if constexpr (sizeof(E) == 4) {
+        reinterpret_cast<float4 *>(at)[0] = make_float4(f2_lo(a), f2_hi(a), f2_lo(b), f2_hi(b));
+        reinterpret_cast<float4 *>(at)[1] = make_float4(f2_lo(c), f2_hi(c), f2_lo(d), f2_hi(d));
+      } else {
+        uint4 u;
+        if constexpr (std::is_same<E, __half>::value) {
+          const __half2 h[4] = {__floats2half2_rn(f2_lo(a), f2_hi(a)), __floats2half2_rn(f2_lo(b), f2_hi(b)),
+                                __floats2half2_rn(f2_lo(c), f2_hi(c)), __floats2half2_rn(f2_lo(d), f2_hi(d))};
+          memcpy(&u, h, sizeof(u));
+        } else {
+          u = make_uint4(pack_bf16x2(f2_lo(a), f2_hi(a)), pack_bf16x2(f2_lo(b), f2_hi(b)),
+                         pack_bf16x2(f2_lo(c), f2_hi(c)), pack_bf16x2(f2_lo(d), f2_hi(d)));
+        }
+        *reinterpret_cast<uint4 *>(at) = u;
+      }
+    }
+    return;
+  }
   uint32_t q[kItems];
 #pragma unroll
   for (int i = 0; i < kItems; ++i) {

@@ -248,7 +248,7 @@ int checkpoint_call(int type, const gdn_checkpoint_tensor *tensors, int count, b
     warps += (items + gdn::rec::kItems - 1) / gdn::rec::kItems;
     const bool dense = unpack || t.rows == 1 ||
                        ((t.inner == 1 || t.inner_stride == t.cols) && t.outer_stride == t.inner * t.cols);
-    k.flat = t.cols % kGroupValues == 0 && dense;
+    k.flat = t.cols % kGroupValues == 0 && dense && (!unpack || (aligned(t.data, 16) && aligned(t.values, 8)));
     vec = vec && t.cols % 4 == 0 && aligned(t.data, 4 * type_size(type)) && aligned(t.values, 4) &&
           (unpack || (t.outer_stride % 4 == 0 && t.inner_stride % 4 == 0));
   }
