@@ -14,6 +14,7 @@ between forward and backward.  No counterpart in the reference.
 from __future__ import annotations
 
 import ctypes
+import math
 from typing import List, Optional, Sequence
 
 import torch
@@ -28,10 +29,11 @@ MAX_TENSORS = 4  # of one launch; more take several
 class Packed:
     """Tensors of one type in 8 bits: one buffer, and what was put into it."""
 
-    __slots__ = ("buffer", "dtype", "shapes", "offsets")
+    __slots__ = ("buffer", "dtype", "shapes", "places")
 
-    def __init__(self, buffer, dtype, shapes, offsets):
-        self.buffer, self.dtype, self.shapes, self.offsets = buffer, dtype, shapes, offsets
+    def __init__(self, buffer, dtype, shapes, places):
+        # places: per tensor where its values and its scales start, rows, columns
+        self.buffer, self.dtype, self.shapes, self.places = buffer, dtype, shapes, places
 
     def __len__(self):
         return len(self.shapes)
@@ -41,45 +43,43 @@ class Packed:
 
     def values(self, i: int) -> torch.Tensor:
         """The int8 values of tensor i, in its shape (a view of the buffer)."""
-        shape, at = self.shapes[i], self.offsets[i]
+        shape, at = self.shapes[i], self.places[i][0]
         return self.buffer[at:at + _count(shape)].view(torch.int8).view(shape)
 
     def scales(self, i: int) -> torch.Tensor:
         """The exponent bytes E (scale 2^(E-127); 255: not finite) of tensor i,
         [..., ceil(last / 128)] uint8 (a view of the buffer)."""
-        shape, at = self.shapes[i], self.offsets[i]
-        at += -(-_count(shape) // 16) * 16
+        shape, at = self.shapes[i], self.places[i][1]
         shape = (*shape[:-1], -(-shape[-1] // GROUP))
         return self.buffer[at:at + _count(shape)].view(shape)
 
 
 def _count(shape) -> int:
-    n = 1
-    for s in shape:
-        n *= s
-    return n
+    return math.prod(shape)
 
 
 def _layout(shapes):
-    """Bytes in all, and where each tensor's values and scales start (values on
-    16-byte boundaries, scales behind them on the next)."""
-    offsets, scales, at = [], [], 0
+    """Bytes in all, and for each tensor where its values and scales start
+    (values on 16-byte boundaries, scales behind them on the next), its rows
+    and its columns."""
+    places, at = [], 0
     for shape in shapes:
-        n, c = _count(shape), shape[-1]
-        offsets.append(at)
-        at += -(-n // 16) * 16
-        scales.append(at)
-        groups = n // c * -(-c // GROUP) if c else 0
-        at += -(-groups // 16) * 16
-    return at, offsets, scales
+        c = shape[-1]
+        n = math.prod(shape)
+        rows = n // c if c else 0
+        scales = at + (n + 15) // 16 * 16
+        places.append((at, scales, rows, c))
+        at = scales + (rows * -(-c // GROUP) + 15) // 16 * 16
+    return at, places
 
 
 def _strides(t: torch.Tensor):
     """(tensor, inner, outer stride, inner stride): row r of the last dimension
     lies at r // inner * outer + r % inner * inner stride."""
+    if t.is_contiguous() or t.dim() == 1 and t.stride(0) == 1:
+        return t, 1, t.shape[-1], 0
     if t.stride(-1) != 1 and t.shape[-1] != 1:
         t = t.contiguous()
-    if t.is_contiguous() or t.dim() == 1:
         return t, 1, t.shape[-1], 0
     if t.dim() == 2:
         return t, 1, t.stride(0), 0
@@ -107,44 +107,40 @@ def _descriptors(rows):
     return (ctypes.c_int64 * len(flat))(*flat)
 
 
-@torch.no_grad()
 def pack(*tensors: torch.Tensor) -> Packed:
     """The 8-bit form of tensors of one type on one device (up to 4 a launch)."""
     dtype, device = _check(tensors)
     shapes = [tuple(t.shape) for t in tensors]
-    total, offsets, scales = _layout(shapes)
+    total, places = _layout(shapes)
     buffer = torch.empty(total, dtype=torch.uint8, device=device)
     at, rows, keep = buffer.data_ptr(), [], []
-    for t, o, s in zip(tensors, offsets, scales):
-        t, inner, outer_stride, inner_stride = _strides(t)
+    for t, (values, scales, n, c) in zip(tensors, places):
+        t, inner, outer_stride, inner_stride = _strides(t.detach())
         keep.append(t)
-        c = t.shape[-1]
-        rows.append((t.data_ptr(), at + o, at + s, t.numel() // c if c else 0, c, inner, outer_stride, inner_stride))
+        rows.append((t.data_ptr(), at + values, at + scales, n, c, inner, outer_stride, inner_stride))
     for i in range(0, len(rows), MAX_TENSORS):
         part = rows[i:i + MAX_TENSORS]
-        _call("gdn_checkpoint_pack", device, (_TYPES[dtype], _descriptors(part), len(part)), None)
-    return Packed(buffer, dtype, shapes, offsets)
+        _call(_native.lib.gdn_checkpoint_pack, device, (_TYPES[dtype], _descriptors(part), len(part)), None)
+    return Packed(buffer, dtype, shapes, places)
 
 
 def unpack_into(packed: Packed, outs: Sequence[torch.Tensor], stream: Optional[int] = None) -> None:
     """Writes the values that `packed` stands for into contiguous tensors of the
     packed shapes and type."""
     assert len(outs) == len(packed)
+    device = packed.buffer.device
     at, rows = packed.buffer.data_ptr(), []
-    _, offsets, scales = _layout(packed.shapes)
-    for t, shape, o, s in zip(outs, packed.shapes, offsets, scales):
-        assert tuple(t.shape) == shape and t.dtype == packed.dtype and t.is_contiguous()
-        if t.device != packed.buffer.device:
-            raise ValueError(f"an output is on {t.device}, the checkpoint on {packed.buffer.device}")
-        c = shape[-1]
-        rows.append((t.data_ptr(), at + o, at + s, t.numel() // c if c else 0, c, 1, c, 0))
+    for t, shape, (values, scales, n, c) in zip(outs, packed.shapes, packed.places):
+        assert t.shape == shape and t.dtype == packed.dtype and t.is_contiguous()
+        if t.device != device:
+            raise ValueError(f"an output is on {t.device}, the checkpoint on {device}")
+        rows.append((t.data_ptr(), at + values, at + scales, n, c, 1, c, 0))
     for i in range(0, len(rows), MAX_TENSORS):
         part = rows[i:i + MAX_TENSORS]
-        _call("gdn_checkpoint_unpack", packed.buffer.device, (_TYPES[packed.dtype], _descriptors(part), len(part)),
+        _call(_native.lib.gdn_checkpoint_unpack, device, (_TYPES[packed.dtype], _descriptors(part), len(part)),
               stream)
 
 
-@torch.no_grad()
 def unpack(packed: Packed) -> List[torch.Tensor]:
     """The tensors that `packed` stands for, in their shapes and type."""
     outs = [torch.empty(s, dtype=packed.dtype, device=packed.buffer.device) for s in packed.shapes]

@@ -544,7 +544,8 @@ cudaError_t launch_backward_t(Backward p, void *workspace, int sms, float *dA_lo
     if (!ok) return cudaErrorInvalidValue;
   }
   auto kernel = recurrence_backward_kernel<E, kTma, kPacked>;
-  if (cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem)) return e;
+  static std::atomic<uint64_t> allowed;
+  if (cudaError_t e = allow_shared(kernel, smem, allowed)) return e;
   const Places w = places(workspace, p.s.T, p.D);
   p.hdr = static_cast<Header *>(workspace);
   p.maps = w.words;

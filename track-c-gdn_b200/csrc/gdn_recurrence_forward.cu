@@ -556,7 +556,8 @@ cudaError_t launch_forward_t(Forward p, void *workspace, int sms, cudaStream_t s
   const bool serial = chunks <= kSerialChunks && (p.s.cu == nullptr || p.s.N <= kSerialSeqs);
   auto kernel = serial ? recurrence_forward_kernel<E, kTma, kPack, false>
                        : recurrence_forward_kernel<E, kTma, kPack, true>;
-  if (cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem)) return e;
+  static std::atomic<uint64_t> allowed[2];
+  if (cudaError_t e = allow_shared(kernel, smem, allowed[serial])) return e;
   int64_t blocks = nt;
   if (!serial) {
     p.hdr = static_cast<Header *>(workspace);

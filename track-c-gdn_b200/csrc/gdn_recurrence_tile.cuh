@@ -4,6 +4,7 @@
 #pragma once
 #include <cuda.h>
 
+#include <atomic>
 #include <type_traits>
 
 #include "gdn_recurrence.cuh"
@@ -433,6 +434,18 @@ __device__ __forceinline__ void mbar_expect_tx(uint32_t mbar, uint32_t bytes) {
 }
 __device__ __forceinline__ void mbar_arrive(uint32_t mbar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(mbar) : "memory");
+}
+
+// Allows a kernel its dynamic shared memory, once per device.
+template <typename K>
+cudaError_t allow_shared(K kernel, int bytes, std::atomic<uint64_t> &done) {
+  int dev = 0;
+  if (cudaError_t e = cudaGetDevice(&dev)) return e;
+  const uint64_t bit = dev < 64 ? uint64_t{1} << dev : 0;
+  if (bit && (done.load(std::memory_order_acquire) & bit)) return cudaSuccess;
+  if (cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes)) return e;
+  done.fetch_or(bit, std::memory_order_release);
+  return cudaSuccess;
 }
 
 // ---- host ---------------------------------------------------------------------

@@ -44,18 +44,21 @@ def _copied(t: torch.Tensor, stream):
     if stream is not None:
         raise ValueError("with `stream` the inputs must be laid out as the kernels read them "
                          "(channels side by side, one distance between tokens)")
-    return t.contiguous()
+    return t.detach().contiguous()
 
 
 def _rows(t: torch.Tensor, stream=None):
     """`t` as rows of channels: (tensor that owns them, elements between rows)."""
-    if t.stride(-1) != 1 and t.shape[-1] != 1:
+    strides, shape = t.stride(), t.shape
+    if strides[-1] != 1 and shape[-1] != 1:
         t = _copied(t, stream)
-    if t.dim() == 2:
-        return t, t.stride(0)
-    if t.shape[0] != 1 and t.shape[1] != 1 and t.stride(0) != t.shape[1] * t.stride(1):
+        strides = t.stride()
+    if len(strides) == 2:
+        return t, strides[0]
+    if shape[0] != 1 and shape[1] != 1 and strides[0] != shape[1] * strides[1]:
         t = _copied(t, stream)
-    return t, (t.stride(0) if t.shape[1] == 1 else t.stride(1))
+        strides = t.stride()
+    return t, (strides[0] if shape[1] == 1 else strides[1])
 
 
 def _vector(t: torch.Tensor, stream):
@@ -110,18 +113,22 @@ def _check_slots(slots, count, pool, D, device):
         raise ValueError(f"the pool ({pool.device}) and slots ({slots.device}) must be on {device}")
 
 
-def _call(name, device, args, stream):
-    """Calls the library with `device` current, on `stream` or the device's current stream."""
+_current_stream, _current_device = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice
+
+
+def _call(fn, device, args, stream):
+    """Calls the library's `fn` with `device` current, on `stream` or the
+    device's current stream."""
+    index = device.index
     if stream is None:
-        stream = torch.cuda.current_stream(device).cuda_stream
-    fn = getattr(_native.lib, name)
-    if device.index == torch.cuda.current_device():
+        stream = _current_stream(index)
+    if index == _current_device():
         st = fn(*args, stream)
     else:
-        with torch.cuda.device(device):
+        with torch.cuda.device(index):
             st = fn(*args, stream)
     if st:
-        _native.check(st, name)
+        _native.check(st, fn.__name__)
 
 
 def _ptr(t: Optional[torch.Tensor]):
@@ -166,13 +173,12 @@ def decode_into(x, state, A_log, a, dt_bias, b, out, new_state, slots: Optional[
     a, as_ = _rows(a, stream)
     b, bs = _rows(b, stream)
     A_log, dt_bias = _vector(A_log, stream), _vector(dt_bias, stream)
-    _call("gdn_recurrence_decode", device,
+    _call(_native.lib.gdn_recurrence_decode, device,
           (_TYPES[x.dtype], x.data_ptr(), xs, a.data_ptr(), as_, b.data_ptr(), bs, A_log.data_ptr(),
            dt_bias.data_ptr(), _ptr(state), _ptr(slots), 0 if slots is None else state.shape[0], B, T, D,
            out.data_ptr(), new_state.data_ptr(), _ptr(intermediate)), stream)
 
 
-@torch.no_grad()
 def decode(x, state, A_log, a, dt_bias, b, return_intermediate: bool = False):
     """Decode with a fresh new state: x, a, b [B, D] or [B, T, D], state [B, D]
     fp32 or None.  Returns (out, new_state), and with return_intermediate the
@@ -188,7 +194,6 @@ def decode(x, state, A_log, a, dt_bias, b, return_intermediate: bool = False):
     return (out, new_state, inter) if return_intermediate else (out, new_state)
 
 
-@torch.no_grad()
 def decode_inplace(x, state, A_log, a, dt_bias, b):
     """Decode with `state` [B, D] updated in place.  Returns out."""
     out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
@@ -196,7 +201,6 @@ def decode_inplace(x, state, A_log, a, dt_bias, b):
     return out
 
 
-@torch.no_grad()
 def decode_pool(x, state_pool, slots, A_log, a, dt_bias, b):
     """Decode with request i's state in state_pool[slots[i]] ([P, D] fp32,
     updated in place; slots [B] int32, distinct).  Returns out."""
@@ -237,7 +241,7 @@ def _prefill(x, state, A_log, a, dt_bias, b, cu_seqlens, out, final_state, works
     b, bs = _rows(b, stream)
     A_log, dt_bias = _vector(A_log, stream), _vector(dt_bias, stream)
     wptr, wbytes = _aligned(workspace)
-    _call("gdn_recurrence_prefill", device,
+    _call(_native.lib.gdn_recurrence_prefill, device,
           (_TYPES[x.dtype], x.data_ptr(), xs, a.data_ptr(), as_, b.data_ptr(), bs, A_log.data_ptr(),
            dt_bias.data_ptr(), _ptr(state), _ptr(slots), 0 if slots is None else state.shape[0], cu, N, T, D,
            int(zero_behind), out.data_ptr(), final_state.data_ptr(), _ptr(carries), _ptr(packed), wptr, wbytes),
@@ -252,7 +256,6 @@ def run_into(x, state, A_log, a, dt_bias, b, cu_seqlens, out, final_state, works
     _prefill(x, state, A_log, a, dt_bias, b, cu_seqlens, out, final_state, workspace, stream=stream)
 
 
-@torch.no_grad()
 def run(x, state, A_log, a, dt_bias, b, cu_seqlens: Optional[torch.Tensor] = None):
     """Prefill of packed (x [T, D], cu_seqlens [N+1] int64) or dense sequences
     (x [N, S, D], or one sequence [S, D]).  state [N, D] fp32 or None.  Returns
@@ -274,7 +277,6 @@ def run_pool_into(x, state_pool, slots, A_log, a, dt_bias, b, cu_seqlens, out, w
              stream=stream)
 
 
-@torch.no_grad()
 def run_pool(x, state_pool, slots, A_log, a, dt_bias, b, cu_seqlens: Optional[torch.Tensor] = None):
     """`run` with the states in a pool ([P, D] fp32, updated in place at
     slots [N] int32, distinct).  Returns out."""
@@ -320,7 +322,7 @@ def _backward(x, state, A_log, a, dt_bias, b, cu_seqlens, d_out, d_final_state, 
     d_out, ds = _rows(d_out, stream)
     A_log, dt_bias = _vector(A_log, stream), _vector(dt_bias, stream)
     wptr, wbytes = _aligned(workspace)
-    _call("gdn_recurrence_backward", device,
+    _call(_native.lib.gdn_recurrence_backward, device,
           (_TYPES[dtype], _ptr(x), strides[0], _ptr(a), strides[1], _ptr(b), strides[2], _ptr(packed),
            A_log.data_ptr(), dt_bias.data_ptr(), _ptr(state), cu, N, T, D, int(zero_behind), d_out.data_ptr(), ds,
            _ptr(d_final_state), _ptr(carries), dx.data_ptr(), da.data_ptr(), db.data_ptr(), dA_log.data_ptr(),
