@@ -25,6 +25,7 @@ own).  No counterpart in the reference.
 """
 from __future__ import annotations
 
+from functools import lru_cache
 from typing import Optional
 
 import torch
@@ -212,6 +213,7 @@ def decode_pool(x, state_pool, slots, A_log, a, dt_bias, b):
 # ---------------------------------------------------------------------------
 # prefill
 # ---------------------------------------------------------------------------
+@lru_cache(maxsize=256)
 def workspace_bytes(total_tokens: int, channels: int) -> int:
     return int(_native.lib.gdn_recurrence_workspace_bytes(total_tokens, channels))
 
@@ -236,16 +238,23 @@ def _prefill(x, state, A_log, a, dt_bias, b, cu_seqlens, out, final_state, works
         _check_states("final_state", final_state, N, D, device)
         assert final_state.is_contiguous(), "final_state must be contiguous"
     assert out.shape == x.shape and out.dtype == x.dtype and out.is_contiguous() and out.device == device
+    _launch_prefill(x, state, A_log, a, dt_bias, b, (T, N, cu), out, final_state, workspace, slots, carries, packed,
+                    zero_behind, stream)
+
+
+def _launch_prefill(x, state, A_log, a, dt_bias, b, seqs, out, final_state, workspace, slots, carries, packed,
+                    zero_behind, stream):
+    T, N, cu = seqs
     x, xs = _rows(x, stream)
     a, as_ = _rows(a, stream)
     b, bs = _rows(b, stream)
     A_log, dt_bias = _vector(A_log, stream), _vector(dt_bias, stream)
     wptr, wbytes = _aligned(workspace)
-    _call(_native.lib.gdn_recurrence_prefill, device,
+    _call(_native.lib.gdn_recurrence_prefill, x.device,
           (_TYPES[x.dtype], x.data_ptr(), xs, a.data_ptr(), as_, b.data_ptr(), bs, A_log.data_ptr(),
-           dt_bias.data_ptr(), _ptr(state), _ptr(slots), 0 if slots is None else state.shape[0], cu, N, T, D,
-           int(zero_behind), out.data_ptr(), final_state.data_ptr(), _ptr(carries), _ptr(packed), wptr, wbytes),
-          stream)
+           dt_bias.data_ptr(), _ptr(state), _ptr(slots), 0 if slots is None else state.shape[0], cu, N, T,
+           x.shape[-1], int(zero_behind), out.data_ptr(), final_state.data_ptr(), _ptr(carries), _ptr(packed), wptr,
+           wbytes), stream)
 
 
 def run_into(x, state, A_log, a, dt_bias, b, cu_seqlens, out, final_state, workspace: torch.Tensor,
@@ -290,6 +299,7 @@ def run_pool(x, state_pool, slots, A_log, a, dt_bias, b, cu_seqlens: Optional[to
 # ---------------------------------------------------------------------------
 # backward
 # ---------------------------------------------------------------------------
+@lru_cache(maxsize=256)
 def backward_workspace_bytes(total_tokens: int, channels: int) -> int:
     return int(_native.lib.gdn_recurrence_backward_workspace_bytes(total_tokens, channels))
 
@@ -312,19 +322,28 @@ def _backward(x, state, A_log, a, dt_bias, b, cu_seqlens, d_out, d_final_state, 
         if t is not None:
             _check_states(name, t, N, D, device)
             assert t.is_contiguous(), f"{name} must be contiguous"
-    strides = [0, 0, 0]
     if packed is None:
         _check_inputs(x, a, b, A_log, dt_bias)
         assert x.shape == d_out.shape and x.dtype == dtype and x.device == device, "d_out must be like x"
-        x, strides[0] = _rows(x, stream)
-        a, strides[1] = _rows(a, stream)
-        b, strides[2] = _rows(b, stream)
+    _launch_backward(x, state, A_log, a, dt_bias, b, (T, N, cu), d_out, d_final_state,
+                     (dx, da, db, dA_log, ddt_bias, d_state), workspace, carries, packed, zero_behind, stream)
+
+
+def _launch_backward(x, state, A_log, a, dt_bias, b, seqs, d_out, d_final_state, grads, workspace, carries, packed,
+                     zero_behind, stream):
+    T, N, cu = seqs
+    xs = as_ = bs = 0
+    if packed is None:
+        x, xs = _rows(x, stream)
+        a, as_ = _rows(a, stream)
+        b, bs = _rows(b, stream)
     d_out, ds = _rows(d_out, stream)
     A_log, dt_bias = _vector(A_log, stream), _vector(dt_bias, stream)
     wptr, wbytes = _aligned(workspace)
-    _call(_native.lib.gdn_recurrence_backward, device,
-          (_TYPES[dtype], _ptr(x), strides[0], _ptr(a), strides[1], _ptr(b), strides[2], _ptr(packed),
-           A_log.data_ptr(), dt_bias.data_ptr(), _ptr(state), cu, N, T, D, int(zero_behind), d_out.data_ptr(), ds,
+    dx, da, db, dA_log, ddt_bias, d_state = grads
+    _call(_native.lib.gdn_recurrence_backward, d_out.device,
+          (_TYPES[d_out.dtype], _ptr(x), xs, _ptr(a), as_, _ptr(b), bs, _ptr(packed), A_log.data_ptr(),
+           dt_bias.data_ptr(), _ptr(state), cu, N, T, d_out.shape[-1], int(zero_behind), d_out.data_ptr(), ds,
            _ptr(d_final_state), _ptr(carries), dx.data_ptr(), da.data_ptr(), db.data_ptr(), dA_log.data_ptr(),
            ddt_bias.data_ptr(), _ptr(d_state), wptr, wbytes), stream)
 
@@ -341,12 +360,15 @@ def backward_into(x, state, A_log, a, dt_bias, b, cu_seqlens, d_out, d_final_sta
               d_state, workspace, stream=stream)
 
 
+_NAMES = ("dx", "da", "db", "dA_log", "ddt_bias", "d_state")
+
+
 def _gradients(like, D, N, need_d_state):
-    dev = like.device
-    g = {n: torch.empty(like.shape, dtype=like.dtype, device=dev) for n in ("dx", "da", "db")}
-    g.update({n: torch.empty(D, dtype=torch.float32, device=dev) for n in ("dA_log", "ddt_bias")})
-    g["d_state"] = torch.empty(N, D, dtype=torch.float32, device=dev) if need_d_state else None
-    return g
+    empty, dtype, dev, f32 = torch.empty, like.dtype, like.device, torch.float32
+    shape = like.shape
+    return (empty(shape, dtype=dtype, device=dev), empty(shape, dtype=dtype, device=dev),
+            empty(shape, dtype=dtype, device=dev), empty(D, dtype=f32, device=dev), empty(D, dtype=f32, device=dev),
+            empty(N, D, dtype=f32, device=dev) if need_d_state else None)
 
 
 @torch.no_grad()
@@ -358,9 +380,16 @@ def backward(x, state, A_log, a, dt_bias, b, cu_seqlens, d_out, d_final_state=No
     D = x.shape[-1]
     g = _gradients(x, D, N, need_d_state)
     _backward(x, None if state is None else state.contiguous(), A_log, a, dt_bias, b, cu_seqlens, d_out.to(x.dtype),
-              None if d_final_state is None else d_final_state.float().contiguous(), g["dx"], g["da"], g["db"],
-              g["dA_log"], g["ddt_bias"], g["d_state"], alloc_backward_workspace(T, D, x.device), zero_behind=True)
-    return g
+              None if d_final_state is None else d_final_state.float().contiguous(), *g,
+              alloc_backward_workspace(T, D, x.device), zero_behind=True)
+    return dict(zip(_NAMES, g))
+
+
+@lru_cache(maxsize=256)
+def _saved_bytes(total_tokens: int, channels: int):
+    lib = _native.lib
+    return (int(lib.gdn_recurrence_carry_bytes(total_tokens, channels)),
+            int(lib.gdn_recurrence_packed_bytes(total_tokens, channels)))
 
 
 class _RecurrenceFunction(torch.autograd.Function):
@@ -370,23 +399,26 @@ class _RecurrenceFunction(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, state, A_log, a, dt_bias, b, cu_seqlens, checkpoint):
-        T, N, _ = _sequences(x, cu_seqlens)
-        D, dev = x.shape[-1], x.device
+        D = _check_inputs(x, a, b, A_log, dt_bias)
+        seqs = T, N, _ = _sequences(x, cu_seqlens)
+        dev = x.device
         if state is not None:
+            _check_states("state", state, N, D, dev)
             state = state.contiguous()
         out = torch.empty(x.shape, dtype=x.dtype, device=dev)
         final_state = torch.empty(N, D, dtype=torch.float32, device=dev)
-        carries = torch.empty(int(_native.lib.gdn_recurrence_carry_bytes(T, D)), dtype=torch.uint8, device=dev)
+        carry_bytes, packed_bytes = _saved_bytes(T, D)
+        carries = torch.empty(carry_bytes, dtype=torch.uint8, device=dev)
         packed = None
         if checkpoint is not None:
-            packed = torch.empty(int(_native.lib.gdn_recurrence_packed_bytes(T, D)), dtype=torch.uint8, device=dev)
-        _prefill(x, state, A_log, a, dt_bias, b, cu_seqlens, out, final_state, alloc_workspace(T, D, dev),
-                 carries=carries, packed=packed, zero_behind=True)
+            packed = torch.empty(packed_bytes, dtype=torch.uint8, device=dev)
+        _launch_prefill(x, state, A_log, a, dt_bias, b, seqs, out, final_state, alloc_workspace(T, D, dev), None,
+                        carries, packed, True, None)
         if packed is None:
             ctx.save_for_backward(x, a, b, None, state, A_log, dt_bias, cu_seqlens, carries)
         else:
             ctx.save_for_backward(None, None, None, packed, state, A_log, dt_bias, cu_seqlens, carries)
-        ctx.like = (x.shape, x.dtype, dev, N)
+        ctx.like = (x.shape, x.dtype, dev, T, N)
         ctx.set_materialize_grads(False)
         return out, final_state
 
@@ -394,16 +426,16 @@ class _RecurrenceFunction(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, d_out, d_final):
         x, a, b, packed, state, A_log, dt_bias, cu_seqlens, carries = ctx.saved_tensors
-        shape, dtype, dev, N = ctx.like
+        shape, dtype, dev, T, N = ctx.like
         if d_out is None:
             d_out = torch.zeros(shape, dtype=dtype, device=dev)
         D = shape[-1]
         g = _gradients(d_out, D, N, state is not None and ctx.needs_input_grad[1])
-        T = d_out.numel() // D
-        _backward(x, state, A_log, a, dt_bias, b, cu_seqlens, d_out, None if d_final is None else d_final.contiguous(),
-                  g["dx"], g["da"], g["db"], g["dA_log"], g["ddt_bias"], g["d_state"],
-                  alloc_backward_workspace(T, D, dev), carries=carries, packed=packed, zero_behind=True)
-        return g["dx"], g["d_state"], g["dA_log"], g["da"], g["ddt_bias"], g["db"], None, None
+        _launch_backward(x, state, A_log, a, dt_bias, b, (T, N, _ptr(cu_seqlens)), d_out,
+                         None if d_final is None else d_final.contiguous(), g, alloc_backward_workspace(T, D, dev),
+                         carries, packed, True, None)
+        dx, da, db, dA_log, ddt_bias, d_state = g
+        return dx, d_state, dA_log, da, ddt_bias, db, None, None
 
 
 def run_autograd(x, state, A_log, a, dt_bias, b, cu_seqlens: Optional[torch.Tensor] = None,
@@ -418,5 +450,4 @@ def run_autograd(x, state, A_log, a, dt_bias, b, cu_seqlens: Optional[torch.Tens
     before the tokens restarted from exact ones at every 64th row."""
     if checkpoint not in (None, "int8"):
         raise ValueError(f"checkpoint must be None or 'int8', got {checkpoint!r}")
-    _check_inputs(x, a, b, A_log, dt_bias)
     return _RecurrenceFunction.apply(x, state, A_log, a, dt_bias, b, cu_seqlens, checkpoint)
