@@ -137,7 +137,9 @@ def backward(x, state, A_log, a, dt_bias, b, cu, d_out, d_final, eight=False):
             R, mag = k.g[t] * v, k.g[t] * mag
         d_state[n], d_state_err[n] = R, r + 2 * U * mag
     sig = torch.sigmoid(k.z)
-    rel_sig = (k.moved + 10) * U
+    # sigmoid(z) = exp(z - softplus(z)) by one exponential: w and softplus are off
+    # as above, their difference is rounded, 4 u for the exponential
+    rel_sig = (2 * k.moved + 3 * k.sp + 16) * U + k.sp * (k.moved + 8) * U
     slope = k.beta * (1 - k.beta)
     dx = k.beta * dh
     dx_err = dx.abs() * (k.rel_beta + U) + k.beta * dh_err

@@ -441,10 +441,10 @@ recurrence_backward_kernel(const __grid_constant__ Backward p) {
             const uint64_t sp = kept.x;
             beta[j] = kept.y;
             xs[j] = f2_mul(in[0], f2_fma(f2_mul(beta[j], f2_dup(-1.f)), beta[j], beta[j]));  // x beta (1 - beta)
-            // sigmoid(z) from e = exp(-|z|): r = 1 / (1 + e) or e r
-            const uint64_t w = f2_fma(in[1], f2_dup(kLog2e), par.dt), e = ex2_neg_abs(w), d1 = f2_add(e, f2_dup(1.f));
-            const uint64_t rz = f2_pack(rcp(f2_lo(d1)), rcp(f2_hi(d1))), erz = f2_mul(e, rz);
-            const uint64_t sig = f2_pack(f2_lo(w) >= 0.f ? f2_lo(rz) : f2_lo(erz), f2_hi(w) >= 0.f ? f2_hi(rz) : f2_hi(erz));
+            // sigmoid(z) = 2^(w - sp): z less softplus(z) is its logarithm (0 at
+            // most; the difference of two infinities counts as that)
+            const uint64_t w = f2_fma(in[1], f2_dup(kLog2e), par.dt), ls = f2_fma(sp, f2_dup(-1.f), w);
+            const uint64_t sig = ex2_pair(f2_pack(fminf(f2_lo(ls), 0.f), fminf(f2_hi(ls), 0.f)));
             g[j] = gate_ex2(f2_mul(par.c, sp));
             const uint64_t gh = f2_mul(g[j], h), cgh = f2_mul(par.c, gh);  // -exp(A_log) g h_{t-1}
             h = f2_fma(g[j], h, f2_mul(beta[j], in[0]));
