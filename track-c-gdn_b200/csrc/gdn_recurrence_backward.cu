@@ -18,20 +18,19 @@
 namespace gdn {
 namespace rec {
 
-template <typename E, bool kTma, bool kPacked>
+template <typename E, Fetch kFetch, bool kPacked>
 struct BwdShape {
   static constexpr int kThreads = 32 * (kSlots + 2);
-  static constexpr int kPlane = kRows * 64 * static_cast<int>(sizeof(E));      // d_out; x, a, b
-  static constexpr int kInPlane = kPacked ? kRows * 64 : kPlane;
-  static constexpr int kStage = kTma ? kPlane + 3 * kInPlane : kSlots * 512;
+  static constexpr int kPitch = row_pitch<static_cast<int>(sizeof(E))>(kFetch);  // of d_out; of x, a, b
+  static constexpr int kInPitch = kPacked ? row_pitch<1>(kFetch) : kPitch;
+  static constexpr int kPlane = kRows * kPitch, kInPlane = kRows * kInPitch;
+  static constexpr int kStage = kPlane + 3 * kInPlane;
   static constexpr int kStages = 2;
   static constexpr int kCtas = kStage > 49152 ? 1 : 2;
-  // where a warp leaves its sums: the stage's first plane, in its own rows
-  static constexpr int kSlotBytes = kTma ? kPlane / kSlots : 512;
 };
 
 struct Backward {
-  CUtensorMap tx, ta, tb, to;  // kTma
+  CUtensorMap tx, ta, tb, to;  // kTmaTile
   const void *x, *a, *b, *d_out;
   int64_t x_stride, a_stride, b_stride, do_stride;
   const uint8_t *packed;  // 8-bit x, a, b instead (kPacked)
@@ -66,11 +65,12 @@ struct BwdShared {
   int broken;
 };
 
-template <typename E, bool kTma, bool kPacked>
-__global__ void __launch_bounds__(BwdShape<E, kTma, kPacked>::kThreads, BwdShape<E, kTma, kPacked>::kCtas)
+template <typename E, Fetch kFetch, bool kPacked>
+__global__ void __launch_bounds__(BwdShape<E, kFetch, kPacked>::kThreads, BwdShape<E, kFetch, kPacked>::kCtas)
 recurrence_backward_kernel(const __grid_constant__ Backward p) {
-  using S = BwdShape<E, kTma, kPacked>;
-  constexpr bool kVec = kTma;
+  using S = BwdShape<E, kFetch, kPacked>;
+  constexpr bool kVec = kFetch == kTmaTile;
+  constexpr int kElement = sizeof(E), kInElement = kPacked ? 1 : kElement;
   constexpr int kStages = S::kStages;
   extern __shared__ __align__(1024) unsigned char smem[];
   BwdShared<S, kPacked> &sh = *reinterpret_cast<BwdShared<S, kPacked> *>(smem + kStages * S::kStage);
@@ -81,7 +81,7 @@ recurrence_backward_kernel(const __grid_constant__ Backward p) {
   if (tid == 0) {
     sh.broken = 0;
     for (int i = 0; i < kStages; ++i) {
-      mbar_init(smem_u32(&sh.full[i]), 1);
+      mbar_init(smem_u32(&sh.full[i]), fetch_arrivals(kFetch));
       mbar_init(smem_u32(&sh.mapped[i]), kSlots);
       mbar_init(smem_u32(&sh.taken[i]), 1);
       mbar_init(smem_u32(&sh.ready[i]), 1);
@@ -94,6 +94,12 @@ recurrence_backward_kernel(const __grid_constant__ Backward p) {
   const int64_t last = total > 0 ? (total - 1) / kRows : 0;
   const int group_len = p.hdr->group;  // 1 or kGroupLen
   uint64_t *const states = group_len == 1 ? p.maps : p.states;
+
+  auto input = [&](int w) -> const void * {
+    if (kPacked) return p.packed + w * p.s.T * p.D;
+    return w == 0 ? p.x : w == 1 ? p.a : p.b;
+  };
+  auto input_stride = [&](int w) { return kPacked ? p.D : w == 0 ? p.x_stride : w == 1 ? p.a_stride : p.b_stride; };
 
   if (warp == kSlots) {
     // ---- producer ----
@@ -113,7 +119,7 @@ recurrence_backward_kernel(const __grid_constant__ Backward p) {
         float4 v = *reinterpret_cast<const float4 *>(sums);
 #pragma unroll
         for (int j = 1; j < kSlots; ++j) {
-          const float4 w = *reinterpret_cast<const float4 *>(sums + j * S::kSlotBytes);
+          const float4 w = *reinterpret_cast<const float4 *>(sums + j * (S::kPlane / kSlots));
           v.x += w.x, v.y += w.y, v.z += w.z, v.w += w.w;
         }
         float2 *dst = p.partials + t.chunk * groups128 * 128 + t.d * 64;
@@ -165,15 +171,16 @@ recurrence_backward_kernel(const __grid_constant__ Backward p) {
           sh.tiles[s].d = -1;
           mbar_arrive(full);
         }
+        if (kFetch == kRowCopies) mbar_arrive(full);
         for (int i = max(k - kStages + 1, 0); i < k; ++i)
           if (!finish(i)) break;
         break;
       }
       if (lane == 0) {
-        mbar_expect_tx(full, 2 * 64 * 4 + (kTma ? S::kStage : 0));
+        mbar_expect_tx(full, 2 * 64 * 4 + (kVec ? S::kStage : 0));
         bulk_load(smem_u32(sh.params[s][0]), p.dt + c0, 64 * 4, full);
         bulk_load(smem_u32(sh.params[s][1]), p.c + c0, 64 * 4, full);
-        if constexpr (kTma) {
+        if constexpr (kFetch == kTmaTile) {
           const uint32_t dst = smem_u32(smem + s * S::kStage);
           const int x = static_cast<int>(c0), y = static_cast<int>(base);
           tma_load_2d(dst, &p.to, x, y, full);
@@ -181,6 +188,16 @@ recurrence_backward_kernel(const __grid_constant__ Backward p) {
           tma_load_2d(dst + S::kPlane + S::kInPlane, &p.ta, x, y, full);
           tma_load_2d(dst + S::kPlane + 2 * S::kInPlane, &p.tb, x, y, full);
         }
+      }
+      if constexpr (kFetch == kRowCopies) {
+        const int rows = static_cast<int>(min(total - base, int64_t{kRows}));
+        const uint32_t dst = smem_u32(smem + s * S::kStage);
+        copy_rows<kElement>(dst, p.d_out, p.do_stride, base, rows, c0, left, lane);
+#pragma unroll
+        for (int w = 0; w < 3; ++w)
+          copy_rows<kInElement>(dst + S::kPlane + w * S::kInPlane, input(w), input_stride(w), base, rows, c0, left,
+                                lane);
+        arrive_after_copies(full);
       }
       if constexpr (kPacked) {
 #pragma unroll
@@ -211,6 +228,7 @@ recurrence_backward_kernel(const __grid_constant__ Backward p) {
       ++k;
     }
     // after a wait that ran out: no copy may be in flight when the CTA ends
+    if (kFetch == kRowCopies) wait_copies();
     if (*static_cast<volatile int *>(&sh.broken))
       for (int i = max(k - kStages, 0); i < k; ++i)
         mbar_wait(smem_u32(&sh.full[i % kStages]), (i / kStages) & 1);
@@ -298,38 +316,21 @@ recurrence_backward_kernel(const __grid_constant__ Backward p) {
   // x, a, b and d_out of a row of a tile
   auto load = [&](int s, const Tile &tile, int i, uint64_t (&in)[3], uint64_t &o) {
     const int row = row0 + i;
-    if constexpr (kTma) {
-      const unsigned char *stage = smem + s * S::kStage;
-      Raw2<E> r;
-      r.v = reinterpret_cast<const decltype(Raw2<E>::v) *>(stage + row * 64 * sizeof(E))[lane];
-      o = r.pair();
+    const unsigned char *stage = smem + s * S::kStage;
+    const int64_t t = sh.tables[s].chunk * kRows + row, c0 = static_cast<int64_t>(tile.d) * 64;
+    const unsigned char *src = stage + row * S::kPitch;
+    if constexpr (kFetch == kRowCopies) src += row_offset<kElement>(p.d_out, p.do_stride, t, c0);
+    o = fetch2<E, kVec>(src, lane).pair();
 #pragma unroll
-      for (int w = 0; w < 3; ++w) {
-        const unsigned char *src = stage + S::kPlane + w * S::kInPlane;
-        if constexpr (kPacked) {
-          in[w] = dequantise2(reinterpret_cast<const uint16_t *>(src + row * 64)[lane], sh.scales[s][w][row]);
-        } else {
-          r.v = reinterpret_cast<const decltype(Raw2<E>::v) *>(src + row * 64 * sizeof(E))[lane];
-          in[w] = r.pair();
-        }
-      }
-    } else {
-      const int64_t t = sh.tables[s].chunk * kRows + row, c0 = static_cast<int64_t>(tile.d) * 64;
-      const int left = t < total ? static_cast<int>(min(p.D - c0, int64_t{64})) : 0;
-      o = load2<E, kVec>(static_cast<const E *>(p.d_out) + t * p.do_stride + c0, lane, left).pair();
+    for (int w = 0; w < 3; ++w) {
+      src = stage + S::kPlane + w * S::kInPlane + row * S::kInPitch;
+      if constexpr (kFetch == kRowCopies) src += row_offset<kInElement>(input(w), input_stride(w), t, c0);
       if constexpr (kPacked) {
-#pragma unroll
-        for (int w = 0; w < 3; ++w) {
-          const uint8_t *src = p.packed + (w * p.s.T + t) * p.D + c0;
-          uint32_t q = 0;
-          if (lane < left) q = src[lane];
-          if (lane + 32 < left) q |= static_cast<uint32_t>(src[lane + 32]) << 8;
-          in[w] = dequantise2(q, sh.scales[s][w][row]);
-        }
+        const uint32_t q = kVec ? reinterpret_cast<const uint16_t *>(src)[lane]
+                                : static_cast<uint32_t>(src[lane]) | static_cast<uint32_t>(src[lane + 32]) << 8;
+        in[w] = dequantise2(q, sh.scales[s][w][row]);
       } else {
-        in[0] = load2<E, kVec>(static_cast<const E *>(p.x) + t * p.x_stride + c0, lane, left).pair();
-        in[1] = load2<E, kVec>(static_cast<const E *>(p.a) + t * p.a_stride + c0, lane, left).pair();
-        in[2] = load2<E, kVec>(static_cast<const E *>(p.b) + t * p.b_stride + c0, lane, left).pair();
+        in[w] = fetch2<E, kVec>(src, lane).pair();
       }
     }
   };
@@ -482,9 +483,9 @@ recurrence_backward_kernel(const __grid_constant__ Backward p) {
         }
         constexpr float kLn2 = 0.6931471805599453f;
         __syncwarp();  // all lanes have read the warp's rows
-        *reinterpret_cast<float4 *>(smem + s * S::kStage + warp * S::kSlotBytes + lane * 16) =
+        *reinterpret_cast<float4 *>(smem + s * S::kStage + warp * (S::kPlane / kSlots) + lane * 16) =
             make_float4(f2_lo(sum_lg) * kLn2, f2_hi(sum_lg) * kLn2, f2_lo(sum_da), f2_hi(sum_da));
-        if (kTma) fence_async_smem();  // the next copy into this stage comes after
+        fence_async_smem();  // the next copy into this stage comes after
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(smem_u32(&sh.empty[s]));
@@ -522,14 +523,14 @@ recurrence_params_kernel(const float2 *partials, const Header *hdr, const Seqs s
   }
 }
 
-template <typename E, bool kTma, bool kPacked>
+template <typename E, Fetch kFetch, bool kPacked>
 cudaError_t launch_backward_t(Backward p, void *workspace, int sms, float *dA_log, float *ddt_bias,
                               cudaStream_t stream) {
-  using S = BwdShape<E, kTma, kPacked>;
+  using S = BwdShape<E, kFetch, kPacked>;
   const int64_t nt = (p.D + 63) / 64, chunks = chunks_of(p.s.T);
   constexpr int smem = S::kStages * S::kStage + static_cast<int>(sizeof(BwdShared<S, kPacked>));
   static_assert(smem * S::kCtas <= 227 * 1024 - 1024 * (S::kCtas - 1), "CTAs of an SM share 228 KiB");
-  if constexpr (kTma) {
+  if constexpr (kFetch == kTmaTile) {
     bool ok = make_row_map<E>(&p.to, p.d_out, p.D, p.s.T, p.do_stride, 64, kRows);
     if constexpr (kPacked) {
       const int64_t plane = p.s.T * p.D;
@@ -543,7 +544,7 @@ cudaError_t launch_backward_t(Backward p, void *workspace, int sms, float *dA_lo
     }
     if (!ok) return cudaErrorInvalidValue;
   }
-  auto kernel = recurrence_backward_kernel<E, kTma, kPacked>;
+  auto kernel = recurrence_backward_kernel<E, kFetch, kPacked>;
   static std::atomic<uint64_t> allowed;
   if (cudaError_t e = allow_shared(kernel, smem, allowed)) return e;
   const Places w = places(workspace, p.s.T, p.D);
@@ -566,10 +567,10 @@ template <typename E>
 cudaError_t launch_backward_e(const Backward &p, bool tma, void *workspace, int sms, float *dA_log, float *ddt_bias,
                               cudaStream_t stream) {
   if (p.packed != nullptr)
-    return tma ? launch_backward_t<E, true, true>(p, workspace, sms, dA_log, ddt_bias, stream)
-               : launch_backward_t<E, false, true>(p, workspace, sms, dA_log, ddt_bias, stream);
-  return tma ? launch_backward_t<E, true, false>(p, workspace, sms, dA_log, ddt_bias, stream)
-             : launch_backward_t<E, false, false>(p, workspace, sms, dA_log, ddt_bias, stream);
+    return tma ? launch_backward_t<E, kTmaTile, true>(p, workspace, sms, dA_log, ddt_bias, stream)
+               : launch_backward_t<E, kRowCopies, true>(p, workspace, sms, dA_log, ddt_bias, stream);
+  return tma ? launch_backward_t<E, kTmaTile, false>(p, workspace, sms, dA_log, ddt_bias, stream)
+             : launch_backward_t<E, kRowCopies, false>(p, workspace, sms, dA_log, ddt_bias, stream);
 }
 
 }  // namespace rec

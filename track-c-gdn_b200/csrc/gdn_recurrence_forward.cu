@@ -10,25 +10,25 @@ namespace rec {
 // consecutive rows.  A stage of shared memory holds one half (64 channels) as
 // planes of x, a and b, and afterwards, in place, what the first pass left: 16
 // bytes for each lane and row.
-template <typename E, bool kTma, bool kPack>
+template <typename E, Fetch kFetch, bool kPack>
 struct FwdShape {
   static constexpr int kHalves = kPack ? 2 : 1;
   static constexpr int kCh = 64 * kHalves;
   static constexpr int kWorkers = kSlots * kHalves;       // consumer warps
   static constexpr int kThreads = 32 * (kWorkers + 1 + 2 * kHalves);
-  static constexpr int kPlane = kRows * 64 * static_cast<int>(sizeof(E));
-  static constexpr int kHalfStage = kTma ? (sizeof(E) == 4 ? 3 : 4) * kPlane : kRows * 512;
+  static constexpr int kPitch = row_pitch<static_cast<int>(sizeof(E))>(kFetch);
+  static constexpr int kPlane = kFetch == kDirect ? kRows * 512 : kRows * kPitch;
+  // where a lane's 16 bytes of row i (of its 8) lie: kPerPlane rows in the
+  // slot's part of each plane; only rows that this warp alone reads are overwritten
+  static constexpr int kPerPlane = kFetch == kDirect ? kTokW : sizeof(E) == 4 ? 4 : 2;
+  static constexpr int kHalfStage = (kFetch == kDirect ? 1 : sizeof(E) == 4 ? 3 : 4) * kPlane;
   static constexpr int kStage = kHalves * kHalfStage;
   static constexpr int kStages = kHalfStage > 32768 ? 2 : 3;
-  static constexpr int kCtas = kPack ? 1 : 2;             // of an SM
-  // where a lane's 16 bytes of row i (of its 8) lie, from its slot's rows in
-  // the first plane: only rows that this warp alone reads are overwritten
-  static constexpr int kPerPlane = kTma ? (sizeof(E) == 4 ? 4 : 2) : kTokW;
-  static constexpr int kPlaneBytes = kTma ? kPlane : kRows * 512;
+  static constexpr int kCtas = kPack || kStages * kStage > 98304 ? 1 : 2;             // of an SM
 };
 
 struct Forward {
-  CUtensorMap tx, ta, tb;  // kTma
+  CUtensorMap tx, ta, tb;  // kTmaTile
   const void *x, *a, *b;
   int64_t x_stride, a_stride, b_stride;  // elements from one token to the next
   const float *A_log, *dt_bias;
@@ -75,11 +75,12 @@ struct FwdShared {
 //              that the look-back's latency costs the consumers nothing.
 // Without kChain (short inputs, one launch) a CTA walks all chunks of its
 // channels and the chain warp keeps the state.
-template <typename E, bool kTma, bool kPack, bool kChain>
-__global__ void __launch_bounds__(FwdShape<E, kTma, kPack>::kThreads, FwdShape<E, kTma, kPack>::kCtas)
+template <typename E, Fetch kFetch, bool kPack, bool kChain>
+__global__ void __launch_bounds__(FwdShape<E, kFetch, kPack>::kThreads, FwdShape<E, kFetch, kPack>::kCtas)
 recurrence_forward_kernel(const __grid_constant__ Forward p) {
-  using S = FwdShape<E, kTma, kPack>;
-  constexpr bool kVec = kTma;
+  using S = FwdShape<E, kFetch, kPack>;
+  constexpr bool kVec = kFetch == kTmaTile;
+  constexpr int kElement = sizeof(E);
   constexpr int kCh = S::kCh, kStages = S::kStages;
   extern __shared__ __align__(1024) unsigned char smem[];
   FwdShared<S, kPack> &sh = *reinterpret_cast<FwdShared<S, kPack> *>(smem + kStages * S::kStage);
@@ -98,7 +99,7 @@ recurrence_forward_kernel(const __grid_constant__ Forward p) {
   if (tid == 0) {
     sh.broken = 0;
     for (int i = 0; i < kStages; ++i) {
-      mbar_init(smem_u32(&sh.full[i]), 1);
+      mbar_init(smem_u32(&sh.full[i]), fetch_arrivals(kFetch));
       for (int w = 0; w < S::kHalves; ++w) {
         mbar_init(smem_u32(&sh.mapped[i][w]), kSlots);
         mbar_init(smem_u32(&sh.taken[i][w]), 1);
@@ -173,6 +174,7 @@ recurrence_forward_kernel(const __grid_constant__ Forward p) {
           sh.tiles[s].d = -1;
           mbar_arrive(full);
         }
+        if (kFetch == kRowCopies) mbar_arrive(full);
         ++k;
         if (++ends == 2) break;  // one for each chain warp
         continue;
@@ -182,7 +184,7 @@ recurrence_forward_kernel(const __grid_constant__ Forward p) {
         bulk_load(smem_u32(sh.params[s][0]), p.dt + c0, kCh * 4, full);
         bulk_load(smem_u32(sh.params[s][1]), p.c + c0, kCh * 4, full);
       }
-      if (kTma && lane == 0) {
+      if (kFetch == kTmaTile && lane == 0) {
         mbar_expect_tx(full, S::kHalves * 3 * S::kPlane);
 #pragma unroll
         for (int w = 0; w < S::kHalves; ++w) {
@@ -192,6 +194,21 @@ recurrence_forward_kernel(const __grid_constant__ Forward p) {
           tma_load_2d(dst + S::kPlane, &p.ta, x, y, full);
           tma_load_2d(dst + 2 * S::kPlane, &p.tb, x, y, full);
         }
+      }
+      if constexpr (kFetch == kRowCopies) {
+        const void *const src[3] = {p.x, p.a, p.b};
+        const int64_t stride[3] = {p.x_stride, p.a_stride, p.b_stride};
+        const int rows = static_cast<int>(min(total - base, int64_t{kRows}));
+#pragma unroll
+        for (int w = 0; w < S::kHalves; ++w) {
+          const int left = static_cast<int>(min(p.D - c0 - 64 * w, int64_t{64}));
+          if (left <= 0) break;
+#pragma unroll
+          for (int j = 0; j < 3; ++j)
+            copy_rows<kElement>(smem_u32(smem + s * S::kStage + w * S::kHalfStage + j * S::kPlane), src[j], stride[j],
+                                base, rows, c0 + 64 * w, left, lane);
+        }
+        arrive_after_copies(full);
       }
       const bool inside = fill_table<kRows>(p.s, t, base, chunk == last, lane, kChain ? p.first : nullptr, [&](int64_t n) {
         if (p.final == nullptr || only_map) return;  // an empty sequence's final state is its initial state
@@ -217,7 +234,8 @@ recurrence_forward_kernel(const __grid_constant__ Forward p) {
       ++k;
     }
     // after a wait that ran out: no copy may be in flight when the CTA ends
-    if ((kTma || kChain) && *static_cast<volatile int *>(&sh.broken))
+    if (kFetch == kRowCopies) wait_copies();
+    if ((kFetch != kDirect || kChain) && *static_cast<volatile int *>(&sh.broken))
       for (int i = max(k - kStages, 0); i < k - ends; ++i)
         mbar_wait(smem_u32(&sh.full[i % kStages]), (i / kStages) & 1);
     return;
@@ -304,7 +322,7 @@ recurrence_forward_kernel(const __grid_constant__ Forward p) {
   // ---- consumers ----
   const int slot = warp / S::kHalves, half = warp % S::kHalves;
   const int row0 = slot * kTokW;
-  unsigned char *const stage0 = smem + half * S::kHalfStage + row0 * (S::kPlaneBytes / kRows);
+  unsigned char *const stage0 = smem + half * S::kHalfStage + slot * (S::kPlane / kSlots);
   Params2 par{};
   int s = 0, s1 = 0, turn = 0;         // stages of this tile and the one before; whose turn to publish
   uint32_t parity = 0, parity1 = 0;    // ... and the phases of their barriers
@@ -329,27 +347,33 @@ recurrence_forward_kernel(const __grid_constant__ Forward p) {
         starts = mask_bits(tab.starts, row0, kTokW);
       }
       Raw2<E> raw[3][kTokW];
-      auto fetch = [&](int w) {  // the lane's 8 rows of x, a or b
-        if constexpr (kTma) {
-#pragma unroll
-          for (int i = 0; i < kTokW; ++i)
-            raw[w][i].v =
-                reinterpret_cast<const decltype(Raw2<E>::v) *>(stage + w * S::kPlane + i * 64 * sizeof(E))[lane];
+      // row i of x, a or b
+      auto fetch_row = [&](int w, int i) {
+        const void *base = w == 0 ? p.x : w == 1 ? p.a : p.b;
+        const int64_t stride = w == 0 ? p.x_stride : w == 1 ? p.a_stride : p.b_stride;
+        if constexpr (kFetch == kDirect) {
+          Raw2<E> r;
+          r.v = {};
+          if (i < valid)
+            r = load2<E, kVec>(static_cast<const E *>(base) + (tab.chunk * kRows + row0 + i) * stride + c0, lane,
+                               static_cast<int>(min(p.D - c0, int64_t{64})));
+          return r;
+        } else {
+          const unsigned char *src = stage + w * S::kPlane + i * S::kPitch;
+          if constexpr (kFetch == kRowCopies)
+            src += row_offset<kElement>(base, stride, tab.chunk * kRows + row0 + i, c0);
+          Raw2<E> r = fetch2<E, kVec>(src, lane);
+          if constexpr (kPack && kFetch == kRowCopies) {  // what lies behind the row's end is no part of its group
+            const int64_t left = p.D - c0;
+            if (left < 64) r.v = (lane < left ? r.v & 0xffffu : 0u) | (lane + 32 < left ? r.v & 0xffff0000u : 0u);
+          }
+          return r;
         }
       };
-      if constexpr (!kTma) {
-        const int64_t t0 = tab.chunk * kRows + row0;
-        const int left = static_cast<int>(min(p.D - c0, int64_t{64}));
+      auto fetch = [&](int w) {
 #pragma unroll
-        for (int i = 0; i < kTokW; ++i) {
-          raw[0][i].v = raw[1][i].v = raw[2][i].v = {};
-          if (i < valid) {
-            raw[0][i] = load2<E, kVec>(static_cast<const E *>(p.x) + (t0 + i) * p.x_stride + c0, lane, left);
-            raw[1][i] = load2<E, kVec>(static_cast<const E *>(p.a) + (t0 + i) * p.a_stride + c0, lane, left);
-            raw[2][i] = load2<E, kVec>(static_cast<const E *>(p.b) + (t0 + i) * p.b_stride + c0, lane, left);
-          }
-        }
-      }
+        for (int i = 0; i < kTokW; ++i) raw[w][i] = fetch_row(w, i);
+      };
       if constexpr (kPack) {
         // The groups' largest magnitudes: each half by one warp, joined through
         // shared memory.  Lane 8 w + i holds what belongs to row i of x, a or b.
@@ -409,14 +433,7 @@ recurrence_forward_kernel(const __grid_constant__ Forward p) {
             uint8_t *dst = p.packed + (w * p.s.T + t0) * p.D + c0;
 #pragma unroll 1
             for (int i = 0; i < valid; ++i, dst += p.D) {
-              Raw2<E> r;
-              if constexpr (kTma) {
-                r.v = reinterpret_cast<const decltype(r.v) *>(stage + w * S::kPlane + i * 64 * sizeof(E))[lane];
-              } else {
-                const void *src = w == 0 ? p.x : w == 1 ? p.a : p.b;
-                const int64_t stride = w == 0 ? p.x_stride : w == 1 ? p.a_stride : p.b_stride;
-                r = load2<E, kVec>(static_cast<const E *>(src) + (t0 + i) * stride + c0, lane, left);
-              }
+              const Raw2<E> r = fetch_row(w, i);
               const uint32_t q = quantise2(r.pair(), __shfl_sync(0xffffffffu, ex, kTokW * w + i), exp_cap<E>());
               if constexpr (kVec) {
                 if (2 * lane < left) reinterpret_cast<uint16_t *>(dst)[lane] = static_cast<uint16_t>(q);
@@ -433,7 +450,7 @@ recurrence_forward_kernel(const __grid_constant__ Forward p) {
       for (int w = 0; w < 3; ++w) fetch(w);
       __syncwarp();  // the warp's rows are overwritten from here on
       auto keep = [&](int i, uint64_t y, uint64_t P) {
-        *reinterpret_cast<ulonglong2 *>(stage + i / S::kPerPlane * S::kPlaneBytes + i % S::kPerPlane * 512 +
+        *reinterpret_cast<ulonglong2 *>(stage + i / S::kPerPlane * S::kPlane + i % S::kPerPlane * 512 +
                                         lane * 16) = make_ulonglong2(y, P);
       };
       uint64_t P = f2_dup(1.f), y = 0;
@@ -498,7 +515,7 @@ recurrence_forward_kernel(const __grid_constant__ Forward p) {
       const unsigned char *const src = stage0 + s1 * S::kStage + lane * 16;
       const uint64_t h = *reinterpret_cast<const uint64_t *>(&sh.own[s1][half][slot][lane]);
       auto kept = [&](int i) {
-        return *reinterpret_cast<const ulonglong2 *>(src + i / S::kPerPlane * S::kPlaneBytes + i % S::kPerPlane * 512);
+        return *reinterpret_cast<const ulonglong2 *>(src + i / S::kPerPlane * S::kPlane + i % S::kPerPlane * 512);
       };
       const Tile before = sh.tiles[s1];
       E *out = static_cast<E *>(p.out) + before.at + row0 * p.D + 64 * half;
@@ -525,7 +542,7 @@ recurrence_forward_kernel(const __grid_constant__ Forward p) {
             store2_f32<kVec>(p.final + p.s.row(tab.end[row0 + i]) * p.D + c0, lane, left, r);
         }
       }
-      if (kTma) fence_async_smem();  // this stage was written here; the next copy into it comes after
+      if (kFetch != kDirect) fence_async_smem();  // this stage was written here; the next copy into it comes after
       __syncwarp();
       if (lane == 0) mbar_arrive(smem_u32(&sh.empty[s1]));
     }
@@ -541,21 +558,21 @@ recurrence_forward_kernel(const __grid_constant__ Forward p) {
 constexpr int64_t kSerialChunks = 4;
 constexpr int64_t kSerialSeqs = 1024;  // each CTA checks all of cu_seqlens then
 
-template <typename E, bool kTma, bool kPack>
+template <typename E, Fetch kFetch, bool kPack>
 cudaError_t launch_forward_t(Forward p, void *workspace, int sms, cudaStream_t stream) {
-  using S = FwdShape<E, kTma, kPack>;
+  using S = FwdShape<E, kFetch, kPack>;
   const int64_t nt = (p.D + S::kCh - 1) / S::kCh, chunks = (max(p.s.T, int64_t{1}) - 1) / kRows + 1;
   constexpr int smem = S::kStages * S::kStage + static_cast<int>(sizeof(FwdShared<S, kPack>));
   static_assert(smem * S::kCtas <= 227 * 1024 - 1024 * (S::kCtas - 1), "CTAs of an SM share 228 KiB");
-  if constexpr (kTma) {
+  if constexpr (kFetch == kTmaTile) {
     if (!make_row_map<E>(&p.tx, p.x, p.D, p.s.T, p.x_stride, 64, kRows) ||
         !make_row_map<E>(&p.ta, p.a, p.D, p.s.T, p.a_stride, 64, kRows) ||
         !make_row_map<E>(&p.tb, p.b, p.D, p.s.T, p.b_stride, 64, kRows))
       return cudaErrorInvalidValue;
   }
   const bool serial = chunks <= kSerialChunks && (p.s.cu == nullptr || p.s.N <= kSerialSeqs);
-  auto kernel = serial ? recurrence_forward_kernel<E, kTma, kPack, false>
-                       : recurrence_forward_kernel<E, kTma, kPack, true>;
+  auto kernel = serial ? recurrence_forward_kernel<E, kFetch, kPack, false>
+                       : recurrence_forward_kernel<E, kFetch, kPack, true>;
   static std::atomic<uint64_t> allowed[2];
   if (cudaError_t e = allow_shared(kernel, smem, allowed[serial])) return e;
   int64_t blocks = nt;
@@ -578,11 +595,12 @@ cudaError_t launch_forward_t(Forward p, void *workspace, int sms, cudaStream_t s
 
 template <typename E>
 cudaError_t launch_forward_e(const Forward &p, bool tma, void *workspace, int sms, cudaStream_t stream) {
+  constexpr Fetch kOther = sizeof(E) == 4 ? kDirect : kRowCopies;
   if (p.packed != nullptr)
-    return tma ? launch_forward_t<E, true, true>(p, workspace, sms, stream)
-               : launch_forward_t<E, false, true>(p, workspace, sms, stream);
-  return tma ? launch_forward_t<E, true, false>(p, workspace, sms, stream)
-             : launch_forward_t<E, false, false>(p, workspace, sms, stream);
+    return tma ? launch_forward_t<E, kTmaTile, true>(p, workspace, sms, stream)
+               : launch_forward_t<E, kOther, true>(p, workspace, sms, stream);
+  return tma ? launch_forward_t<E, kTmaTile, false>(p, workspace, sms, stream)
+             : launch_forward_t<E, kRowCopies, false>(p, workspace, sms, stream);
 }
 
 }  // namespace rec

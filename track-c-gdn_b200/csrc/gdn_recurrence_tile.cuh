@@ -251,6 +251,53 @@ inline cudaError_t launch_init(Header *hdr, uint64_t *words, int64_t n, const Se
   return cudaGetLastError();
 }
 
+// ---- how inputs reach shared memory ------------------------------------------------
+// kTmaTile: one tensor copy a plane, rows of 64 channels side by side.  It wants
+// 16-byte rows.  kRowCopies: asynchronous copies of the 16-byte blocks that hold
+// a row's 64 channels (blocks never leave the pages of the data that they hold);
+// the row then starts up to 15 bytes into its place.  A bulk copy a row instead
+// took 49 cycles a row and was slower than loads without any stage (494 against
+// 328 us, 47000 x 1021 fp16).  kDirect: none; the consumers load from global
+// memory (4-byte types that are packed as well, whose rows with gaps do not fit).
+enum Fetch { kDirect, kTmaTile, kRowCopies };
+// arrivals that complete a stage: the producer's, and its lanes' copies
+constexpr int fetch_arrivals(Fetch f) { return f == kRowCopies ? 33 : 1; }
+
+// bytes from one row of a plane to the next
+template <int kElement>
+__host__ __device__ constexpr int row_pitch(Fetch f) {
+  return 64 * kElement + (f == kRowCopies ? 16 : 0);
+}
+
+// Issues the copies of rows [t0, t0 + rows) x `left` channels of a plane by all
+// lanes of a warp.
+template <int kElement>
+__device__ __forceinline__ void copy_rows(uint32_t dst, const void *base, int64_t stride, int64_t t0, int rows,
+                                          int64_t c0, int left, int lane) {
+  constexpr int kPieces = row_pitch<kElement>(kRowCopies) / 16;
+  const uintptr_t first = reinterpret_cast<uintptr_t>(base) + (t0 * stride + c0) * kElement;
+#pragma unroll 4
+  for (int q = lane; q < rows * kPieces; q += 32) {
+    const int r = q / kPieces, c = q - r * kPieces;
+    const uintptr_t at = first + r * (stride * kElement);
+    if (16 * c < static_cast<int>(at & 15) + left * kElement)
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst + 16 * q),
+                   "l"((at & ~uintptr_t{15}) + 16 * c)
+                   : "memory");
+  }
+}
+// This lane's arrival on a stage's barrier when its copies so far are there.
+__device__ __forceinline__ void arrive_after_copies(uint32_t mbar) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared.b64 [%0];" ::"r"(mbar) : "memory");
+}
+__device__ __forceinline__ void wait_copies() { asm volatile("cp.async.wait_all;" ::: "memory"); }
+// The byte at which row t starts in its place.
+template <int kElement>
+__device__ __forceinline__ uint32_t row_offset(const void *base, int64_t stride, int64_t t, int64_t c0) {
+  return (static_cast<uint32_t>(reinterpret_cast<uintptr_t>(base)) +
+          static_cast<uint32_t>(t * stride + c0) * static_cast<uint32_t>(kElement)) & 15u;
+}
+
 // ---- two channels of a lane -----------------------------------------------------
 // With kVec neighbours (one access), else lane and lane + 32 of 64 channels.
 template <typename E>
@@ -348,6 +395,22 @@ __device__ __forceinline__ void store2_f32(float *p, int lane, int left, uint64_
     if (lane < left) p[lane] = f2_lo(a);
     if (lane + 32 < left) p[lane + 32] = f2_hi(a);
   }
+}
+
+// A lane's two channels of a row in shared memory: neighbours of an aligned row
+// (kVec), else lane and lane + 32 of a row at `src` (aligned to an element).
+template <typename E, bool kVec>
+__device__ __forceinline__ Raw2<E> fetch2(const unsigned char *src, int lane) {
+  Raw2<E> r;
+  if constexpr (kVec) {
+    r.v = reinterpret_cast<const decltype(r.v) *>(src)[lane];
+  } else if constexpr (std::is_same<E, float>::value) {
+    r.v = make_float2(reinterpret_cast<const float *>(src)[lane], reinterpret_cast<const float *>(src)[lane + 32]);
+  } else {
+    const uint16_t *p = reinterpret_cast<const uint16_t *>(src);
+    r.v = static_cast<uint32_t>(p[lane]) | static_cast<uint32_t>(p[lane + 32]) << 16;
+  }
+  return r;
 }
 
 struct Params2 {
