@@ -62,6 +62,7 @@ def test_backward_arguments(gdn):
     assert backward(lib, ws_bytes=need - 1) == 4 and backward(lib, ws=P(0x10000010)) == 4
     assert backward(lib, state=far(3), d_state=P(0x30000000 + 16)) == 7
     assert backward(lib, d_final=far(3), d_state=P(0x30000000 + 16)) == 7
+    assert backward(lib, d_final=far(3), d_state=far(3)) == 7
 
 
 def decode(lib, type=BF16, x=OK, state=None, slots=None, pool=0, B=4, T=1, D=64, out=OK, new=far(3), inter=None):

@@ -163,6 +163,23 @@ def test_pool_equals_dense_states(gdn, lens):
     assert torch.equal(pool[others], before[others])
 
 
+@pytest.mark.parametrize("lens", [[5000, 100, 37, 3000, 65, 1], [70] * 60, [1000, 7000], [33] * 7 + [3000]])
+def test_states_in_place_where_chunks_are_cut(gdn, lens):
+    """Sequences that start inside a chunk where the rows are cut into streams:
+    the later stream may finish such a sequence, and overwrite its state, before
+    the earlier one has come to the chunk where it starts."""
+    for D in (64, 512):
+        x, state, A_log, a, dt_bias, b = dev(inputs(lens, D, BF16, 13, slow=True))
+        cu = cumulative(lens).cuda()
+        out, final = gdn.recurrence.run(x, state, A_log, a, dt_bias, b, cu)
+        slots = torch.randperm(len(lens), generator=torch.Generator().manual_seed(3)).to(torch.int32).cuda()
+        for _ in range(4):
+            pool = torch.empty_like(state)
+            pool[slots.long()] = state
+            assert torch.equal(gdn.recurrence.run_pool(x, pool, slots, A_log, a, dt_bias, b, cu), out)
+            assert torch.equal(pool[slots.long()], final)
+
+
 @pytest.mark.parametrize("T,used", [(100, 37), (256, 0), (900, 512), (900, 70)])
 def test_rows_behind_the_last_sequence(gdn, T, used):
     """Padded rows, NaN in all inputs there, are left alone by the _into form

@@ -139,7 +139,7 @@ int gdn_recurrence_backward(int type, const void *x, int64_t x_stride, const voi
     return GDN_ERR_WORKSPACE;
   const size_t states = static_cast<size_t>(num_seqs) * channels * 4;
   if (d_state && ((state && overlap(state, states, d_state, states)) ||
-                  (d_final_state && d_final_state != d_state && overlap(d_final_state, states, d_state, states))))
+                  (d_final_state && overlap(d_final_state, states, d_state, states))))
     return GDN_ERR_ALIASING;
   int sms = 0;
   if (int st = check_device(&sms)) return st;

@@ -24,6 +24,10 @@ struct FwdShape {
   static constexpr int kHalfStage = (kFetch == kDirect ? 1 : sizeof(E) == 4 ? 3 : 4) * kPlane;
   static constexpr int kStage = kHalves * kHalfStage;
   static constexpr int kStages = kHalfStage > 32768 ? 2 : 3;
+  // With three stages the second pass is put off by a tile.  With two the next
+  // tile's copy would have to wait for it (47000 x 1021 fp16: 295 us, and NEWODD
+  // with both passes in one turn; 65536 x 1024 fp32: 266 and NEWFP32).
+  static constexpr bool kDefer = kStages > 2;
   static constexpr int kCtas = kPack || kStages * kStage > 98304 ? 1 : 2;             // of an SM
 };
 
@@ -43,6 +47,7 @@ struct Forward {
   Header *hdr;     // kChain
   uint64_t *maps, *states;  // kChain
   const float *dt, *c;      // kChain: prepared
+  const float *aside;       // ... or null: the states are not updated in place
   const int *first;
 };
 
@@ -68,8 +73,8 @@ struct FwdShared {
 //   consumers  first pass: gates; per row the state y from a zero start and the
 //              product P of the gates so far, left in shared memory; the map
 //              (P, y) of the slot, and the tile's, which is published.  Second
-//              pass, one tile later: out = y + P h, with h the state that
-//              enters the slot.
+//              pass, one tile later (kDefer): out = y + P h, with h the state
+//              that enters the slot.
 //   chain      (two per half, for tiles in turn) looks back and hands each slot
 //              its state.  It has the time of two first passes for that, so
 //              that the look-back's latency costs the consumers nothing.
@@ -225,6 +230,7 @@ recurrence_forward_kernel(const __grid_constant__ Forward p) {
         t.d = d;
         t.last = chunk == last;
         t.only_map = only_map;
+        t.cut = kChain && p.aside != nullptr && !only_map && chunk == st.to - 1 ? st.cut : -1;
         t.valid = min(total - base, int64_t{kRows});
         const bool plain = inside && !only_map && base + kRows <= total && c0 + kCh <= p.D && p.out != nullptr;
         sh.tiles[s] = Tile{base * p.D + c0, d, plain ? 1 : 0};
@@ -324,6 +330,44 @@ recurrence_forward_kernel(const __grid_constant__ Forward p) {
   const int row0 = slot * kTokW;
   unsigned char *const stage0 = smem + half * S::kHalfStage + slot * (S::kPlane / kSlots);
   Params2 par{};
+  // second pass over the tile of a stage; false if its wait ran out
+  auto second_pass = [&](int s1, uint32_t parity1) {
+    if (!__all_sync(0xffffffffu, wait_phase(smem_u32(&sh.ready[s1]), parity1, &sh.broken))) return false;
+    const unsigned char *const src = stage0 + s1 * S::kStage + lane * 16;
+    const uint64_t h = *reinterpret_cast<const uint64_t *>(&sh.own[s1][half][slot][lane]);
+    auto kept = [&](int i) {
+      return *reinterpret_cast<const ulonglong2 *>(src + i / S::kPerPlane * S::kPlane + i % S::kPerPlane * 512);
+    };
+    const Tile before = sh.tiles[s1];
+    E *out = static_cast<E *>(p.out) + before.at + row0 * p.D + 64 * half;
+    if (before.plain) {
+#pragma unroll
+      for (int i = 0; i < kTokW; ++i) {
+        const ulonglong2 v = kept(i);
+        store2<E, kVec>(out, lane, 64, f2_fma(v.y, h, v.x));
+        out += p.D;
+      }
+    } else if (!sh.tables[s1].only_map) {
+      const Table<kRows> &tab = sh.tables[s1];
+      const int64_t c0 = static_cast<int64_t>(before.d) * kCh + 64 * half;
+      const int left = static_cast<int>(min(p.D - c0, int64_t{64}));
+      const int valid = static_cast<int>(max(int64_t{0}, min(int64_t{kTokW}, tab.valid - row0)));
+      const unsigned starts = mask_bits(tab.starts, row0, kTokW), ends = mask_bits(tab.ends, row0, kTokW);
+      const int first = starts ? __ffs(starts) - 1 : kTokW;
+#pragma unroll
+      for (int i = 0; i < kTokW; ++i) {
+        const ulonglong2 v = kept(i);
+        const uint64_t r = i < first ? f2_fma(v.y, h, v.x) : v.x;
+        if (p.out != nullptr && i < valid) store2<E, kVec>(out + i * p.D, lane, left, r);
+        if (((ends >> i) & 1) && p.final != nullptr)
+          store2_f32<kVec>(p.final + p.s.row(tab.end[row0 + i]) * p.D + c0, lane, left, r);
+      }
+    }
+    if (kFetch != kDirect) fence_async_smem();  // this stage was written here; the next copy into it comes after
+    __syncwarp();
+    if (lane == 0) mbar_arrive(smem_u32(&sh.empty[s1]));
+    return true;
+  };
   int s = 0, s1 = 0, turn = 0;         // stages of this tile and the one before; whose turn to publish
   uint32_t parity = 0, parity1 = 0;    // ... and the phases of their barriers
   for (int k = 0;; ++k) {
@@ -474,10 +518,13 @@ recurrence_forward_kernel(const __grid_constant__ Forward p) {
           gate_pair(r[0].pair(), r[1].pair(), r[2].pair(), par.dt, par.c, g, u);
           if (i >= valid) g = f2_dup(1.f), u = 0;
           if ((starts >> i) & 1) {  // y is the state itself from here on
-            y = p.state != nullptr
-                    ? load2_f32<kVec>(p.state + p.s.row(tab.start[row0 + i]) * p.D + c0, lane,
-                                      static_cast<int>(min(p.D - c0, int64_t{64})))
-                    : 0;
+            const int left = static_cast<int>(min(p.D - c0, int64_t{64}));
+            const int row = row0 + i;
+            // of a cut chunk the last sequence's was set aside if it goes on
+            const bool goes_on = tab.cut >= 0 && !last_bits(tab.starts, row + 1) && !last_bits(tab.ends, row);
+            y = p.state == nullptr ? 0
+                : goes_on          ? load2_f32<kVec>(p.aside + tab.cut * ((p.D + 127) / 128 * 128) + c0, lane, left)
+                                   : load2_f32<kVec>(p.state + p.s.row(tab.start[row]) * p.D + c0, lane, left);
             P = f2_dup(-1.f);
           }
           P = f2_mul(P, g);
@@ -509,42 +556,10 @@ recurrence_forward_kernel(const __grid_constant__ Forward p) {
       }
       turn = turn + 1 == kSlots ? 0 : turn + 1;
     }
-    if (k > 0) {
-      // second pass, over the tile before
-      if (!__all_sync(0xffffffffu, wait_phase(smem_u32(&sh.ready[s1]), parity1, &sh.broken))) return;
-      const unsigned char *const src = stage0 + s1 * S::kStage + lane * 16;
-      const uint64_t h = *reinterpret_cast<const uint64_t *>(&sh.own[s1][half][slot][lane]);
-      auto kept = [&](int i) {
-        return *reinterpret_cast<const ulonglong2 *>(src + i / S::kPerPlane * S::kPlane + i % S::kPerPlane * 512);
-      };
-      const Tile before = sh.tiles[s1];
-      E *out = static_cast<E *>(p.out) + before.at + row0 * p.D + 64 * half;
-      if (before.plain) {
-#pragma unroll
-        for (int i = 0; i < kTokW; ++i) {
-          const ulonglong2 v = kept(i);
-          store2<E, kVec>(out, lane, 64, f2_fma(v.y, h, v.x));
-          out += p.D;
-        }
-      } else if (!sh.tables[s1].only_map) {
-        const Table<kRows> &tab = sh.tables[s1];
-        const int64_t c0 = static_cast<int64_t>(before.d) * kCh + 64 * half;
-        const int left = static_cast<int>(min(p.D - c0, int64_t{64}));
-        const int valid = static_cast<int>(max(int64_t{0}, min(int64_t{kTokW}, tab.valid - row0)));
-        const unsigned starts = mask_bits(tab.starts, row0, kTokW), ends = mask_bits(tab.ends, row0, kTokW);
-        const int first = starts ? __ffs(starts) - 1 : kTokW;
-#pragma unroll
-        for (int i = 0; i < kTokW; ++i) {
-          const ulonglong2 v = kept(i);
-          const uint64_t r = i < first ? f2_fma(v.y, h, v.x) : v.x;
-          if (p.out != nullptr && i < valid) store2<E, kVec>(out + i * p.D, lane, left, r);
-          if (((ends >> i) & 1) && p.final != nullptr)
-            store2_f32<kVec>(p.final + p.s.row(tab.end[row0 + i]) * p.D + c0, lane, left, r);
-        }
-      }
-      if (kFetch != kDirect) fence_async_smem();  // this stage was written here; the next copy into it comes after
-      __syncwarp();
-      if (lane == 0) mbar_arrive(smem_u32(&sh.empty[s1]));
+    if constexpr (S::kDefer) {
+      if (k > 0 && !second_pass(s1, parity1)) return;
+    } else {
+      if (tile.d >= 0 && !second_pass(s, parity)) return;
     }
     if (tile.d < 0) return;
     s1 = s;
@@ -582,10 +597,12 @@ cudaError_t launch_forward_t(Forward p, void *workspace, int sms, cudaStream_t s
     p.maps = w.words;
     p.states = p.maps + chunks * nt * S::kCh;
     p.dt = w.dt, p.c = w.c;
+    p.aside = p.state != nullptr && p.state == p.final ? w.aside : nullptr;
     p.first = w.first;
     const int64_t words = (chunks + (chunks + kGroupLen - 1) / kGroupLen) * nt * S::kCh;
     const Prepared q{p.A_log,     p.dt_bias, w.dt,  w.c, p.D, w.first, chunks, kRows,
-                     streams_for(nt, int64_t{sms} * S::kCtas), false};
+                     streams_for(nt, int64_t{sms} * S::kCtas), false,
+                     p.aside != nullptr ? p.state : nullptr, w.aside};
     if (cudaError_t e = launch_init(p.hdr, p.maps, words, p.s, q, stream)) return e;
     blocks = min(chunks * nt, int64_t{sms} * S::kCtas);
   }

@@ -33,6 +33,7 @@ struct Table {
   int d;
   int last;       // the last chunk
   int only_map;   // nothing but the tile's map is wanted
+  int cut;        // the cut that goes through the chunk, or -1
   uint32_t starts[kRows / 32], ends[kRows / 32];
   int start[kRows], end[kRows];  // the sequence, or -1
 };
@@ -66,6 +67,8 @@ struct Stream {
   int64_t from, to;  // chunks [from, to)
   uint32_t ticket;
   int only_map;      // 1: starts with the map of chunk from - 1 (backwards: to)
+  int cut;           // forwards: the cut that goes through chunk to - 1, or -1
+  int pad;
 };
 struct Header {
   uint32_t bad;      // cu_seqlens or slots are not valid: write nothing
@@ -74,8 +77,8 @@ struct Header {
   uint32_t pad;
   Stream stream[kStreams];
 };
-static_assert(sizeof(Header) <= 1024, "what follows starts 1024 bytes into the workspace");
-constexpr size_t kHeaderBytes = 1024;
+static_assert(sizeof(Header) <= 2048, "what follows starts 2048 bytes into the workspace");
+constexpr size_t kHeaderBytes = 2048;
 
 // Checks cu_seqlens and slots with all threads of a CTA; returns the device
 // status code of what is wrong, or 0.
@@ -118,7 +121,20 @@ struct Prepared {
   int64_t chunks, rows;
   int streams;      // as many as wanted, at most kStreams
   bool backwards;   // the chain runs from the last chunk to the first
+  // States that the call updates in place (else null): a sequence that starts
+  // in a cut chunk and goes on behind it is finished by the stream that begins
+  // there, perhaps before the stream before has come to the chunk and read where
+  // it starts from.  That state is set aside, one row for each cut.
+  const float *state;
+  float *aside;     // [kStreams][D up to 128s]
 };
+
+// Forwards: the first chunk that begins where the first sequence does that starts
+// from an even cut on, or after that.
+__device__ __forceinline__ int64_t first_of_stream(const Seqs &s, int64_t chunks, int64_t rows, int i, int streams) {
+  const int64_t n = first_by_halves(s, chunks * i / streams * rows);
+  return i == 0 ? 0 : n < s.N ? (s.at(n) + rows - 1) / rows : chunks;
+}
 
 // Empties the words, prepares, and checks the sequences, before the tiles run.
 __global__ void __launch_bounds__(1024) recurrence_init_kernel(Header *hdr, ulonglong2 *words, int64_t n,
@@ -127,6 +143,16 @@ __global__ void __launch_bounds__(1024) recurrence_init_kernel(Header *hdr, ulon
   for (int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; i < n;
        i += static_cast<int64_t>(gridDim.x) * blockDim.x)
     words[i] = e;
+  if (q.state != nullptr) {
+    for (int i = 1 + blockIdx.x; i < q.streams; i += gridDim.x) {
+      // the sequence that covers the first row behind the cut chunk
+      const int64_t n = first_by_halves(s, first_of_stream(s, q.chunks, q.rows, i, q.streams) * q.rows) - 1;
+      const int64_t row = n >= 0 ? s.row(n) : -1;
+      if (row < 0 || (s.slots != nullptr && row >= s.pool)) continue;
+      for (int64_t c = threadIdx.x; c < q.D; c += blockDim.x)
+        q.aside[i * ((q.D + 127) / 128 * 128) + c] = q.state[row * q.D + c];
+    }
+  }
   const int64_t me = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x;
   for (int64_t c = me; c < (q.D + 127) / 128 * 128; c += static_cast<int64_t>(gridDim.x) * blockDim.x) {
     q.dt[c] = c < q.D ? param_dt(q.dt_bias[c]) : 0.f;
@@ -158,13 +184,14 @@ __global__ void __launch_bounds__(1024) recurrence_init_kernel(Header *hdr, ulon
     if (i == 0) {
       int n = 1;
       int64_t prev = 0;
-      hdr->stream[0] = Stream{0, q.chunks, 0, 0};
+      hdr->stream[0] = Stream{0, q.chunks, 0, 0, -1, 0};
       for (int j = 1; j < q.streams; ++j)
         if (from[j] > prev && from[j] < q.chunks) {
           prev = from[j];
           hdr->stream[n - 1].to = from[j];
           if (q.backwards) hdr->stream[n - 1].only_map = only_map[j];
-          hdr->stream[n] = Stream{from[j], q.chunks, 0, q.backwards ? 0 : only_map[j]};
+          if (!q.backwards && only_map[j]) hdr->stream[n - 1].cut = j;
+          hdr->stream[n] = Stream{from[j], q.chunks, 0, q.backwards ? 0 : only_map[j], -1, 0};
           ++n;
         }
       hdr->streams = n;
@@ -249,6 +276,12 @@ inline cudaError_t launch_init(Header *hdr, uint64_t *words, int64_t n, const Se
   recurrence_init_kernel<<<static_cast<unsigned>(max(blocks, int64_t{1})), 1024, 0, stream>>>(
       hdr, reinterpret_cast<ulonglong2 *>(words), n / 2, s, q);
   return cudaGetLastError();
+}
+
+// whether any bit from `row` on is set (row up to 64)
+__device__ __forceinline__ bool last_bits(const uint32_t (&words)[2], int row) {
+  const uint64_t m = static_cast<uint64_t>(words[1]) << 32 | words[0];
+  return row < 64 && m >> row;
 }
 
 // ---- how inputs reach shared memory ------------------------------------------------
@@ -533,7 +566,7 @@ bool make_row_map(CUtensorMap *m, const void *base, int64_t channels, int64_t ro
 // The workspace: header, prepared parameters and first sequences, words (as
 // many as the widest tiles need).
 struct Places {
-  float *dt, *c;
+  float *dt, *c, *aside;
   int *first;
   uint64_t *words;
   size_t bytes;
@@ -542,10 +575,10 @@ inline int64_t tiles_of(int64_t D) { return (D + 127) / 128; }
 inline int64_t chunks_of(int64_t T) { return T > 0 ? (T + kRows - 1) / kRows : 1; }
 inline Places places(void *workspace, int64_t T, int64_t D) {
   const int64_t width = tiles_of(D) * 128, chunks = chunks_of(T);
-  const size_t first = kHeaderBytes + 8 * width, words = first + (4 * (chunks + 1) + 15) / 16 * 16;
+  const size_t first = kHeaderBytes + (8 + 4 * kStreams) * width, words = first + (4 * (chunks + 1) + 15) / 16 * 16;
   char *w = static_cast<char *>(workspace);
-  return Places{reinterpret_cast<float *>(w + kHeaderBytes), reinterpret_cast<float *>(w + kHeaderBytes + 4 * width),
-                reinterpret_cast<int *>(w + first), reinterpret_cast<uint64_t *>(w + words),
+  float *f = reinterpret_cast<float *>(w + kHeaderBytes);
+  return Places{f, f + width, f + 2 * width, reinterpret_cast<int *>(w + first), reinterpret_cast<uint64_t *>(w + words),
                 words + 8 * (chunks + (chunks + kGroupLen - 1) / kGroupLen) * width};
 }
 
