@@ -24,10 +24,11 @@ struct FwdShape {
   static constexpr int kHalfStage = (kFetch == kDirect ? 1 : sizeof(E) == 4 ? 3 : 4) * kPlane;
   static constexpr int kStage = kHalves * kHalfStage;
   static constexpr int kStages = kHalfStage > 32768 ? 2 : 3;
-  // With three stages the second pass is put off by a tile.  With two the next
-  // tile's copy would have to wait for it (47000 x 1021 fp16: 295 us, and NEWODD
-  // with both passes in one turn; 65536 x 1024 fp32: 266 and NEWFP32).
-  static constexpr bool kDefer = kStages > 2;
+  // The second pass is put off by a tile, but not with two stages of row copies:
+  // the next tile's copies, which take long, would have to wait for it (47000 x
+  // 1021 fp16: 295 against 269 us; with tensor copies it still pays: 65536 x
+  // 1024 fp32 266 against 315 us).
+  static constexpr bool kDefer = kStages > 2 || kFetch == kTmaTile;
   static constexpr int kCtas = kPack || kStages * kStage > 98304 ? 1 : 2;             // of an SM
 };
 

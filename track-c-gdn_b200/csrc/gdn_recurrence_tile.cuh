@@ -307,17 +307,19 @@ __host__ __device__ constexpr int row_pitch(Fetch f) {
 template <int kElement>
 __device__ __forceinline__ void copy_rows(uint32_t dst, const void *base, int64_t stride, int64_t t0, int rows,
                                           int64_t c0, int left, int lane) {
-  constexpr int kPieces = row_pitch<kElement>(kRowCopies) / 16;
-  const uintptr_t first = reinterpret_cast<uintptr_t>(base) + (t0 * stride + c0) * kElement;
+  // 32 / kPieces rows at a time, a lane's piece of the row always the same
+  constexpr int kPieces = row_pitch<kElement>(kRowCopies) / 16, kStep = 32 / kPieces;
+  const int r0 = lane / kPieces, c = lane - r0 * kPieces;
+  if (r0 >= kStep) return;
+  uintptr_t at = reinterpret_cast<uintptr_t>(base) + ((t0 + r0) * stride + c0) * kElement;
+  const int64_t step = kStep * stride * kElement;
+  dst += 16 * lane;
+  const int end = left * kElement - 16 * c;
 #pragma unroll 4
-  for (int q = lane; q < rows * kPieces; q += 32) {
-    const int r = q / kPieces, c = q - r * kPieces;
-    const uintptr_t at = first + r * (stride * kElement);
-    if (16 * c < static_cast<int>(at & 15) + left * kElement)
-      asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst + 16 * q),
-                   "l"((at & ~uintptr_t{15}) + 16 * c)
+  for (int r = r0; r < rows; r += kStep, at += step, dst += 16 * kStep * kPieces)
+    if (static_cast<int>(at & 15) + end > 0)
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"((at & ~uintptr_t{15}) + 16 * c)
                    : "memory");
-  }
 }
 // This lane's arrival on a stage's barrier when its copies so far are there.
 __device__ __forceinline__ void arrive_after_copies(uint32_t mbar) {
