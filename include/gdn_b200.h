@@ -285,9 +285,9 @@ int gdn_prefill_backward_qk4_v8_d128_k_last(
  * x, a, b   [T, D], a token's channels contiguous, `*_stride` elements from one
  *           token to the next (so they may be parts of one projection's output)
  * A_log, dt_bias [D] fp32
- * Pointers need the alignment of their elements; where D and the strides are
- * multiples of 4 and the pointers aligned to 4 elements the kernels use wide
- * accesses.  1 <= D <= 2^24, T <= 2^31.
+ * Pointers need the alignment of their elements; the kernels are fastest where
+ * rows and pointers of the inputs are multiples of 16 bytes.  1 <= D <= 2^24,
+ * T <= 2^31.
  */
 #define GDN_BF16 0
 #define GDN_FP16 1
@@ -296,16 +296,16 @@ int gdn_prefill_backward_qk4_v8_d128_k_last(
 /*
  * Prefill of N sequences packed into total_tokens rows.
  * cu_seqlens  [N+1] int64 on the device as in gdn_prefill_qk4_v8_d128_k_last,
- *             except that cu_seqlens[N] may be less than total_tokens: the
- *             rows behind the last sequence are not read, and left as they
- *             were in `out` or, with `zero_behind`, set to zero.
+ *             except that cu_seqlens[N] may be less than total_tokens: what
+ *             the rows behind the last sequence hold plays no part, and they
+ *             are left as they were in `out` or, with `zero_behind`, set to zero.
  *             Bad values set device status 1 and nothing is written.  NULL:
  *             N sequences of total_tokens / N tokens each.
  * state       [N,D] fp32 initial states or NULL (zeros); with `slots`
  *             ([N] int32 on the device, distinct) a pool [pool_slots,D] of
  *             which sequence n uses row slots[n] (outside the pool: device
  *             status 3, nothing is written)
- * out         [T,D]; final_state [N,D] fp32 (the pool with `slots`), may be
+ * out         [T,D], sharing no memory with x, a or b; final_state [N,D] fp32 (the pool with `slots`), may be
  *             `state`; an empty sequence's final state is its initial state
  * carries     NULL, or gdn_recurrence_carry_bytes(T, D) bytes (16-byte
  *             aligned) that receive the state before every 64th row, which
@@ -332,7 +332,8 @@ int gdn_recurrence_prefill(int type, const void *x, int64_t x_stride, const void
 /*
  * Gradients of (out, final_state) of the prefill, given d_out ([T,D] of
  * `type`, d_out_stride between rows) and d_final_state ([N,D] fp32 or NULL).
- * dx, da, db  [T,D] of `type`; rows behind the last sequence as in `out`
+ * dx, da, db  [T,D] of `type`, sharing no memory with the inputs; rows behind
+ *             the last sequence as in `out`
  * dA_log, ddt_bias [D] fp32;  d_state [N,D] fp32 or NULL (not computed)
  * carries     what the forward saved, or NULL: the call then runs the
  *             recurrence once more to find them

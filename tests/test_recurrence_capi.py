@@ -19,7 +19,7 @@ def far(n):
 
 
 def prefill(lib, type=BF16, x=OK, xs=64, a=OK, b=OK, A_log=OK, dt_bias=OK, state=None, slots=None, pool=0, cu=OK,
-            N=2, T=100, D=64, out=OK, final=far(9), carries=None, packed=None, ws=far(20), ws_bytes=BIG):
+            N=2, T=100, D=64, out=far(5), final=far(9), carries=None, packed=None, ws=far(20), ws_bytes=BIG):
     return lib.gdn_recurrence_prefill(type, x, xs, a, 64, b, 64, A_log, dt_bias, state, slots, pool, cu, N, T, D, 0,
                                       out, final, carries, packed, ws, ws_bytes, None)
 
@@ -40,10 +40,12 @@ def test_prefill_arguments(gdn):
     need = lib.gdn_recurrence_workspace_bytes(100, 64)
     assert need > 0 and prefill(lib, ws_bytes=need - 1) == 4
     assert prefill(lib, state=P(0x90000000 - 256)) == 7
+    for out in (OK, P(0x100000 + 99 * 128), P(0x100000 - 64)):
+        assert prefill(lib, out=out) == 7
 
 
 def backward(lib, type=BF16, x=OK, a=OK, b=OK, packed=None, state=None, cu=OK, N=2, T=100, D=64, d_out=OK,
-             d_final=None, carries=None, dx=OK, da=OK, db=OK, dA=OK, ddt=OK, d_state=None, ws=far(20), ws_bytes=BIG):
+             d_final=None, carries=None, dx=far(5), da=far(6), db=far(7), dA=OK, ddt=OK, d_state=None, ws=far(20), ws_bytes=BIG):
     return lib.gdn_recurrence_backward(type, x, 64, a, 64, b, 64, packed, OK, OK, state, cu, N, T, D, 0, d_out, 64,
                                        d_final, carries, dx, da, db, dA, ddt, d_state, ws, ws_bytes, None)
 
@@ -63,6 +65,7 @@ def test_backward_arguments(gdn):
     assert backward(lib, state=far(3), d_state=P(0x30000000 + 16)) == 7
     assert backward(lib, d_final=far(3), d_state=P(0x30000000 + 16)) == 7
     assert backward(lib, d_final=far(3), d_state=far(3)) == 7
+    assert backward(lib, dx=OK) == 7 and backward(lib, db=P(0x100000 + 99 * 128)) == 7
 
 
 def decode(lib, type=BF16, x=OK, state=None, slots=None, pool=0, B=4, T=1, D=64, out=OK, new=far(3), inter=None):

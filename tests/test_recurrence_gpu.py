@@ -123,6 +123,17 @@ def test_nothing_to_do(gdn):
     assert torch.equal(final, d[1])
 
 
+@pytest.mark.parametrize("lens", [[0] * 1100, [0] * 600 + [5] + [0] * 600, [0, 1, 0, 2] * 500])
+def test_many_sequences_most_of_them_empty(gdn, lens):
+    args = inputs(lens, 24, BF16, 77)
+    cu = cumulative(lens)
+    check_forward(gdn.recurrence.run(*dev(args), cu.cuda()), args, cu, "empty")
+    d_final = torch.randn(len(lens), 24, generator=torch.Generator().manual_seed(1))
+    d_out = torch.randn(sum(lens), 24, generator=torch.Generator().manual_seed(2)).to(BF16)
+    got = gdn.recurrence.backward(*dev(args), cu.cuda(), d_out.cuda(), d_final.cuda())
+    check_gradients(got, ref.backward(*args, cu.tolist(), d_out, d_final), BF16, "empty")
+
+
 @pytest.mark.parametrize("T", [100, 1000])
 def test_state_updated_in_place_and_continued(gdn, T):
     """A sequence cut in two, the second part continued from the state that the

@@ -4,19 +4,23 @@
 //   g_t = exp(-exp(A_log) softplus(a_t + dt_bias)),  beta_t = sigmoid(b_t)
 //   h_t = g_t h_{t-1} + beta_t x_t,   out_t = h_t           (per channel, fp32)
 //
-// Prefill and backward cut the packed tokens into chunks of 64, whatever the
-// sequences' lengths, and the channels into tiles of 128; a tile (chunk x 128
-// channels) is one CTA's work, so ragged batches load every SM alike.  A
-// chunk maps the state before it to the state after it by one affine map per
-// channel, h -> A h + H, with A the product of its gates; a chunk in which a
-// sequence starts maps to a constant.
+// Prefill (gdn_recurrence_forward.cu) and backward (gdn_recurrence_backward.cu)
+// cut the packed rows into chunks of 64, whatever the sequences' lengths, and the
+// channels into tiles of 64 (128 where 8-bit copies are written), so that ragged
+// batches load every SM alike.  A chunk maps the state before it to the state
+// after it by one affine map per channel, h -> A h + H, with A the product of its
+// gates; a chunk in which a sequence starts maps to a constant.  Backwards the
+// same holds for R (see there) from the last row of a chunk to its first.
 //
-// Look-back: the CTA of a chunk publishes its map, fetches the maps of the
-// chunks before it in its group of 32 and the state after the previous group,
-// and applies them in order; the last chunk of a group publishes the state
-// after it.  A serial chain thus has one link per 32 chunks, and the order of
-// all roundings is fixed: results do not depend on timing.  Tiles are taken
-// by ticket in chunk order, so a CTA only ever waits for CTAs that already run.
+// Look-back: a chunk's map is published, its CTA fetches the maps of the chunks
+// before it in its group of 8 and the state after the previous group, and applies
+// them in order; the last chunk of a group publishes the state after it.  A serial
+// chain thus has one link per 8 chunks.  Batches of several sequences are worked
+// on in streams that run side by side (Stream in gdn_recurrence_tile.cuh); a
+// chunk's predecessor is then done when its turn comes, and groups are of one.
+// The order of all roundings is fixed by the sizes and cu_seqlens: results do not
+// depend on timing.  Tiles are taken by ticket in the chain's order, so a CTA only
+// ever waits for tiles that running CTAs have in hand, and every wait is bounded.
 #include "gdn_recurrence_tile.cuh"
 
 namespace gdn {
@@ -79,7 +83,7 @@ __global__ void __launch_bounds__(kThreads) recurrence_decode_kernel(const __gri
 }
 
 // ---- sizes and launches ----------------------------------------------------------
-inline size_t saved_bytes(int64_t T, int64_t D) {  // carries
+inline size_t saved_bytes(int64_t T, int64_t D) {  // the states before every 64th row
   return static_cast<size_t>(chunks_of(T) * tiles_of(D) * kTileCh * 4);
 }
 

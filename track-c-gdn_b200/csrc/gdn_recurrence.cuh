@@ -15,17 +15,9 @@
 namespace gdn {
 namespace rec {
 
-// A tile is 64 packed tokens x 128 channels, worked on by 8 warps: a warp owns
-// 8 consecutive tokens of all 128 channels, a lane 4 of the channels.
-constexpr int kTileCh = 128;
-constexpr int kTok = 8;
-constexpr int kWarps = 8;
+constexpr int kWarps = 8;  // of a decode or checkpoint CTA
 constexpr int kThreads = kWarps * 32;
-constexpr int kChunkTok = kTok * kWarps;  // 64: also the distance of saved states
-// Chunks whose affine maps are joined through one group state (see
-// gdn_recurrence.cu, "look-back").
-constexpr int kGroup = 32;
-constexpr int kLook = kGroup / kWarps;  // maps that one warp fetches
+constexpr int kTileCh = 128;  // channels of a decode warp: 4 a lane
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr uint64_t kEmptyWord = ~0ull;  // a word that has not been handed over
@@ -63,11 +55,6 @@ struct Raw<float> {
 // Channels of a lane: with kVec 4 neighbours (one 8- or 16-byte access), else
 // lane, lane + 32, lane + 64, lane + 96 of the tile, so that single-element
 // accesses of a warp still fall next to one another.
-template <bool kVec>
-__device__ __forceinline__ int lane_channel(int lane, int j) {
-  return kVec ? 4 * lane + j : lane + 32 * j;
-}
-
 // left: channels of the tile that exist (D - first channel; may exceed 128).
 template <typename E, bool kVec>
 __device__ __forceinline__ Raw<E> load4(const E *p, int lane, int left) {
@@ -237,29 +224,8 @@ __device__ __forceinline__ void gate_pair(uint64_t x, uint64_t a, uint64_t b, ui
 // ---- affine maps h -> A h + H, per channel -----------------------------------
 // A is never negative as a product of gates; a set sign bit marks a map that
 // restarts (h -> H whatever h is, even where h is infinite or NaN).
-struct Map4 {
-  float A[4], H[4];
-};
 __device__ __forceinline__ bool restarts(float A) { return __float_as_uint(A) >> 31; }
 __device__ __forceinline__ float apply(float A, float H, float h) { return restarts(A) ? H : fmaf(A, h, H); }
-__device__ __forceinline__ void compose(Map4 &first, const Map4 &then) {
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    first.H[j] = apply(then.A[j], then.H[j], first.H[j]);
-    first.A[j] = restarts(then.A[j]) ? then.A[j] : then.A[j] * first.A[j];
-  }
-}
-// shared-memory rows of maps: 128 float2 (A, H), a lane's four side by side
-__device__ __forceinline__ void put_map(float2 *row, int lane, const Map4 &m) {
-  float4 *p = reinterpret_cast<float4 *>(row + 4 * lane);
-  p[0] = make_float4(m.A[0], m.H[0], m.A[1], m.H[1]);
-  p[1] = make_float4(m.A[2], m.H[2], m.A[3], m.H[3]);
-}
-__device__ __forceinline__ Map4 get_map(const float2 *row, int lane) {
-  const float4 *p = reinterpret_cast<const float4 *>(row + 4 * lane);
-  const float4 a = p[0], b = p[1];
-  return Map4{{a.x, a.z, b.x, b.z}, {a.y, a.w, b.y, b.w}};
-}
 
 // ---- words handed from chunk to chunk -----------------------------------------
 // A word is a map (A low, H high) or a state (0 low, h high) in 64 bits that is
@@ -268,46 +234,6 @@ __device__ __forceinline__ Map4 get_map(const float2 *row, int lane) {
 // NaN that an operation returns is 0x7fffffff); keep_apart covers the case that
 // a NaN was only passed through.
 __device__ __forceinline__ uint64_t keep_apart(uint64_t w) { return w == kEmptyWord ? w >> 1 : w; }
-__device__ __forceinline__ void put_words(uint64_t *dst, int lane, const float (&lo)[4], const float (&hi)[4]) {
-  uint64_t w[4];
-#pragma unroll
-  for (int j = 0; j < 4; ++j) w[j] = keep_apart(f2_pack(lo[j], hi[j]));
-  uint64_t *p = dst + 4 * lane;
-  asm volatile("st.relaxed.gpu.global.v2.b64 [%0], {%1, %2};" ::"l"(p), "l"(w[0]), "l"(w[1]) : "memory");
-  asm volatile("st.relaxed.gpu.global.v2.b64 [%0], {%1, %2};" ::"l"(p + 2), "l"(w[2]), "l"(w[3]) : "memory");
-}
-__device__ __forceinline__ void try_words(const uint64_t *src, int lane, uint64_t (&w)[4]) {
-  const uint64_t *p = src + 4 * lane;
-  asm volatile("ld.relaxed.gpu.global.v2.b64 {%0, %1}, [%2];" : "=l"(w[0]), "=l"(w[1]) : "l"(p) : "memory");
-  asm volatile("ld.relaxed.gpu.global.v2.b64 {%0, %1}, [%2];" : "=l"(w[2]), "=l"(w[3]) : "l"(p + 2) : "memory");
-}
-__device__ __forceinline__ bool have_words(const uint64_t (&w)[4]) {
-  return w[0] != kEmptyWord && w[1] != kEmptyWord && w[2] != kEmptyWord && w[3] != kEmptyWord;
-}
-// Waits (bounded) until all lanes' words are there.  A wait that runs out
-// records device status 2 and goes on with zeros, as do all later waits of the
-// CTA; nothing hangs.
-__device__ __noinline__ void wait_words_slow(const uint64_t *src, int lane, uint64_t (&w)[4],
-                                             volatile int *broken) {
-  const long long t0 = clock64();
-  const long long limit = wait_limit_cycles();
-  while (true) {
-    for (int i = 0; i < 32; ++i) {
-      try_words(src, lane, w);
-      if (have_words(w)) return;
-    }
-    if (*broken || clock64() - t0 > limit) {
-      if (!*broken) set_device_status(kDevStatusWaitTimeout);
-      *broken = 1;
-      w[0] = w[1] = w[2] = w[3] = 0;
-      return;
-    }
-  }
-}
-__device__ __forceinline__ Map4 as_map(const uint64_t (&w)[4]) {
-  return Map4{{f2_lo(w[0]), f2_lo(w[1]), f2_lo(w[2]), f2_lo(w[3])},
-              {f2_hi(w[0]), f2_hi(w[1]), f2_hi(w[2]), f2_hi(w[3])}};
-}
 
 // ---- 8-bit groups ---------------------------------------------------------------
 // 128 neighbouring values of a row share one power of two 2^(E - 127), E in one

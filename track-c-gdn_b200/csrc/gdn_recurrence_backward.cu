@@ -503,7 +503,7 @@ recurrence_params_kernel(const float2 *partials, const Header *hdr, const Seqs s
   __shared__ float2 part[32][33];
   if (hdr->bad) return;
   const int64_t total = s.total();
-  const int64_t chunks = total > 0 ? (total - 1) / kChunkTok + 1 : 0;
+  const int64_t chunks = total > 0 ? (total - 1) / kRows + 1 : 0;
   const int64_t channel = static_cast<int64_t>(blockIdx.x) * 32 + threadIdx.x, width = (D + 127) / 128 * 128;
   float2 v = make_float2(0.f, 0.f);
 #pragma unroll 8

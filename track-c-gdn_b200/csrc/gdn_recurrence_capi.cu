@@ -42,6 +42,13 @@ bool tma_rows(const void *p, int type, int64_t stride) {
   return aligned(p, 16) && stride * type_size(type) % 16 == 0 && stride > 0;
 }
 
+// Whether rows of D elements at p, `stride` elements apart, share memory with the
+// dense [T, D] at q.
+bool rows_overlap(const void *p, int64_t stride, const void *q, int type, int64_t T, int64_t D) {
+  const size_t e = type_size(type);
+  return p && q && T > 0 && overlap(p, ((T - 1) * stride + D) * e, q, static_cast<size_t>(T) * D * e);
+}
+
 gdn::rec::Seqs sequences(const int64_t *cu, int64_t N, int64_t T, const int32_t *slots, int64_t pool) {
   return gdn::rec::Seqs{cu, N, T, N > 0 ? T / N : 0, slots, pool};
 }
@@ -103,6 +110,11 @@ int gdn_recurrence_prefill(int type, const void *x, int64_t x_stride, const void
     return GDN_ERR_WORKSPACE;
   const size_t states = static_cast<size_t>(slots ? pool_slots : num_seqs) * channels * 4;
   if (state && state != final_state && overlap(state, states, final_state, states)) return GDN_ERR_ALIASING;
+  // rows are read again after others have been written (chunks cut by streams)
+  if (rows_overlap(x, x_stride, out, type, total_tokens, channels) ||
+      rows_overlap(a, a_stride, out, type, total_tokens, channels) ||
+      rows_overlap(b, b_stride, out, type, total_tokens, channels))
+    return GDN_ERR_ALIASING;
   int sms = 0;
   if (int st = check_device(&sms)) return st;
   gdn::rec::Forward p{};
@@ -141,6 +153,13 @@ int gdn_recurrence_backward(int type, const void *x, int64_t x_stride, const voi
   if (d_state && ((state && overlap(state, states, d_state, states)) ||
                   (d_final_state && overlap(d_final_state, states, d_state, states))))
     return GDN_ERR_ALIASING;
+  for (void *g : {dx, da, db}) {
+    if (rows_overlap(d_out, d_out_stride, g, type, total_tokens, channels)) return GDN_ERR_ALIASING;
+    if (!packed && (rows_overlap(x, x_stride, g, type, total_tokens, channels) ||
+                    rows_overlap(a, a_stride, g, type, total_tokens, channels) ||
+                    rows_overlap(b, b_stride, g, type, total_tokens, channels)))
+      return GDN_ERR_ALIASING;
+  }
   int sms = 0;
   if (int st = check_device(&sms)) return st;
   cudaStream_t s = static_cast<cudaStream_t>(stream);

@@ -260,7 +260,7 @@ recurrence_forward_kernel(const __grid_constant__ Forward p) {
       const Table<kRows> &tab = sh.tables[s];
       const int64_t chunk = tab.chunk;
       if (chunk < 0) return;
-      const bool last_chunk = tab.last, enters = !(tab.starts[0] & 1);
+      const bool last_chunk = tab.last, enters = !(tab.starts[0] & 1), only_map = tab.only_map;
       const int64_t lane_ch = static_cast<int64_t>(tab.d) * kCh + 64 * half + 2 * lane;
       const int64_t row_ch = static_cast<int64_t>(nt) * kCh;
       const int64_t group = group_len == 1 ? chunk : chunk / kGroupLen;
@@ -269,7 +269,7 @@ recurrence_forward_kernel(const __grid_constant__ Forward p) {
       const int before = from_state ? place : static_cast<int>(tab.reach);
       // the words that are wanted, asked for before the first pass is done: maps
       // of the chunks before, and the state that enters the first of them
-      const bool looks = kChain && enters && !tab.only_map;
+      const bool looks = kChain && enters && !only_map;
       const bool groups = kChain && group_len > 1;
       Words2 w[kGroupLen];
       auto src = [&](int j) {
@@ -286,7 +286,7 @@ recurrence_forward_kernel(const __grid_constant__ Forward p) {
                                        wait_phase(smem_u32(&sh.taken[s][half]), parity, &sh.broken)))
         return;
       float4 *own = &sh.own[s][half][0][lane];
-      const bool publishes = kChain && !last_chunk && !tab.only_map && place == group_len - 1;
+      const bool publishes = kChain && !last_chunk && !only_map && place == group_len - 1;
       if (kChain && !groups) {
         h = 0;
         if (looks && from_state) {
@@ -321,7 +321,7 @@ recurrence_forward_kernel(const __grid_constant__ Forward p) {
       if (publishes && !groups) put_words2(states + group * row_ch + lane_ch, 0, h);
       __syncwarp();
       if (lane == 0) mbar_arrive(smem_u32(&sh.ready[s]));
-      if (p.carries != nullptr && !tab.only_map)
+      if (p.carries != nullptr && !only_map)  // the table may hold another tile by now
         store2_f32<kVec>(p.carries + chunk * ((p.D + 127) / 128 * 128) + lane_ch - 2 * lane, lane, 64, h_in);
     }
   }
