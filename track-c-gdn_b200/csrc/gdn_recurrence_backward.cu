@@ -362,7 +362,7 @@ recurrence_backward_kernel(const __grid_constant__ Backward p) {
         const uint64_t w = f2_fma(in[1], f2_dup(kLog2e), par.dt), sp = softplus2(w, ex2_neg_abs(w));
         const uint64_t beta = sigmoid_pair(in[2]);
         sh.kept[warp][i][lane] = make_ulonglong2(sp, beta);
-        uint64_t g = gate_ex2(f2_mul(par.c, sp)), u = f2_mul(beta, in[0]);
+        uint64_t g = gate_of(par.c, sp), u = f2_mul(beta, in[0]);
         if (edge) {
           if (i >= valid) g = f2_dup(1.f), u = 0, o = 0;
           if ((starts >> i) & 1) y = initial(tab, c0, i);
@@ -446,7 +446,7 @@ recurrence_backward_kernel(const __grid_constant__ Backward p) {
             // most; the difference of two infinities counts as that)
             const uint64_t w = f2_fma(in[1], f2_dup(kLog2e), par.dt), ls = f2_fma(sp, f2_dup(-1.f), w);
             const uint64_t sig = ex2_pair(f2_pack(fminf(f2_lo(ls), 0.f), fminf(f2_hi(ls), 0.f)));
-            g[j] = gate_ex2(f2_mul(par.c, sp));
+            g[j] = gate_of(par.c, sp);
             const uint64_t gh = f2_mul(g[j], h), cgh = f2_mul(par.c, gh);  // -exp(A_log) g h_{t-1}
             h = f2_fma(g[j], h, f2_mul(beta[j], in[0]));
             ca[j] = f2_mul(cgh, sig);

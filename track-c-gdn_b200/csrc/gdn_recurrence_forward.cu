@@ -15,7 +15,7 @@ struct FwdShape {
   static constexpr int kHalves = kPack ? 2 : 1;
   static constexpr int kCh = 64 * kHalves;
   static constexpr int kWorkers = kSlots * kHalves;       // consumer warps
-  static constexpr int kThreads = 32 * (kWorkers + 1 + 2 * kHalves);
+  static constexpr int kThreads = 32 * (kWorkers + 1 + kHalves);
   static constexpr int kPitch = row_pitch<static_cast<int>(sizeof(E))>(kFetch);
   static constexpr int kPlane = kFetch == kDirect ? kRows * 512 : kRows * kPitch;
   // where a lane's 16 bytes of row i (of its 8) lie: kPerPlane rows in the
@@ -76,9 +76,10 @@ struct FwdShared {
 //              (P, y) of the slot, and the tile's, which is published.  Second
 //              pass, one tile later (kDefer): out = y + P h, with h the state
 //              that enters the slot.
-//   chain      (two per half, for tiles in turn) looks back and hands each slot
-//              its state.  It has the time of two first passes for that, so
-//              that the look-back's latency costs the consumers nothing.
+//   chain      (one per half) looks back and hands each slot its state.  It has
+//              the time of a first pass for that.  (Two per half, for tiles in
+//              turn, leave 80 instead of 96 registers a thread: 65536 x 1024
+//              fp32 274 instead of 218 us, elsewhere the same.)
 // Without kChain (short inputs, one launch) a CTA walks all chunks of its
 // channels and the chain warp keeps the state.
 template <typename E, Fetch kFetch, bool kPack, bool kChain>
@@ -136,7 +137,7 @@ recurrence_forward_kernel(const __grid_constant__ Forward p) {
       st = p.hdr->stream[stream];
       if (lane == 0) ticket = atomicAdd(&p.hdr->stream[stream].ticket, 1u);
     }
-    int k = 0, ends = 0;
+    int k = 0;
     while (true) {
       int64_t chunk = -1;
       int d = blockIdx.x;
@@ -181,9 +182,7 @@ recurrence_forward_kernel(const __grid_constant__ Forward p) {
           mbar_arrive(full);
         }
         if (kFetch == kRowCopies) mbar_arrive(full);
-        ++k;
-        if (++ends == 2) break;  // one for each chain warp
-        continue;
+        break;
       }
       if (kChain && lane == 0) {
         mbar_expect_tx(full, 2 * kCh * 4);
@@ -243,17 +242,16 @@ recurrence_forward_kernel(const __grid_constant__ Forward p) {
     // after a wait that ran out: no copy may be in flight when the CTA ends
     if (kFetch == kRowCopies) wait_copies();
     if ((kFetch != kDirect || kChain) && *static_cast<volatile int *>(&sh.broken))
-      for (int i = max(k - kStages, 0); i < k - ends; ++i)
+      for (int i = max(k - kStages, 0); i < k; ++i)
         mbar_wait(smem_u32(&sh.full[i % kStages]), (i / kStages) & 1);
     return;
   }
 
   if (warp > S::kWorkers) {
     // ---- chain ----
-    const int half = (warp - S::kWorkers - 1) >> 1, odd = (warp - S::kWorkers - 1) & 1;
-    if (!kChain && odd) return;
+    const int half = warp - S::kWorkers - 1;
     uint64_t h = 0;
-    for (int k = odd;; k += kChain ? 2 : 1) {
+    for (int k = 0;; ++k) {
       const int s = k % kStages;
       const uint32_t parity = (k / kStages) & 1;
       if (!__all_sync(0xffffffffu, wait_phase(smem_u32(&sh.full[s]), parity, &sh.broken))) return;
