@@ -41,8 +41,8 @@ struct Decode {
 };
 
 // A warp takes one request's 128 channels through its tokens, the state in
-// registers: 16 bytes a channel and token for 2-byte types (state in and out
-// and four vectors), bound by HBM for large batches, by latency for small.
+// registers: 8 bytes a channel and token and 8 for the state for 2-byte types,
+// bound by HBM for large batches, by latency for small.
 template <typename E, bool kVec>
 __global__ void __launch_bounds__(kThreads) recurrence_decode_kernel(const __grid_constant__ Decode p) {
   const int lane = threadIdx.x & 31;
@@ -82,6 +82,44 @@ __global__ void __launch_bounds__(kThreads) recurrence_decode_kernel(const __gri
                   make_float4(f2_lo(h[0]), f2_hi(h[0]), f2_lo(h[1]), f2_hi(h[1])));
 }
 
+// One token: all loads before the first use, nothing else in registers.  A warp
+// to a request's 128 channels: two or four requests a warp, their loads all in
+// flight at once, were no faster (4096 x 1024 bf16 in a pool, not in L2: 13.8 us,
+// 4.9 TB/s; 14.0 and 14.4 us with two and four).
+template <typename E, bool kVec>
+__global__ void __launch_bounds__(kThreads) recurrence_decode_one_kernel(const __grid_constant__ Decode p) {
+  const int lane = threadIdx.x & 31;
+  const int nd = static_cast<int>((p.D + kTileCh - 1) / kTileCh);
+  const int64_t item = static_cast<int64_t>(blockIdx.x) * kWarps + (threadIdx.x >> 5);
+  if (item >= p.B * nd) return;
+  const int64_t req = item / nd, c0 = item % nd * kTileCh;
+  const int left = static_cast<int>(min(p.D - c0, int64_t{kTileCh}));
+  const Raw<E> x = load4<E, kVec>(static_cast<const E *>(p.x) + req * p.x_stride + c0, lane, left);
+  const Raw<E> a = load4<E, kVec>(static_cast<const E *>(p.a) + req * p.a_stride + c0, lane, left);
+  const Raw<E> b = load4<E, kVec>(static_cast<const E *>(p.b) + req * p.b_stride + c0, lane, left);
+  const Params par = load_params<kVec>(p.A_log + c0, p.dt_bias + c0, lane, left);
+  const int64_t row = p.slots != nullptr ? p.slots[req] : req;
+  if (p.slots != nullptr && (row < 0 || row >= p.pool)) {
+    if (lane == 0) set_device_status(kDevStatusBadSlot);
+    return;
+  }
+  const float4 s = p.state != nullptr ? load_f32<kVec>(p.state + row * p.D + c0, lane, left)
+                                      : make_float4(0.f, 0.f, 0.f, 0.f);
+  uint64_t xp[2], ap[2], bp[2], h[2] = {f2_pack(s.x, s.y), f2_pack(s.z, s.w)};
+  x.pairs(xp[0], xp[1]);
+  a.pairs(ap[0], ap[1]);
+  b.pairs(bp[0], bp[1]);
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    uint64_t g, u;
+    gate_pair(xp[k], ap[k], bp[k], par.dt[k], par.c[k], g, u);
+    h[k] = f2_fma(g, h[k], u);
+  }
+  store4<E, kVec>(static_cast<E *>(p.out) + req * p.D + c0, lane, left, h[0], h[1]);
+  store_f32<kVec>(p.new_state + row * p.D + c0, lane, left,
+                  make_float4(f2_lo(h[0]), f2_hi(h[0]), f2_lo(h[1]), f2_hi(h[1])));
+}
+
 // ---- sizes and launches ----------------------------------------------------------
 inline size_t saved_bytes(int64_t T, int64_t D) {  // the states before every 64th row
   return static_cast<size_t>(chunks_of(T) * tiles_of(D) * kTileCh * 4);
@@ -90,7 +128,9 @@ inline size_t saved_bytes(int64_t T, int64_t D) {  // the states before every 64
 template <typename E>
 cudaError_t launch_decode_e(const Decode &p, bool vec, cudaStream_t stream) {
   const int64_t blocks = (p.B * tiles_of(p.D) + kWarps - 1) / kWarps;
-  auto kernel = vec ? recurrence_decode_kernel<E, true> : recurrence_decode_kernel<E, false>;
+  auto kernel = p.tokens == 1 && p.inter == nullptr
+                    ? (vec ? recurrence_decode_one_kernel<E, true> : recurrence_decode_one_kernel<E, false>)
+                    : (vec ? recurrence_decode_kernel<E, true> : recurrence_decode_kernel<E, false>);
   kernel<<<static_cast<unsigned>(blocks), kThreads, 0, stream>>>(p);
   return cudaGetLastError();
 }

@@ -184,8 +184,9 @@ def decode(x, state, A_log, a, dt_bias, b, return_intermediate: bool = False):
     """Decode with a fresh new state: x, a, b [B, D] or [B, T, D], state [B, D]
     fp32 or None.  Returns (out, new_state), and with return_intermediate the
     states after each token [B, T, D] fp32 too."""
-    out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    new_state = torch.empty(x.shape[0], x.shape[-1], dtype=torch.float32, device=x.device)
+    out = x.new_empty(x.shape)
+    new_state = (torch.empty(x.shape[0], x.shape[-1], dtype=torch.float32, device=x.device) if state is None
+                 else state.new_empty(state.shape))
     inter = None
     if return_intermediate:
         T = x.shape[1] if x.dim() == 3 else 1
@@ -197,7 +198,7 @@ def decode(x, state, A_log, a, dt_bias, b, return_intermediate: bool = False):
 
 def decode_inplace(x, state, A_log, a, dt_bias, b):
     """Decode with `state` [B, D] updated in place.  Returns out."""
-    out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    out = x.new_empty(x.shape)
     decode_into(x, state, A_log, a, dt_bias, b, out, state)
     return out
 
@@ -205,7 +206,7 @@ def decode_inplace(x, state, A_log, a, dt_bias, b):
 def decode_pool(x, state_pool, slots, A_log, a, dt_bias, b):
     """Decode with request i's state in state_pool[slots[i]] ([P, D] fp32,
     updated in place; slots [B] int32, distinct).  Returns out."""
-    out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    out = x.new_empty(x.shape)
     decode_into(x, state_pool, A_log, a, dt_bias, b, out, state_pool, slots=slots)
     return out
 
@@ -271,7 +272,7 @@ def run(x, state, A_log, a, dt_bias, b, cu_seqlens: Optional[torch.Tensor] = Non
     (out, final_state [N, D] fp32)."""
     T, N, _ = _sequences(x, cu_seqlens)
     D = x.shape[-1]
-    out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    out = x.new_empty(x.shape)
     final_state = torch.empty(N, D, dtype=torch.float32, device=x.device)
     _prefill(x, None if state is None else state.contiguous(), A_log, a, dt_bias, b, cu_seqlens, out, final_state,
              alloc_workspace(T, D, x.device), zero_behind=True)
@@ -290,7 +291,7 @@ def run_pool(x, state_pool, slots, A_log, a, dt_bias, b, cu_seqlens: Optional[to
     """`run` with the states in a pool ([P, D] fp32, updated in place at
     slots [N] int32, distinct).  Returns out."""
     T, _, _ = _sequences(x, cu_seqlens)
-    out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    out = x.new_empty(x.shape)
     _prefill(x, state_pool, A_log, a, dt_bias, b, cu_seqlens, out, state_pool,
              alloc_workspace(T, x.shape[-1], x.device), slots=slots, zero_behind=True)
     return out
@@ -364,11 +365,9 @@ _NAMES = ("dx", "da", "db", "dA_log", "ddt_bias", "d_state")
 
 
 def _gradients(like, D, N, need_d_state):
-    empty, dtype, dev, f32 = torch.empty, like.dtype, like.device, torch.float32
-    shape = like.shape
-    return (empty(shape, dtype=dtype, device=dev), empty(shape, dtype=dtype, device=dev),
-            empty(shape, dtype=dtype, device=dev), empty(D, dtype=f32, device=dev), empty(D, dtype=f32, device=dev),
-            empty(N, D, dtype=f32, device=dev) if need_d_state else None)
+    shape, params = like.shape, torch.empty(D, dtype=torch.float32, device=like.device)
+    return (like.new_empty(shape), like.new_empty(shape), like.new_empty(shape), params, params.new_empty(D),
+            params.new_empty((N, D)) if need_d_state else None)
 
 
 @torch.no_grad()
@@ -405,7 +404,7 @@ class _RecurrenceFunction(torch.autograd.Function):
         if state is not None:
             _check_states("state", state, N, D, dev)
             state = state.contiguous()
-        out = torch.empty(x.shape, dtype=x.dtype, device=dev)
+        out = x.new_empty(x.shape)
         final_state = torch.empty(N, D, dtype=torch.float32, device=dev)
         carry_bytes, packed_bytes = _saved_bytes(T, D)
         carries = torch.empty(carry_bytes, dtype=torch.uint8, device=dev)
