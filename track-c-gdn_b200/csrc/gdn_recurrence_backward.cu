@@ -554,7 +554,7 @@ cudaError_t launch_backward_t(Backward p, void *workspace, int sms, float *dA_lo
   p.dt = w.dt, p.c = w.c, p.first = w.first;
   const int64_t words = (chunks + (chunks + kGroupLen - 1) / kGroupLen) * nt * 64;
   const Prepared q{p.A_log,     p.dt_bias, w.dt,  w.c, p.D, w.first, chunks, kRows,
-                   streams_for(nt, int64_t{sms} * S::kCtas), true, nullptr, nullptr};
+                   streams_for(nt, int64_t{sms} * S::kCtas), nt, int64_t{sms} * S::kCtas, true, nullptr, nullptr};
   if (cudaError_t e = launch_init(p.hdr, p.maps, words, p.s, q, stream)) return e;
   kernel<<<static_cast<unsigned>(min(chunks * nt, int64_t{sms} * S::kCtas)), S::kThreads, smem, stream>>>(p);
   if (cudaError_t e = cudaGetLastError()) return e;

@@ -600,7 +600,7 @@ cudaError_t launch_forward_t(Forward p, void *workspace, int sms, cudaStream_t s
     p.first = w.first;
     const int64_t words = (chunks + (chunks + kGroupLen - 1) / kGroupLen) * nt * S::kCh;
     const Prepared q{p.A_log,     p.dt_bias, w.dt,  w.c, p.D, w.first, chunks, kRows,
-                     streams_for(nt, int64_t{sms} * S::kCtas), false,
+                     streams_for(nt, int64_t{sms} * S::kCtas), nt, int64_t{sms} * S::kCtas, false,
                      p.aside != nullptr ? p.state : nullptr, w.aside};
     if (cudaError_t e = launch_init(p.hdr, p.maps, words, p.s, q, stream)) return e;
     blocks = min(chunks * nt, int64_t{sms} * S::kCtas);

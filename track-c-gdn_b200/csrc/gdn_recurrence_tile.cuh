@@ -15,8 +15,9 @@ namespace rec {
 // Chunks joined through one published state: 8 where one sequence (or a few) has
 // to be worked on by all CTAs at once -- a state then travels one link of about
 // 0.75 us for 8 chunks (65536 x 1024 bf16: 185 us; groups of 4: 214, 16: 212,
-// 2: 380) -- and 1 where the streams leave about one chunk of each in work,
-// whose predecessor is done: then a state per chunk is all that is published.
+// 2: 380) -- and 1 where streams and tiles of channels together give most CTAs a
+// tile of a chunk whose predecessor is done: then a state per chunk is all that
+// is published.
 constexpr int kGroupLen = 8;
 
 constexpr int kTokW = 8;
@@ -120,6 +121,7 @@ struct Prepared {
   int *first;       // [chunks + 1], or null
   int64_t chunks, rows;
   int streams;      // as many as wanted, at most kStreams
+  int64_t tiles, ctas;  // of channels; that work at once
   bool backwards;   // the chain runs from the last chunk to the first
   // States that the call updates in place (else null): a sequence that starts
   // in a cut chunk and goes on behind it is finished by the stream that begins
@@ -195,7 +197,7 @@ __global__ void __launch_bounds__(1024) recurrence_init_kernel(Header *hdr, ulon
           ++n;
         }
       hdr->streams = n;
-      hdr->group = 2 * n > q.streams && q.streams > 1 ? 1 : kGroupLen;
+      hdr->group = 2 * n * q.tiles >= q.ctas ? 1 : kGroupLen;
       hdr->bad = code != 0;
       if (code) set_device_status(code);
     }
@@ -584,10 +586,12 @@ inline Places places(void *workspace, int64_t T, int64_t D) {
                 words + 8 * (chunks + (chunks + kGroupLen - 1) / kGroupLen) * width};
 }
 
-// Streams for nt tiles of channels on `ctas` CTAs: about as many CTAs to a stream
-// as it has tiles of channels, so that the chunk before is done or nearly so.
+// Streams for nt tiles of channels on `ctas` CTAs: about two tiles of channels to a
+// CTA of the stream, so that the chunk before is done when a tile's turn comes
+// and there is a stream left to join for CTAs whose own has ended (1.1 M x 1024
+// bf16 1951 us with half as many, 1897; backward of 47000 x 1024 294 and 272).
 inline int streams_for(int64_t nt, int64_t ctas) {
-  return static_cast<int>(max(int64_t{1}, min(int64_t{kStreams}, ctas / nt)));
+  return static_cast<int>(max(int64_t{1}, min(int64_t{kStreams}, 2 * ctas / nt)));
 }
 
 }  // namespace rec
