@@ -413,23 +413,18 @@ recurrence_forward_kernel(const __grid_constant__ Forward p) {
           return r;
         }
       };
-      auto fetch = [&](int w) {
+#pragma unroll
+      for (int w = 0; w < 3; ++w)
 #pragma unroll
         for (int i = 0; i < kTokW; ++i) raw[w][i] = fetch_row(w, i);
-      };
       if constexpr (kPack) {
         // The groups' largest magnitudes: each half by one warp, joined through
         // shared memory.  Lane 8 w + i holds what belongs to row i of x, a or b.
-        // The values are fetched anew for each use, not kept: registers are scarcer.
         uint32_t mine = 0;
 #pragma unroll
         for (int w = 0; w < 3; ++w) {
-          fetch(w);
-#pragma unroll
-          for (int i = 0; i < kTokW; ++i) {
-            const uint32_t m = __reduce_max_sync(0xffffffffu, raw[w][i].abs_max());
-            if (lane == kTokW * w + i) mine = m;
-          }
+          const uint32_t m = row_maximum(raw[w], lane);
+          if (lane / kTokW == w) mine = m;
         }
         uint32_t *amax = sh.amax + ((k & 1) * kSlots + slot) * 64;
         amax[32 * half + lane] = mine;
@@ -453,7 +448,6 @@ recurrence_forward_kernel(const __grid_constant__ Forward p) {
 #pragma unroll
           for (int w = 0; w < 3; ++w) {
             uint16_t *dst = reinterpret_cast<uint16_t *>(p.packed + (w * p.s.T + t0) * p.D + c0) + lane;
-            fetch(w);
             float f[kTokW];
 #pragma unroll
             for (int i = 0; i < kTokW; i += 4)
@@ -488,9 +482,6 @@ recurrence_forward_kernel(const __grid_constant__ Forward p) {
           }
         }
       }
-      asm volatile("" ::: "memory");
-#pragma unroll
-      for (int w = 0; w < 3; ++w) fetch(w);
       __syncwarp();  // the warp's rows are overwritten from here on
       auto keep = [&](int i, uint64_t y, uint64_t P) {
         *reinterpret_cast<ulonglong2 *>(stage + i / S::kPerPlane * S::kPlane + i % S::kPerPlane * 512 +

@@ -342,11 +342,12 @@ struct Raw2;
 template <>
 struct Raw2<__nv_bfloat16> {
   uint32_t v;
-  // the larger magnitude as bits whose order is that of the values, and those
-  // bits as an fp32's
-  __device__ __forceinline__ uint32_t abs_max() const {  // in both halves
-    const __nv_bfloat162 a = *reinterpret_cast<const __nv_bfloat162 *>(&v);
-    const __nv_bfloat162 m = __hmax2_nan(__habs2(a), __habs2(__lowhigh2highlow(a)));
+  // magnitudes as bits whose order is that of the values, the larger of two for
+  // each half, and one as an fp32's bits
+  __device__ __forceinline__ uint32_t magnitudes() const { return v & 0x7fff7fffu; }
+  __device__ static __forceinline__ uint32_t larger(uint32_t a, uint32_t b) {
+    const __nv_bfloat162 m =
+        __hmax2_nan(*reinterpret_cast<const __nv_bfloat162 *>(&a), *reinterpret_cast<const __nv_bfloat162 *>(&b));
     return *reinterpret_cast<const uint32_t *>(&m);
   }
   __device__ static __forceinline__ uint32_t magnitude(uint32_t m) { return m << 16; }
@@ -355,9 +356,9 @@ struct Raw2<__nv_bfloat16> {
 template <>
 struct Raw2<__half> {
   uint32_t v;
-  __device__ __forceinline__ uint32_t abs_max() const {  // in both halves
-    const __half2 a = *reinterpret_cast<const __half2 *>(&v);
-    const __half2 m = __hmax2_nan(__habs2(a), __habs2(__lowhigh2highlow(a)));
+  __device__ __forceinline__ uint32_t magnitudes() const { return v & 0x7fff7fffu; }
+  __device__ static __forceinline__ uint32_t larger(uint32_t a, uint32_t b) {
+    const __half2 m = __hmax2_nan(*reinterpret_cast<const __half2 *>(&a), *reinterpret_cast<const __half2 *>(&b));
     return *reinterpret_cast<const uint32_t *>(&m);
   }
   __device__ static __forceinline__ uint32_t magnitude(uint32_t m) {
@@ -371,12 +372,39 @@ struct Raw2<__half> {
 template <>
 struct Raw2<float> {
   float2 v;
-  __device__ __forceinline__ uint32_t abs_max() const {
+  __device__ __forceinline__ uint32_t magnitudes() const {  // of both in one
     return max(__float_as_uint(v.x) & 0x7fffffffu, __float_as_uint(v.y) & 0x7fffffffu);
   }
+  __device__ static __forceinline__ uint32_t larger(uint32_t a, uint32_t b) { return max(a, b); }
   __device__ static __forceinline__ uint32_t magnitude(uint32_t m) { return m; }
   __device__ __forceinline__ uint64_t pair() const { return f2_pack(v.x, v.y); }
 };
+
+// The largest magnitude of row l % 8 over the warp's 64 channels, in lane l: each
+// exchange halves the rows that a lane still holds, so 9 exchanges serve 8 rows
+// where a redux per row takes 8 of a slower pipe.  8 x 4096 x 2048 bf16 with
+// 8-bit copies: 202 -> 190 us, with the rows fetched once instead of twice.
+template <typename E>
+__device__ __forceinline__ uint32_t row_maximum(const Raw2<E> (&r)[kTokW], int lane) {
+  static_assert(kTokW == 8, "three halvings");
+  using R = Raw2<E>;
+  uint32_t v[kTokW];
+#pragma unroll
+  for (int i = 0; i < kTokW; ++i) v[i] = r[i].magnitudes();
+#pragma unroll
+  for (int step = 4; step >= 1; step /= 2) {
+    const bool high = lane & step;
+#pragma unroll
+    for (int j = 0; j < step; ++j) {
+      const uint32_t given = __shfl_xor_sync(0xffffffffu, high ? v[j] : v[j + step], step);
+      v[j] = R::larger(high ? v[j + step] : v[j], given);
+    }
+  }
+#pragma unroll
+  for (int step = 8; step <= 16; step *= 2) v[0] = R::larger(v[0], __shfl_xor_sync(0xffffffffu, v[0], step));
+  if constexpr (sizeof(E) == 2) return R::larger(v[0], __byte_perm(v[0], v[0], 0x1032)) & 0xffffu;
+  return v[0];
+}
 
 template <typename E, bool kVec>
 __device__ __forceinline__ Raw2<E> load2(const E *p, int lane, int left) {
