@@ -7,9 +7,11 @@ namespace rec {
 
 // Shape of a tile: 64 rows x 64 channels for 8 consumer warps, or with kPack
 // the 128 channels that share a scale for 16.  A lane has 2 channels of 8
-// consecutive rows.  A stage of shared memory holds one half (64 channels) as
-// planes of x, a and b, and afterwards, in place, what the first pass left: 16
-// bytes for each lane and row.
+// consecutive rows, a warp's slot.  A stage of shared memory holds one half (64
+// channels) of x, a and b, and afterwards, in place of rows that the same warp
+// has read, what the first pass left: 16 bytes for each lane and row.  A tensor
+// copy brings a plane of all 64 rows at a time; row copies lay a slot's rows of
+// the three planes side by side, which fits the 16 bytes exactly.
 template <typename E, Fetch kFetch, bool kPack>
 struct FwdShape {
   static constexpr int kHalves = kPack ? 2 : 1;
@@ -17,17 +19,17 @@ struct FwdShape {
   static constexpr int kWorkers = kSlots * kHalves;       // consumer warps
   static constexpr int kThreads = 32 * (kWorkers + 1 + kHalves);
   static constexpr int kPitch = row_pitch<static_cast<int>(sizeof(E))>(kFetch);
-  static constexpr int kPlane = kFetch == kDirect ? kRows * 512 : kRows * kPitch;
-  // where a lane's 16 bytes of row i (of its 8) lie: kPerPlane rows in the
-  // slot's part of each plane; only rows that this warp alone reads are overwritten
-  static constexpr int kPerPlane = kFetch == kDirect ? kTokW : sizeof(E) == 4 ? 4 : 2;
-  static constexpr int kHalfStage = (kFetch == kDirect ? 1 : sizeof(E) == 4 ? 3 : 4) * kPlane;
+  static constexpr int kRead = kFetch == kDirect ? 0 : 3 * kTokW * kPitch, kLeft = kTokW * 512;  // bytes of a slot
+  static constexpr int kSlotStep = kFetch == kTmaTile ? kTokW * kPitch : kRead > kLeft ? kRead : kLeft;
+  static constexpr int kPlane = kFetch == kTmaTile ? kRows * kPitch : kTokW * kPitch;
+  // where a lane's 16 bytes of row i lie: kPerPlane rows in the slot's part of each plane
+  static constexpr int kPerPlane = kFetch != kTmaTile ? kTokW : sizeof(E) == 4 ? 4 : 2;
+  static constexpr int kHalfStage = kSlots * (kRead > kLeft ? kRead : kLeft);
   static constexpr int kStage = kHalves * kHalfStage;
   static constexpr int kStages = kHalfStage > 32768 ? 2 : 3;
-  // The second pass is put off by a tile, but not with two stages of row copies:
-  // the next tile's copies, which take long, would have to wait for it (47000 x
-  // 1021 fp16: 295 against 269 us; with tensor copies it still pays: 65536 x
-  // 1024 fp32 266 against 315 us).
+  // The second pass is put off by a tile where there is a stage for it (47000 x
+  // 1021 fp16: 254 against 221 us), and with tensor copies even with two stages:
+  // 65536 x 1024 fp32 266 against 315 us.
   static constexpr bool kDefer = kStages > 2 || kFetch == kTmaTile;
   static constexpr int kCtas = kPack || kStages * kStage > 98304 ? 1 : 2;             // of an SM
 };
@@ -52,6 +54,11 @@ struct Forward {
   const int *first;
 };
 
+struct Next {
+  int64_t chunk;  // -1: no more tiles
+  int64_t d;
+};
+
 template <typename Shape, bool kPack>
 struct FwdShared {
   // maps of the slots' rows (A, A, H, H of a lane's channels); the chain warp
@@ -60,17 +67,22 @@ struct FwdShared {
   float params[Shape::kStages][2][Shape::kCh];  // kChain: dt and c of the tile's channels
   Table<kRows> tables[Shape::kStages];
   Tile tiles[Shape::kStages];
+  Next next[Shape::kStages];      // kRowCopies: the tile that comes into a stage
+  uint64_t posted[Shape::kStages];  // ... is known
   uint64_t full[Shape::kStages], ready[Shape::kStages], empty[Shape::kStages];
   uint64_t mapped[Shape::kStages][Shape::kHalves];  // the slots' maps are there
   uint64_t taken[Shape::kStages][Shape::kHalves];   // ... and have been read for the tile's
   uint64_t pair[kPack ? kSlots : 1];
   uint32_t amax[kPack ? 2 * kSlots * 64 : 1];
-  alignas(16) float inverse[kPack ? Shape::kWorkers : 1][32];
+  alignas(16) float inverse[kPack ? Shape::kWorkers : 1][3 * kTokW];
   int broken;
 };
 
 // Roles of the warps, joined by mbarriers alone:
-//   producer   takes tiles by ticket, fills the table, has the inputs copied
+//   producer   takes tiles by ticket, fills the table, has the inputs copied.
+//              Row copies are issued by the consumers, each warp for its own
+//              rows as soon as it is done with a stage: 66 a tile would keep one
+//              warp busy for 4000 cycles (47000 x 1021 fp16: 227 against 204 us).
 //   consumers  first pass: gates; per row the state y from a zero start and the
 //              product P of the gates so far, left in shared memory; the map
 //              (P, y) of the slot, and the tile's, which is published.  Second
@@ -106,7 +118,8 @@ recurrence_forward_kernel(const __grid_constant__ Forward p) {
   if (tid == 0) {
     sh.broken = 0;
     for (int i = 0; i < kStages; ++i) {
-      mbar_init(smem_u32(&sh.full[i]), fetch_arrivals(kFetch));
+      mbar_init(smem_u32(&sh.full[i]), kFetch == kRowCopies ? 1 + 32 * S::kWorkers : 1);
+      mbar_init(smem_u32(&sh.posted[i]), 1);
       for (int w = 0; w < S::kHalves; ++w) {
         mbar_init(smem_u32(&sh.mapped[i][w]), kSlots);
         mbar_init(smem_u32(&sh.taken[i][w]), 1);
@@ -171,6 +184,12 @@ recurrence_forward_kernel(const __grid_constant__ Forward p) {
       }
       if (chunk > last) continue;
       const int s = k % kStages;
+      if (kFetch == kRowCopies && lane == 0) {
+        // read by all consumers before they leave the stage's last tile, which
+        // the wait below saw for the entry that this one replaces
+        sh.next[s] = Next{chunk, d};
+        mbar_arrive(smem_u32(&sh.posted[s]));
+      }
       const bool go = k < kStages || wait_phase(smem_u32(&sh.empty[s]), ((k / kStages) - 1) & 1, &sh.broken);
       if (!__all_sync(0xffffffffu, go)) break;
       Table<kRows> &t = sh.tables[s];
@@ -181,10 +200,17 @@ recurrence_forward_kernel(const __grid_constant__ Forward p) {
           sh.tiles[s].d = -1;
           mbar_arrive(full);
         }
-        if (kFetch == kRowCopies) mbar_arrive(full);
         break;
       }
-      if (kChain && lane == 0) {
+      uint64_t dt[S::kHalves], c[S::kHalves];
+      if constexpr (kChain && kFetch == kRowCopies) {
+#pragma unroll
+        for (int w = 0; w < S::kHalves; ++w) {
+          dt[w] = load2_f32<true>(p.dt + c0 + 64 * w, lane, 64);
+          c[w] = load2_f32<true>(p.c + c0 + 64 * w, lane, 64);
+        }
+      }
+      if (kChain && kFetch != kRowCopies && lane == 0) {
         mbar_expect_tx(full, 2 * kCh * 4);
         bulk_load(smem_u32(sh.params[s][0]), p.dt + c0, kCh * 4, full);
         bulk_load(smem_u32(sh.params[s][1]), p.c + c0, kCh * 4, full);
@@ -200,21 +226,6 @@ recurrence_forward_kernel(const __grid_constant__ Forward p) {
           tma_load_2d(dst + 2 * S::kPlane, &p.tb, x, y, full);
         }
       }
-      if constexpr (kFetch == kRowCopies) {
-        const void *const src[3] = {p.x, p.a, p.b};
-        const int64_t stride[3] = {p.x_stride, p.a_stride, p.b_stride};
-        const int rows = static_cast<int>(min(total - base, int64_t{kRows}));
-#pragma unroll
-        for (int w = 0; w < S::kHalves; ++w) {
-          const int left = static_cast<int>(min(p.D - c0 - 64 * w, int64_t{64}));
-          if (left <= 0) break;
-#pragma unroll
-          for (int j = 0; j < 3; ++j)
-            copy_rows<kElement>(smem_u32(smem + s * S::kStage + w * S::kHalfStage + j * S::kPlane), src[j], stride[j],
-                                base, rows, c0 + 64 * w, left, lane);
-        }
-        arrive_after_copies(full);
-      }
       const bool inside = fill_table<kRows>(p.s, t, base, chunk == last, lane, kChain ? p.first : nullptr, [&](int64_t n) {
         if (p.final == nullptr || only_map) return;  // an empty sequence's final state is its initial state
 #pragma unroll
@@ -225,6 +236,13 @@ recurrence_forward_kernel(const __grid_constant__ Forward p) {
                            p.state != nullptr ? load2_f32<kVec>(p.state + row, lane, left) : 0);
         }
       });
+      if constexpr (kChain && kFetch == kRowCopies) {
+#pragma unroll
+        for (int w = 0; w < S::kHalves; ++w) {
+          store2_f32<true>(sh.params[s][0] + 64 * w, lane, 64, dt[w]);
+          store2_f32<true>(sh.params[s][1] + 64 * w, lane, 64, c[w]);
+        }
+      }
       if (lane == 0) {
         t.chunk = chunk;
         t.d = d;
@@ -240,8 +258,7 @@ recurrence_forward_kernel(const __grid_constant__ Forward p) {
       ++k;
     }
     // after a wait that ran out: no copy may be in flight when the CTA ends
-    if (kFetch == kRowCopies) wait_copies();
-    if ((kFetch != kDirect || kChain) && *static_cast<volatile int *>(&sh.broken))
+    if (kFetch != kRowCopies && (kFetch != kDirect || kChain) && *static_cast<volatile int *>(&sh.broken))
       for (int i = max(k - kStages, 0); i < k; ++i)
         mbar_wait(smem_u32(&sh.full[i % kStages]), (i / kStages) & 1);
     return;
@@ -327,8 +344,37 @@ recurrence_forward_kernel(const __grid_constant__ Forward p) {
   // ---- consumers ----
   const int slot = warp / S::kHalves, half = warp % S::kHalves;
   const int row0 = slot * kTokW;
-  unsigned char *const stage0 = smem + half * S::kHalfStage + slot * (S::kPlane / kSlots);
+  unsigned char *const stage0 = smem + half * S::kHalfStage + slot * S::kSlotStep;
   Params2 par{};
+  // kRowCopies: this warp's rows of the tile that comes into stage s next
+  bool ended = kFetch != kRowCopies;
+  Next next{};
+  auto await_next = [&](int s, uint32_t parity) {
+    if (ended) return true;
+    if (!__all_sync(0xffffffffu, wait_phase(smem_u32(&sh.posted[s]), parity, &sh.broken))) return false;
+    next = sh.next[s];
+    return true;
+  };
+  auto copy_next = [&](int s) {
+    if (ended) return;
+    ended = next.chunk < 0;
+    if (!ended) {
+      const int64_t base = next.chunk * kRows + row0, c0 = next.d * kCh + 64 * half;
+      const int rows = static_cast<int>(min(total - base, int64_t{kTokW}));
+      const int left = static_cast<int>(min(p.D - c0, int64_t{64}));
+      const uint32_t dst = smem_u32(stage0 + s * S::kStage);
+      if (left > 0) {
+        copy_rows<kElement>(dst, p.x, p.x_stride, base, rows, c0, left, lane);
+        copy_rows<kElement>(dst + S::kPlane, p.a, p.a_stride, base, rows, c0, left, lane);
+        copy_rows<kElement>(dst + 2 * S::kPlane, p.b, p.b_stride, base, rows, c0, left, lane);
+      }
+    }
+    arrive_after_copies(smem_u32(&sh.full[s]));
+  };
+  // after a wait that ran out: no copy may be in flight when the CTA ends
+  auto leave = [] {
+    if (kFetch == kRowCopies) wait_copies();
+  };
   // second pass over the tile of a stage; false if its wait ran out
   auto second_pass = [&](int s1, uint32_t parity1) {
     if (!__all_sync(0xffffffffu, wait_phase(smem_u32(&sh.ready[s1]), parity1, &sh.broken))) return false;
@@ -362,15 +408,23 @@ recurrence_forward_kernel(const __grid_constant__ Forward p) {
           store2_f32<kVec>(p.final + p.s.row(tab.end[row0 + i]) * p.D + c0, lane, left, r);
       }
     }
-    if (kFetch != kDirect) fence_async_smem();  // this stage was written here; the next copy into it comes after
+    if (kFetch == kTmaTile) fence_async_smem();  // this stage was written here; the next copy into it comes after
+    if (!await_next(s1, parity1 ^ 1)) return false;
     __syncwarp();
     if (lane == 0) mbar_arrive(smem_u32(&sh.empty[s1]));
+    copy_next(s1);
     return true;
   };
+  if (!await_next(0, 0)) return leave();
+  copy_next(0);
   int s = 0, s1 = 0, turn = 0;         // stages of this tile and the one before; whose turn to publish
   uint32_t parity = 0, parity1 = 0;    // ... and the phases of their barriers
   for (int k = 0;; ++k) {
-    if (!__all_sync(0xffffffffu, wait_phase(smem_u32(&sh.full[s]), parity, &sh.broken))) return;
+    if (k + 1 < kStages) {
+      if (!await_next(k + 1, 0)) return leave();
+      copy_next(k + 1);
+    }
+    if (!__all_sync(0xffffffffu, wait_phase(smem_u32(&sh.full[s]), parity, &sh.broken))) return leave();
     const Tile tile = sh.tiles[s];
     if (tile.d >= 0) {
       // first pass
@@ -430,7 +484,7 @@ recurrence_forward_kernel(const __grid_constant__ Forward p) {
         amax[32 * half + lane] = mine;
         __syncwarp();
         if (lane == 0) mbar_arrive(smem_u32(&sh.pair[slot]));
-        if (!__all_sync(0xffffffffu, wait_phase(smem_u32(&sh.pair[slot]), k & 1, &sh.broken))) return;
+        if (!__all_sync(0xffffffffu, wait_phase(smem_u32(&sh.pair[slot]), k & 1, &sh.broken))) return leave();
         asm volatile("" ::: "memory");
         const uint32_t ex =
             group_exponent(Raw2<E>::magnitude(max(mine, amax[32 * (half ^ 1) + lane])), exp_cap<E>());
@@ -531,7 +585,7 @@ recurrence_forward_kernel(const __grid_constant__ Forward p) {
         // so that it does not wait for the look-back of the tile before
         const bool group_end = group_len == 1 || tab.chunk % kGroupLen == kGroupLen - 1;
         if (kChain && !tab.last && (!group_end || tab.only_map)) {
-          if (!__all_sync(0xffffffffu, wait_phase(mapped, parity, &sh.broken))) return;
+          if (!__all_sync(0xffffffffu, wait_phase(mapped, parity, &sh.broken))) return leave();
           Map2 all = get_map2(&sh.own[s][half][0][0], lane);
 #pragma unroll
           for (int i = 1; i < kSlots; ++i) all = compose2(all, get_map2(&sh.own[s][half][i][0], lane));
@@ -547,9 +601,9 @@ recurrence_forward_kernel(const __grid_constant__ Forward p) {
       turn = turn + 1 == kSlots ? 0 : turn + 1;
     }
     if constexpr (S::kDefer) {
-      if (k > 0 && !second_pass(s1, parity1)) return;
+      if (k > 0 && !second_pass(s1, parity1)) return leave();
     } else {
-      if (tile.d >= 0 && !second_pass(s, parity)) return;
+      if (tile.d >= 0 && !second_pass(s, parity)) return leave();
     }
     if (tile.d < 0) return;
     s1 = s;

@@ -317,7 +317,7 @@ __device__ __forceinline__ void copy_rows(uint32_t dst, const void *base, int64_
   const int64_t step = kStep * stride * kElement;
   dst += 16 * lane;
   const int end = left * kElement - 16 * c;
-#pragma unroll 4
+#pragma unroll 1
   for (int r = r0; r < rows; r += kStep, at += step, dst += 16 * kStep * kPieces)
     if (static_cast<int>(at & 15) + end > 0)
       asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"((at & ~uintptr_t{15}) + 16 * c)
