@@ -46,6 +46,7 @@ struct Forward {
   float *final;    // rows of D, or null; may be `state`
   float *carries;  // [T / 64][D up to 128s] states before every 64th row, or null
   uint8_t *packed; // 8-bit x, a, b (kPack)
+  uint32_t skew[3][kTokW];  // kRowCopies: the byte at which row i (mod 8) of x, a, b starts in its place
   int zero_behind; // write zeros to out behind the last sequence
   Header *hdr;     // kChain
   uint64_t *maps, *states;  // kChain
@@ -82,7 +83,7 @@ struct FwdShared {
 //   producer   takes tiles by ticket, fills the table, has the inputs copied.
 //              Row copies are issued by the consumers, each warp for its own
 //              rows as soon as it is done with a stage: 66 a tile would keep one
-//              warp busy for 4000 cycles (47000 x 1021 fp16: 227 against 204 us).
+//              warp busy for 4000 cycles (47000 x 1021 fp16: 227 against 203 us).
 //   consumers  first pass: gates; per row the state y from a zero start and the
 //              product P of the gates so far, left in shared memory; the map
 //              (P, y) of the slot, and the tile's, which is published.  Second
@@ -457,8 +458,7 @@ recurrence_forward_kernel(const __grid_constant__ Forward p) {
           return r;
         } else {
           const unsigned char *src = stage + w * S::kPlane + i * S::kPitch;
-          if constexpr (kFetch == kRowCopies)
-            src += row_offset<kElement>(base, stride, tab.chunk * kRows + row0 + i, c0);
+          if constexpr (kFetch == kRowCopies) src += p.skew[w][i];
           Raw2<E> r = fetch2<E, kVec>(src, lane);
           if constexpr (kPack && kFetch == kRowCopies) {  // what lies behind the row's end is no part of its group
             const int64_t left = p.D - c0;
@@ -623,6 +623,15 @@ cudaError_t launch_forward_t(Forward p, void *workspace, int sms, cudaStream_t s
   const int64_t nt = (p.D + S::kCh - 1) / S::kCh, chunks = (max(p.s.T, int64_t{1}) - 1) / kRows + 1;
   constexpr int smem = S::kStages * S::kStage + static_cast<int>(sizeof(FwdShared<S, kPack>));
   static_assert(smem * S::kCtas <= 227 * 1024 - 1024 * (S::kCtas - 1), "CTAs of an SM share 228 KiB");
+  if constexpr (kFetch == kRowCopies) {
+    static_assert(kTokW * sizeof(E) % 16 == 0 && 64 * sizeof(E) % 16 == 0, "the same for all slots and tiles");
+    const void *const base[3] = {p.x, p.a, p.b};
+    const int64_t stride[3] = {p.x_stride, p.a_stride, p.b_stride};
+    for (int w = 0; w < 3; ++w)
+      for (int i = 0; i < kTokW; ++i)
+        p.skew[w][i] = static_cast<uint32_t>(
+            (reinterpret_cast<uintptr_t>(base[w]) + static_cast<uintptr_t>(i * stride[w]) * sizeof(E)) & 15);
+  }
   if constexpr (kFetch == kTmaTile) {
     if (!make_row_map<E>(&p.tx, p.x, p.D, p.s.T, p.x_stride, 64, kRows) ||
         !make_row_map<E>(&p.ta, p.a, p.D, p.s.T, p.a_stride, 64, kRows) ||
