@@ -6,7 +6,8 @@
 // writes a byte a value and a byte a group: 3 bytes a value each way for 2-byte
 // types, bound by HBM.  Where a tensor's groups follow one another in memory
 // (full groups, rows without gaps) a group's place is its number; elsewhere it
-// takes two 32-bit divisions a group.
+// takes two 32-bit divisions a group.  134 M bf16 values: 60 us each way at 6.7
+// TB/s, as fast as a copy.
 #include "gdn_recurrence.cuh"
 
 namespace gdn {

@@ -13,6 +13,10 @@
 // and beta stay in shared memory.  Second pass, when the chain warp has what
 // enters: half a slot (4 rows) at a time, first upwards for the states, then
 // downwards for the gradients.
+//
+// What bounds it: instructions (66 of a warp for 32 values, 2.2 a cycle of 4).
+// 8 x 4096 x 2048 bf16 takes 216 us (4.3 TB/s; 144 us at the rate of a copy),
+// from 8-bit x, a, b 252 us: converting bytes costs more than they save to read.
 #include "gdn_recurrence_tile.cuh"
 
 namespace gdn {

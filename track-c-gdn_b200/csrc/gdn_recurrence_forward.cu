@@ -27,9 +27,9 @@ struct FwdShape {
   static constexpr int kHalfStage = kSlots * (kRead > kLeft ? kRead : kLeft);
   static constexpr int kStage = kHalves * kHalfStage;
   static constexpr int kStages = kHalfStage > 32768 ? 2 : 3;
-  // The second pass is put off by a tile where there is a stage for it (47000 x
-  // 1021 fp16: 254 against 221 us), and with tensor copies even with two stages:
-  // 65536 x 1024 fp32 266 against 315 us.
+  // The second pass is put off by a tile (8 x 4096 x 2048 bf16: 136 -> 120 us),
+  // also where tensor copies have two stages only (65536 x 1024 fp32: 279 -> 209
+  // us), but not with two stages of row copies, which wait for a stage longer.
   static constexpr bool kDefer = kStages > 2 || kFetch == kTmaTile;
   static constexpr int kCtas = kPack || kStages * kStage > 98304 ? 1 : 2;             // of an SM
 };
@@ -90,11 +90,18 @@ struct FwdShared {
 //              pass, one tile later (kDefer): out = y + P h, with h the state
 //              that enters the slot.
 //   chain      (one per half) looks back and hands each slot its state.  It has
-//              the time of a first pass for that.  (Two per half, for tiles in
-//              turn, leave 80 instead of 96 registers a thread: 65536 x 1024
-//              fp32 274 instead of 218 us, elsewhere the same.)
+//              the time of a first pass for that.
 // Without kChain (short inputs, one launch) a CTA walks all chunks of its
 // channels and the chain warp keeps the state.
+//
+// What bounds it: instructions, not memory.  8 x 4096 x 2048 bf16 takes 120 us
+// (4.5 TB/s; 82 us at the rate of a copy): 37 warp instructions for 32 values,
+// 2.2 a cycle of 4, the exponentials' pipe half busy.  256 sequences, 1.15 M x
+// 1024 bf16: 1.89 ms, 5.0 TB/s.  One sequence of 65536 x 1024: 171 us in bf16,
+// bound by the chain's links, 209 us in fp32 (5.1 TB/s).  With 8-bit copies 190
+// us for 8 x 4096 x 2048 (3.9 TB/s), bound by integer work on groups and bytes.
+// Rows that no tensor copy fits, 47000 x 1021 fp16: 187 us, 2.1 TB/s, bound by
+// instructions (two 16-bit accesses for each pair of values, copies by address).
 template <typename E, Fetch kFetch, bool kPack, bool kChain>
 __global__ void __launch_bounds__(FwdShape<E, kFetch, kPack>::kThreads, FwdShape<E, kFetch, kPack>::kCtas)
 recurrence_forward_kernel(const __grid_constant__ Forward p) {

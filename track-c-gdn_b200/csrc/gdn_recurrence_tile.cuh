@@ -14,10 +14,10 @@ namespace rec {
 
 // Chunks joined through one published state: 8 where one sequence (or a few) has
 // to be worked on by all CTAs at once -- a state then travels one link of about
-// 0.75 us for 8 chunks (65536 x 1024 bf16: 185 us; groups of 4: 214, 16: 212,
-// 2: 380) -- and 1 where streams and tiles of channels together give most CTAs a
-// tile of a chunk whose predecessor is done: then a state per chunk is all that
-// is published.
+// 0.75 us for 8 chunks (65536 x 1024 bf16: 171 us; groups of 4: 218, of 16: 317,
+// with more maps to fetch and apply for each tile) -- and 1 where streams and
+// tiles of channels together give most CTAs a tile of a chunk whose predecessor
+// is done: then a state per chunk is all that is published.
 constexpr int kGroupLen = 8;
 
 constexpr int kTokW = 8;
@@ -112,7 +112,8 @@ __device__ __forceinline__ int64_t first_by_halves(const Seqs &s, int64_t v) {
   return lo;
 }
 
-// What the init kernel prepares besides: the parameters of all channels (zeros up to a multiple of 128), and the first sequence that starts
+// What the init kernel prepares besides: the parameters of all channels (zeros up
+// to a multiple of 128), and the first sequence that starts
 // at or behind each chunk's first row.
 struct Prepared {
   const float *A_log, *dt_bias;
