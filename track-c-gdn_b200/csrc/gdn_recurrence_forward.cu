@@ -100,7 +100,7 @@ struct FwdShared {
 // 1024 bf16: 1.89 ms, 5.0 TB/s.  One sequence of 65536 x 1024: 171 us in bf16,
 // bound by the chain's links, 209 us in fp32 (5.1 TB/s).  With 8-bit copies 190
 // us for 8 x 4096 x 2048 (3.9 TB/s), bound by integer work on groups and bytes.
-// Rows that no tensor copy fits, 47000 x 1021 fp16: 187 us, 2.1 TB/s, bound by
+// Rows that no tensor copy fits, 47000 x 1021 fp16: 191 us, 2.0 TB/s, bound by
 // instructions (two 16-bit accesses for each pair of values, copies by address).
 template <typename E, Fetch kFetch, bool kPack, bool kChain>
 __global__ void __launch_bounds__(FwdShape<E, kFetch, kPack>::kThreads, FwdShape<E, kFetch, kPack>::kCtas)
@@ -192,11 +192,17 @@ recurrence_forward_kernel(const __grid_constant__ Forward p) {
       }
       if (chunk > last) continue;
       const int s = k % kStages;
-      if (kFetch == kRowCopies && lane == 0) {
-        // read by all consumers before they leave the stage's last tile, which
-        // the wait below saw for the entry that this one replaces
-        sh.next[s] = Next{chunk, d};
-        mbar_arrive(smem_u32(&sh.posted[s]));
+      if constexpr (kFetch == kRowCopies) {
+        // Consumers read an entry before they leave the stage's tile before it, so
+        // the wait for `empty` below has covered the entry that this one replaces
+        // -- but for a stage's first entry, which has been read when its copies
+        // are there.
+        const bool read = k < kStages || k >= 2 * kStages || wait_phase(smem_u32(&sh.full[s]), 0, &sh.broken);
+        if (!__all_sync(0xffffffffu, read)) break;
+        if (lane == 0) {
+          sh.next[s] = Next{chunk, d};
+          mbar_arrive(smem_u32(&sh.posted[s]));
+        }
       }
       const bool go = k < kStages || wait_phase(smem_u32(&sh.empty[s]), ((k / kStages) - 1) & 1, &sh.broken);
       if (!__all_sync(0xffffffffu, go)) break;
