@@ -283,7 +283,7 @@ int gdn_prefill_backward_qk4_v8_d128_k_last(
  *           GDN_FP16 or GDN_FP32; everything is computed and carried in fp32
  *           and a result is rounded once, when it is stored
  * x, a, b   [T, D], a token's channels contiguous, `*_stride` elements from one
- *           token to the next (so they may be parts of one projection's output)
+ *           token to the next, not negative (parts of one projection's output)
  * A_log, dt_bias [D] fp32
  * Pointers need the alignment of their elements; the kernels are fastest where
  * rows and pointers of the inputs are multiples of 16 bytes.  1 <= D <= 2^24,
@@ -349,7 +349,8 @@ int gdn_recurrence_backward(int type, const void *x, int64_t x_stride, const voi
                             const void *b, int64_t b_stride, const void *packed, const float *A_log,
                             const float *dt_bias, const float *state, const int64_t *cu_seqlens,
                             int64_t num_seqs, int64_t total_tokens, int64_t channels, int zero_behind,
-                            const void *d_out, int64_t d_out_stride, const float *d_final_state, const float *carries, void *dx,
+                            const void *d_out, int64_t d_out_stride, const float *d_final_state,
+                            const float *carries, void *dx,
                             void *da, void *db, float *dA_log, float *ddt_bias, float *d_state,
                             void *workspace, size_t workspace_bytes, void *stream);
 

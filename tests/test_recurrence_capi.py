@@ -44,6 +44,22 @@ def test_prefill_arguments(gdn):
         assert prefill(lib, out=out) == 7
 
 
+def test_negative_strides(gdn):
+    lib = gdn._native.lib
+    assert prefill(lib, xs=-64) == 2
+    for i in (2, 4, 6):
+        args = [BF16, OK, 64, OK, 64, OK, 64, OK, OK]
+        args[i] = -1
+        assert lib.gdn_recurrence_prefill(*args, None, None, 0, OK, 2, 100, 64, 0, far(5), far(9), None, None, far(20),
+                                          BIG, None) == 2
+        assert lib.gdn_recurrence_decode(*args, None, None, 0, 4, 1, 64, OK, far(3), None, None) == 2
+        args[7:7] = [None]
+        assert lib.gdn_recurrence_backward(*args, None, OK, 2, 100, 64, 0, OK, 64, None, None, far(5), far(6), far(7),
+                                           OK, OK, None, far(20), BIG, None) == 2
+    assert lib.gdn_recurrence_backward(BF16, OK, 64, OK, 64, OK, 64, None, OK, OK, None, OK, 2, 100, 64, 0, OK, -64,
+                                       None, None, far(5), far(6), far(7), OK, OK, None, far(20), BIG, None) == 2
+
+
 def backward(lib, type=BF16, x=OK, a=OK, b=OK, packed=None, state=None, cu=OK, N=2, T=100, D=64, d_out=OK,
              d_final=None, carries=None, dx=far(5), da=far(6), db=far(7), dA=OK, ddt=OK, d_state=None, ws=far(20), ws_bytes=BIG):
     return lib.gdn_recurrence_backward(type, x, 64, a, 64, b, 64, packed, OK, OK, state, cu, N, T, D, 0, d_out, 64,

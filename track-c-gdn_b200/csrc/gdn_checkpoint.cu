@@ -37,7 +37,10 @@ struct Place {
   int left;  // values of the row from there on
 };
 __device__ __forceinline__ Place place_of(const PackTensor &t, uint32_t item, bool unpack) {
-  if (t.flat) return Place{static_cast<int64_t>(item) * kGroupValues, static_cast<int64_t>(item) * kGroupValues, kGroupValues};
+  if (t.flat) {
+    const int64_t at = static_cast<int64_t>(item) * kGroupValues;
+    return Place{at, at, kGroupValues};
+  }
   const uint32_t row = item / t.groups, c0 = (item - row * t.groups) * kGroupValues;
   const int64_t values = row * t.cols + c0;
   const uint32_t outer = row / t.inner;

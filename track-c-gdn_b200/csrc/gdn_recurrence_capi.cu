@@ -96,6 +96,7 @@ int gdn_recurrence_prefill(int type, const void *x, int64_t x_stride, const void
                            int64_t channels, int zero_behind, void *out, float *final_state, float *carries,
                            void *packed, void *workspace, size_t workspace_bytes, void *stream) {
   if (!good_sizes(type, total_tokens, num_seqs, channels) || (slots && pool_slots < 1)) return GDN_ERR_BAD_SIZE;
+  if (x_stride < 0 || a_stride < 0 || b_stride < 0) return GDN_ERR_BAD_SIZE;
   if (num_seqs == 0) return total_tokens == 0 ? GDN_OK : GDN_ERR_BAD_SIZE;
   if (!cu_seqlens && total_tokens % num_seqs != 0) return GDN_ERR_BAD_SIZE;
   if (!A_log || !dt_bias || !final_state || !workspace) return GDN_ERR_NULL_POINTER;
@@ -131,10 +132,11 @@ int gdn_recurrence_backward(int type, const void *x, int64_t x_stride, const voi
                             const void *b, int64_t b_stride, const void *packed, const float *A_log,
                             const float *dt_bias, const float *state, const int64_t *cu_seqlens,
                             int64_t num_seqs, int64_t total_tokens, int64_t channels, int zero_behind,
-                            const void *d_out, int64_t d_out_stride, const float *d_final_state, const float *carries, void *dx,
-                            void *da, void *db, float *dA_log, float *ddt_bias, float *d_state,
+                            const void *d_out, int64_t d_out_stride, const float *d_final_state,
+                            const float *carries, void *dx, void *da, void *db, float *dA_log, float *ddt_bias, float *d_state,
                             void *workspace, size_t workspace_bytes, void *stream) {
   if (!good_sizes(type, total_tokens, num_seqs, channels)) return GDN_ERR_BAD_SIZE;
+  if (x_stride < 0 || a_stride < 0 || b_stride < 0 || d_out_stride < 0) return GDN_ERR_BAD_SIZE;
   if (num_seqs == 0 && total_tokens != 0) return GDN_ERR_BAD_SIZE;
   if (!cu_seqlens && num_seqs > 0 && total_tokens % num_seqs != 0) return GDN_ERR_BAD_SIZE;
   if (!A_log || !dt_bias || !dA_log || !ddt_bias || !workspace) return GDN_ERR_NULL_POINTER;
@@ -209,7 +211,8 @@ int gdn_recurrence_decode(int type, const void *x, int64_t x_stride, const void 
                           float *intermediate_states, void *stream) {
   if (!known_type(type) || batch < 0 || batch > kMaxSeqs || num_tokens < 1 ||
       num_tokens > GDN_DECODE_MTP_MAX_TOKENS || channels < 1 || channels > (int64_t{1} << 24) ||
-      batch * tiles_of(channels) > INT32_MAX || (slots && pool_slots < 1))
+      batch * tiles_of(channels) > INT32_MAX || (slots && pool_slots < 1) || x_stride < 0 || a_stride < 0 ||
+      b_stride < 0)
     return GDN_ERR_BAD_SIZE;
   if (batch == 0) return GDN_OK;
   if (!x || !a || !b || !A_log || !dt_bias || !out || !new_state || (slots && !state))
