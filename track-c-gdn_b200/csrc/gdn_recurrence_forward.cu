@@ -262,7 +262,7 @@ recurrence_forward_kernel(const __grid_constant__ Forward p) {
         t.d = d;
         t.last = chunk == last;
         t.only_map = only_map;
-        t.cut = kChain && p.aside != nullptr && !only_map && chunk == st.to - 1 ? st.cut : -1;
+        t.cut = !kChain || p.aside == nullptr ? -1 : only_map ? st.opens : chunk == st.to - 1 ? st.cut : -1;
         t.valid = min(total - base, int64_t{kRows});
         const bool plain = inside && !only_map && base + kRows <= total && c0 + kCh <= p.D && p.out != nullptr;
         sh.tiles[s] = Tile{base * p.D + c0, d, plain ? 1 : 0};
@@ -579,6 +579,9 @@ recurrence_forward_kernel(const __grid_constant__ Forward p) {
             const int row = row0 + i;
             // of a cut chunk the last sequence's was set aside if it goes on
             const bool goes_on = tab.cut >= 0 && !last_bits(tab.starts, row + 1) && !last_bits(tab.ends, row);
+#ifdef GDN_DEBUG_CHECKS
+            if (tab.only_map && !last_bits(tab.starts, row + 1)) delay(kMapOnlyDelayCycles);
+#endif
             y = p.state == nullptr ? 0
                 : goes_on          ? load2_f32<kVec>(p.aside + tab.cut * ((p.D + 127) / 128 * 128) + c0, lane, left)
                                    : load2_f32<kVec>(p.state + p.s.row(tab.start[row]) * p.D + c0, lane, left);

@@ -34,7 +34,7 @@ struct Table {
   int d;
   int last;       // the last chunk
   int only_map;   // nothing but the tile's map is wanted
-  int cut;        // the cut that goes through the chunk, or -1
+  int cut;        // the cut that goes through the chunk where states are updated in place, or -1
   uint32_t starts[kRows / 32], ends[kRows / 32];
   int start[kRows], end[kRows];  // the sequence, or -1
 };
@@ -62,14 +62,17 @@ struct Seqs {
 // in the chain has usually long been finished when its turn comes; one sequence
 // alone is one stream.  The cut may go through a chunk: that chunk belongs to
 // the stream that ends with it, but its map is needed by the other from the
-// start, and is worked out there once more (only_map).
+// start, and is worked out there once more (only_map).  Both publish the map in
+// the same word, and neither waits for the other: they have to find the same
+// bits whenever they run, so what they read must not change during the call
+// (Prepared::aside).
 constexpr int kStreams = 32;
 struct Stream {
   int64_t from, to;  // chunks [from, to)
   uint32_t ticket;
   int only_map;      // 1: starts with the map of chunk from - 1 (backwards: to)
   int cut;           // forwards: the cut that goes through chunk to - 1, or -1
-  int pad;
+  int opens;         // forwards with only_map: the cut that goes through chunk from - 1
 };
 struct Header {
   uint32_t bad;      // cu_seqlens or slots are not valid: write nothing
@@ -80,6 +83,17 @@ struct Header {
 };
 static_assert(sizeof(Header) <= 2048, "what follows starts 2048 bytes into the workspace");
 constexpr size_t kHeaderBytes = 2048;
+
+#ifdef GDN_DEBUG_CHECKS
+// The debug build holds a map-only tile back (about 0.5 ms) before it reads the
+// state that the last sequence of its chunk starts from: the others have by then
+// usually finished that sequence, and a read of what they write shows.
+constexpr long long kMapOnlyDelayCycles = 1ll << 20;
+__device__ __forceinline__ void delay(long long cycles) {
+  for (const long long t0 = clock64(); clock64() - t0 < cycles;) {
+  }
+}
+#endif
 
 // Checks cu_seqlens and slots with all threads of a CTA; returns the device
 // status code of what is wrong, or 0.
@@ -126,8 +140,9 @@ struct Prepared {
   bool backwards;   // the chain runs from the last chunk to the first
   // States that the call updates in place (else null): a sequence that starts
   // in a cut chunk and goes on behind it is finished by the stream that begins
-  // there, perhaps before the stream before has come to the chunk and read where
-  // it starts from.  That state is set aside, one row for each cut.
+  // there, perhaps before the stream before, or this one's own map of the chunk,
+  // has read where it starts from.  That state is set aside, one row for each
+  // cut, and both take it from there.
   const float *state;
   float *aside;     // [kStreams][D up to 128s]
 };
@@ -187,14 +202,14 @@ __global__ void __launch_bounds__(1024) recurrence_init_kernel(Header *hdr, ulon
     if (i == 0) {
       int n = 1;
       int64_t prev = 0;
-      hdr->stream[0] = Stream{0, q.chunks, 0, 0, -1, 0};
+      hdr->stream[0] = Stream{0, q.chunks, 0, 0, -1, -1};
       for (int j = 1; j < q.streams; ++j)
         if (from[j] > prev && from[j] < q.chunks) {
           prev = from[j];
           hdr->stream[n - 1].to = from[j];
           if (q.backwards) hdr->stream[n - 1].only_map = only_map[j];
           if (!q.backwards && only_map[j]) hdr->stream[n - 1].cut = j;
-          hdr->stream[n] = Stream{from[j], q.chunks, 0, q.backwards ? 0 : only_map[j], -1, 0};
+          hdr->stream[n] = Stream{from[j], q.chunks, 0, q.backwards ? 0 : only_map[j], -1, j};
           ++n;
         }
       hdr->streams = n;
