@@ -104,6 +104,17 @@ def check(status: int, what: str) -> None:
         raise GdnError(f"{what} failed: status {status} ({msg})")
 
 
+def aligned_workspace(ws, device):
+    """(address, bytes) of a caller's workspace tensor from its first 1024-byte
+    boundary on; 0 bytes where the tensor ends before that."""
+    if ws.device != device:
+        raise ValueError(f"the workspace is on {ws.device}, the inputs on {device}")
+    assert ws.is_contiguous(), "the workspace must be contiguous"
+    p = ws.data_ptr()
+    off = -p % 1024
+    return p + off, max(0, ws.numel() * ws.element_size() - off)
+
+
 def prefill_kernel_launches(total_tokens: int, num_seqs: int) -> int:
     """Kernels one prefill call launches for this problem size (3, or 5 when
     it runs the segmented evaluation)."""

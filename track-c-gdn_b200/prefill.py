@@ -61,15 +61,9 @@ def workspace_bytes(total_tokens: int, num_seqs: int) -> int:
 def alloc_workspace(total_tokens: int, num_seqs: int, device) -> torch.Tensor:
     """A workspace buffer for `prefill_into` (1024-byte aligned: the caching
     allocator returns 512-byte aligned blocks, so 1 KiB of slack is added and
-    `workspace_view` picks the aligned start)."""
+    the calls pick the aligned start)."""
     return torch.empty(workspace_bytes(total_tokens, num_seqs) + 1024, dtype=torch.uint8,
                        device=device)
-
-
-def _aligned_ptr(ws: torch.Tensor):
-    p = ws.data_ptr()
-    off = (-p) % 1024
-    return p + off, ws.numel() - off
 
 
 def prefill_into(q, k, v, state, A_log, a, dt_bias, b, cu_seqlens, scale, out, final_state,
@@ -87,7 +81,7 @@ def prefill_into(q, k, v, state, A_log, a, dt_bias, b, cu_seqlens, scale, out, f
         scale = 1.0 / math.sqrt(HEAD_SIZE)
     if stream is None:
         stream = torch.cuda.current_stream(q.device).cuda_stream
-    wptr, wbytes = _aligned_ptr(workspace)
+    wptr, wbytes = _native.aligned_workspace(workspace, q.device)
     args = (q.data_ptr(), k.data_ptr(), v.data_ptr(), None if state is None else state.data_ptr(),
             A_log.data_ptr(), a.data_ptr(), dt_bias.data_ptr(), b.data_ptr(),
             cu_seqlens.data_ptr(), N, T, float(scale), out.data_ptr(), final_state.data_ptr(),
@@ -135,7 +129,7 @@ def prefill_pool_into(q, k, v, state_pool, slots, A_log, a, dt_bias, b, cu_seqle
         scale = 1.0 / math.sqrt(HEAD_SIZE)
     if stream is None:
         stream = torch.cuda.current_stream(q.device).cuda_stream
-    wptr, wbytes = _aligned_ptr(workspace)
+    wptr, wbytes = _native.aligned_workspace(workspace, q.device)
     st = _native.lib.gdn_prefill_pool_qk4_v8_d128_k_last(
         q.data_ptr(), k.data_ptr(), v.data_ptr(), state_pool.data_ptr(), state_pool.shape[0],
         slots.data_ptr(), A_log.data_ptr(), a.data_ptr(), dt_bias.data_ptr(), b.data_ptr(),
@@ -191,7 +185,7 @@ def backward_into(q, k, v, state, A_log, a, dt_bias, b, cu_seqlens, scale, d_out
         scale = 1.0 / math.sqrt(HEAD_SIZE)
     if stream is None:
         stream = torch.cuda.current_stream(q.device).cuda_stream
-    wptr, wbytes = _aligned_ptr(workspace)
+    wptr, wbytes = _native.aligned_workspace(workspace, q.device)
 
     def p(x):
         return None if x is None else x.data_ptr()

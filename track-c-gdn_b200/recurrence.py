@@ -136,12 +136,6 @@ def _ptr(t: Optional[torch.Tensor]):
     return None if t is None else t.data_ptr()
 
 
-def _aligned(ws: torch.Tensor):
-    p = ws.data_ptr()
-    off = -p % 1024
-    return p + off, ws.numel() - off
-
-
 # ---------------------------------------------------------------------------
 # decode
 # ---------------------------------------------------------------------------
@@ -246,11 +240,11 @@ def _prefill(x, state, A_log, a, dt_bias, b, cu_seqlens, out, final_state, works
 def _launch_prefill(x, state, A_log, a, dt_bias, b, seqs, out, final_state, workspace, slots, carries, packed,
                     zero_behind, stream):
     T, N, cu = seqs
+    wptr, wbytes = _native.aligned_workspace(workspace, x.device)
     x, xs = _rows(x, stream)
     a, as_ = _rows(a, stream)
     b, bs = _rows(b, stream)
     A_log, dt_bias = _vector(A_log, stream), _vector(dt_bias, stream)
-    wptr, wbytes = _aligned(workspace)
     _call(_native.lib.gdn_recurrence_prefill, x.device,
           (_TYPES[x.dtype], x.data_ptr(), xs, a.data_ptr(), as_, b.data_ptr(), bs, A_log.data_ptr(),
            dt_bias.data_ptr(), _ptr(state), _ptr(slots), 0 if slots is None else state.shape[0], cu, N, T,
@@ -333,6 +327,7 @@ def _backward(x, state, A_log, a, dt_bias, b, cu_seqlens, d_out, d_final_state, 
 def _launch_backward(x, state, A_log, a, dt_bias, b, seqs, d_out, d_final_state, grads, workspace, carries, packed,
                      zero_behind, stream):
     T, N, cu = seqs
+    wptr, wbytes = _native.aligned_workspace(workspace, d_out.device)
     xs = as_ = bs = 0
     if packed is None:
         x, xs = _rows(x, stream)
@@ -340,7 +335,6 @@ def _launch_backward(x, state, A_log, a, dt_bias, b, seqs, d_out, d_final_state,
         b, bs = _rows(b, stream)
     d_out, ds = _rows(d_out, stream)
     A_log, dt_bias = _vector(A_log, stream), _vector(dt_bias, stream)
-    wptr, wbytes = _aligned(workspace)
     dx, da, db, dA_log, ddt_bias, d_state = grads
     _call(_native.lib.gdn_recurrence_backward, d_out.device,
           (_TYPES[d_out.dtype], _ptr(x), xs, _ptr(a), as_, _ptr(b), bs, _ptr(packed), A_log.data_ptr(),
