@@ -240,22 +240,21 @@ class _PrefillFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, state, A_log, a, dt_bias, b, cu_seqlens, scale, checkpoint):
         out, final_state = run(q, k, v, state, A_log, a, dt_bias, b, cu_seqlens, scale)
-        if checkpoint is None:
-            ctx.packed = None
-            ctx.save_for_backward(q, k, v, state, A_log, a, dt_bias, b, cu_seqlens)
-        else:
-            ctx.packed = _checkpoint.pack(q, k, v)
-            ctx.save_for_backward(state, A_log, a, dt_bias, b, cu_seqlens)
+        ctx.packed = None
+        if checkpoint is not None:
+            # what the bytes mean; they themselves are saved as q is
+            p = _checkpoint.pack(q, k, v)
+            ctx.packed = (p.dtype, p.shapes, p.places)
+            q, k, v = p.buffer, None, None
+        ctx.save_for_backward(q, k, v, state, A_log, a, dt_bias, b, cu_seqlens)
         ctx.scale = scale
         return out, final_state
 
     @staticmethod
     def backward(ctx, d_out, d_final):
-        if ctx.packed is None:
-            q, k, v, state, A_log, a, dt_bias, b, cu_seqlens = ctx.saved_tensors
-        else:
-            state, A_log, a, dt_bias, b, cu_seqlens = ctx.saved_tensors
-            q, k, v = _checkpoint.unpack(ctx.packed)
+        q, k, v, state, A_log, a, dt_bias, b, cu_seqlens = ctx.saved_tensors
+        if ctx.packed is not None:
+            q, k, v = _checkpoint.unpack(_checkpoint.Packed(q, *ctx.packed))
         if d_out is None:
             d_out = torch.zeros(q.shape[0], NUM_V_HEADS, HEAD_SIZE, dtype=torch.bfloat16,
                                 device=q.device)
