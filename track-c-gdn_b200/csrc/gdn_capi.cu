@@ -12,6 +12,7 @@
 
 #include "../../include/gdn_b200.h"
 #include "gdn_common.cuh"
+#include "gdn_context.cuh"
 
 namespace gdn {
 cudaError_t launch_decode(const void *q, const void *k, const void *v, const float *state,
@@ -60,12 +61,15 @@ bool overlap(const void *a, size_t na, const void *b, size_t nb) {
 }
 
 // Current device must be sm_100 (B200 family); cached per device ordinal.  Makes
-// its context current for the calling thread: a thread that has not used CUDA
-// yet (autograd's, for one) has none, and tensor maps cannot be encoded then.
+// its primary context current for a calling thread that has none: a thread that
+// has not used CUDA yet (autograd's, for one), where tensor maps cannot be
+// encoded.  A caller's own context stays current: its streams and memory are
+// valid there alone.
 int check_device(int *num_sms) {
   static int cached_dev = -1, cached_ok = 0, cached_sms = 0;
   int dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess || cudaSetDevice(dev) != cudaSuccess) return GDN_ERR_DEVICE;
+  if (cudaGetDevice(&dev) != cudaSuccess) return GDN_ERR_DEVICE;
+  if (gdn::current_context() == nullptr && cudaSetDevice(dev) != cudaSuccess) return GDN_ERR_DEVICE;
   if (dev != cached_dev) {
     cudaDeviceProp prop;
     if (cudaGetDeviceProperties(&prop, dev) != cudaSuccess) return GDN_ERR_DEVICE;
