@@ -103,6 +103,43 @@ def decode_in_own_context(gdn):
     assert d.current() == d.ctx.value
 
 
+def recurrence_after_the_primary_context(gdn):
+    """Forward and backward first through torch, then in a context of the
+    caller's own, then in another: kernels with much shared memory have to be
+    allowed it in each."""
+    import numpy as np
+    import torch
+
+    T, D = 1000, 64
+    host = rows(T, D, 2)
+    x, a, b, A_log, dt_bias = (torch.from_numpy(t).cuda() for t in host)
+    want, want_final = gdn.recurrence.run(x, None, A_log, a, dt_bias, b)
+    grads = gdn.recurrence.backward(x, None, A_log, a, dt_bias, b, None, x)
+    want, want_final = want.cpu().numpy(), want_final.cpu().numpy()
+    grads = {k: v.cpu().numpy() for k, v in grads.items() if v is not None}
+    lib = gdn._native.lib
+    need, bneed = lib.gdn_recurrence_workspace_bytes(T, D), lib.gdn_recurrence_backward_workspace_bytes(T, D)
+    for _ in range(2):
+        d = start(gdn)
+        dx, da, db, dA, ddt = (d.put(t) for t in host)
+        out, final = d.alloc(want.nbytes), d.alloc(want_final.nbytes)
+        ws, bws = (P(-(-d.alloc(n + 1024).value // 1024) * 1024) for n in (need, bneed))
+        assert lib.gdn_recurrence_prefill(2, dx, D, da, D, db, D, dA, ddt, None, None, 0, None, 1, T, D, 0, out, final,
+                                          None, None, ws, need, None) == 0
+        assert np.array_equal(d.get(out, want), want) and np.array_equal(d.get(final, want_final), want_final)
+        g = {k: d.alloc(v.nbytes) for k, v in grads.items()}
+        assert lib.gdn_recurrence_backward(2, dx, D, da, D, db, D, None, dA, ddt, None, None, 1, T, D, 0, dx, D, None,
+                                           None, g["dx"], g["da"], g["db"], g["dA_log"], g["ddt_bias"], g["d_state"], bws,
+                                           bneed, None) == 0
+        for k, v in grads.items():
+            assert np.array_equal(d.get(g[k], v), v), k
+        assert d.current() == d.ctx.value
+        d.ok("cuCtxDestroy_v2", d.ctx)
+    # torch's context is the one below: back to it
+    again, _ = gdn.recurrence.run(x, None, A_log, a, dt_bias, b)
+    assert np.array_equal(again.cpu().numpy(), want)
+
+
 def run_part(name):
     res = subprocess.run([sys.executable, __file__, name], cwd=ROOT, capture_output=True, text=True, timeout=300)
     assert res.returncode == 0, res.stdout[-2000:] + res.stderr[-3000:]
@@ -115,6 +152,10 @@ def test_first_call_leaves_the_context_current():
 
 def test_decode_in_own_context():
     run_part("decode_in_own_context")
+
+
+def test_recurrence_after_the_primary_context():
+    run_part("recurrence_after_the_primary_context")
 
 
 if __name__ == "__main__":

@@ -24,4 +24,12 @@ inline CUcontext current_context() {
   return get != nullptr && get(&ctx) == CUDA_SUCCESS ? ctx : nullptr;
 }
 
+// A number that no other context of the process has or had; 0 for none.
+inline unsigned long long current_context_id() {
+  static const auto get = driver_function<CUresult (*)(CUcontext, unsigned long long *)>("cuCtxGetId");
+  unsigned long long id = 0;
+  const CUcontext ctx = current_context();
+  return ctx != nullptr && get != nullptr && get(ctx, &id) == CUDA_SUCCESS ? id : 0;
+}
+
 }  // namespace gdn

@@ -549,7 +549,7 @@ cudaError_t launch_backward_t(Backward p, void *workspace, int sms, float *dA_lo
     if (!ok) return cudaErrorInvalidValue;
   }
   auto kernel = recurrence_backward_kernel<E, kFetch, kPacked>;
-  static std::atomic<uint64_t> allowed;
+  static std::atomic<unsigned long long> allowed;
   if (cudaError_t e = allow_shared(kernel, smem, allowed)) return e;
   const Places w = places(workspace, p.s.T, p.D);
   p.hdr = static_cast<Header *>(workspace);

@@ -660,7 +660,7 @@ cudaError_t launch_forward_t(Forward p, void *workspace, int sms, cudaStream_t s
   const bool serial = chunks <= kSerialChunks && (p.s.cu == nullptr || p.s.N <= kSerialSeqs);
   auto kernel = serial ? recurrence_forward_kernel<E, kFetch, kPack, false>
                        : recurrence_forward_kernel<E, kFetch, kPack, true>;
-  static std::atomic<uint64_t> allowed[2];
+  static std::atomic<unsigned long long> allowed[2];
   if (cudaError_t e = allow_shared(kernel, smem, allowed[serial])) return e;
   int64_t blocks = nt;
   if (!serial) {

@@ -7,6 +7,7 @@
 #include <atomic>
 #include <type_traits>
 
+#include "gdn_context.cuh"
 #include "gdn_recurrence.cuh"
 
 namespace gdn {
@@ -580,15 +581,14 @@ __device__ __forceinline__ void mbar_arrive(uint32_t mbar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(mbar) : "memory");
 }
 
-// Allows a kernel its dynamic shared memory, once per device.
+// Allows a kernel its dynamic shared memory.  That holds in the context it was
+// asked for in: `last` is the one of the last call, which need not ask again.
 template <typename K>
-cudaError_t allow_shared(K kernel, int bytes, std::atomic<uint64_t> &done) {
-  int dev = 0;
-  if (cudaError_t e = cudaGetDevice(&dev)) return e;
-  const uint64_t bit = dev < 64 ? uint64_t{1} << dev : 0;
-  if (bit && (done.load(std::memory_order_acquire) & bit)) return cudaSuccess;
+cudaError_t allow_shared(K kernel, int bytes, std::atomic<unsigned long long> &last) {
+  const unsigned long long id = current_context_id();
+  if (id != 0 && last.load(std::memory_order_acquire) == id) return cudaSuccess;
   if (cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes)) return e;
-  done.fetch_or(bit, std::memory_order_release);
+  last.store(id, std::memory_order_release);
   return cudaSuccess;
 }
 
