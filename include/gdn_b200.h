@@ -360,6 +360,8 @@ int gdn_recurrence_backward(int type, const void *x, int64_t x_stride, const voi
  * for zeros, or with `slots` a pool as above (a request whose slot is outside
  * the pool is skipped, device status 3); new_state may be `state`;
  * intermediate_states NULL or [B,num_tokens,D] fp32, the state after each token.
+ * out may be x, a or b itself (the same rows, D apart); apart from that no
+ * output shares memory with x, a, b, a state or another output.
  */
 int gdn_recurrence_decode(int type, const void *x, int64_t x_stride, const void *a, int64_t a_stride,
                           const void *b, int64_t b_stride, const float *A_log, const float *dt_bias,

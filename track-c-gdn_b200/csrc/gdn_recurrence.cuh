@@ -56,13 +56,16 @@ struct Raw<float> {
 // lane, lane + 32, lane + 64, lane + 96 of the tile, so that single-element
 // accesses of a warp still fall next to one another.
 // left: channels of the tile that exist (D - first channel; may exceed 128).
-template <typename E, bool kVec>
+// kReadOnly: nothing writes to the data while the kernel runs.
+template <typename E, bool kVec, bool kReadOnly = true>
 __device__ __forceinline__ Raw<E> load4(const E *p, int lane, int left) {
   Raw<E> r;
   if constexpr (kVec) {
     r.v = {};
-    if (4 * lane < left)
-      r.v = __ldg(reinterpret_cast<const decltype(r.v) *>(p) + lane);
+    if (4 * lane < left) {
+      const auto *q = reinterpret_cast<const decltype(r.v) *>(p) + lane;
+      r.v = kReadOnly ? __ldg(q) : *q;
+    }
   } else {
     E e[4];
 #pragma unroll

@@ -221,11 +221,25 @@ int gdn_recurrence_decode(int type, const void *x, int64_t x_stride, const void 
       bad_f32_alignment({A_log, dt_bias, state, new_state, intermediate_states, slots}))
     return GDN_ERR_MISALIGNED;
   const size_t states = static_cast<size_t>(slots ? pool_slots : batch) * channels * 4;
-  const size_t inter = static_cast<size_t>(batch) * num_tokens * channels * 4;
+  const int64_t rows = batch * num_tokens;
+  const size_t inter = static_cast<size_t>(rows) * channels * 4, outs = static_cast<size_t>(rows) * channels * type_size(type);
   if ((state && state != new_state && overlap(state, states, new_state, states)) ||
       (intermediate_states && ((state && overlap(state, states, intermediate_states, inter)) ||
                                overlap(new_state, states, intermediate_states, inter))))
     return GDN_ERR_ALIASING;
+  if (overlap(out, outs, new_state, states) || (state && overlap(out, outs, state, states)) ||
+      (intermediate_states && overlap(out, outs, intermediate_states, inter)))
+    return GDN_ERR_ALIASING;
+  // `out` in the very place of an input: a lane reads what it then writes
+  const void *const inputs[3] = {x, a, b};
+  const int64_t strides[3] = {x_stride, a_stride, b_stride};
+  for (int i = 0; i < 3; ++i) {
+    const size_t bytes = static_cast<size_t>((rows - 1) * strides[i] + channels) * type_size(type);
+    const bool same = out == inputs[i] && (strides[i] == channels || rows == 1);
+    if ((!same && overlap(inputs[i], bytes, out, outs)) || overlap(inputs[i], bytes, new_state, states) ||
+        (intermediate_states && overlap(inputs[i], bytes, intermediate_states, inter)))
+      return GDN_ERR_ALIASING;
+  }
   if (int st = check_device(nullptr)) return st;
   gdn::rec::Decode p{x, a, b, x_stride, a_stride, b_stride, A_log, dt_bias, state, slots, pool_slots, batch,
                      channels, static_cast<int>(num_tokens), out, new_state, intermediate_states};

@@ -146,7 +146,8 @@ def decode_into(x, state, A_log, a, dt_bias, b, out, new_state, slots: Optional[
     `state` ([B, D], None: zeros).  With `slots` ([B] int32, distinct) both are
     one pool [P, D], updated in place; a request whose slot is outside the pool
     is skipped (device status 3).  `intermediate` [B, T, D] fp32 receives the
-    state after each token."""
+    state after each token.  `out` may be x, a or b itself, if that is
+    contiguous; no output may share memory with an input otherwise."""
     D = _check_inputs(x, a, b, A_log, dt_bias)
     B, T = x.shape[0], (x.shape[1] if x.dim() == 3 else 1)
     assert 1 <= T <= DECODE_MAX_TOKENS, f"1 <= T <= {DECODE_MAX_TOKENS}"
