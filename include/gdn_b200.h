@@ -316,8 +316,9 @@ int gdn_prefill_backward_qk4_v8_d128_k_last(
  *             [3,T,ceil(D/128)] scales
  * workspace   gdn_recurrence_workspace_bytes(T, D) bytes, 1024-byte aligned;
  *             calls that overlap in time need one each
- * One launch for up to 256 rows, else two.  Results are the same bits on
- * every run.
+ * One launch for short inputs (up to 512 rows of one sequence of 2-byte
+ * elements, less for other forms; at most 1024 sequences in cu_seqlens), else
+ * two.  Results are the same bits on every run.
  */
 size_t gdn_recurrence_workspace_bytes(int64_t total_tokens, int64_t channels);
 size_t gdn_recurrence_carry_bytes(int64_t total_tokens, int64_t channels);

@@ -35,13 +35,13 @@ def header(ws):
     return None if streams == EMPTY else (streams, group)
 
 
-def forward(gdn, args, cu):
-    """run_into; returns (out, final_state) and the header."""
+def forward(gdn, args, cu, packed=None):
+    """run_into, with 8-bit copies too; returns (out, final_state) and the header."""
     x = args[0]
     ws = gdn.recurrence.alloc_workspace(*x.shape, "cuda")
     ws.fill_(0x5a)
     out, final = torch.empty(x.shape, dtype=x.dtype, device="cuda"), torch.empty(len(cu) - 1, x.shape[1], device="cuda")
-    gdn.recurrence.run_into(*args, cu.cuda(), out, final, ws)
+    gdn.recurrence._prefill(*args, cu.cuda(), out, final, ws, packed=packed)
     return (out, final), header(ws)
 
 
@@ -64,16 +64,35 @@ def grads_of(lens, D, dtype, seed):
 # ---------------------------------------------------------------------------
 # the limit of the one launch
 # ---------------------------------------------------------------------------
-@pytest.mark.parametrize("lens,one", [([512], True), ([513], False), ([500, 12], True), ([1, 512], False),
-                                      ([64] * 8, True), ([0] * 1022 + [511, 1], True), ([0] * 1023 + [511, 1], False)],
-                         ids=lambda v: f"{sum(v)}rows{len(v)}" if isinstance(v, list) else "")
-@pytest.mark.parametrize("D", [128, 132])
-def test_one_launch_up_to_512_rows_and_1024_sequences(gdn, lens, one, D):
-    args = inputs(lens, D, BF16, sum(lens), slow=True)
-    cu = cumulative(lens)
-    got, head = forward(gdn, dev(args), cu)
-    assert (head is None) == one
-    check_forward(got, args, cu, str(lens[-3:]))
+LIMITS = [      # type, channels, 8-bit copies, chunks of one sequence, of several
+    (BF16, 128, False, 8, 7),
+    (FP16, 136, False, 8, 7),
+    (FP32, 128, False, 5, 4),
+    (BF16, 132, False, 5, 5),
+    (FP32, 130, False, 3, 3),
+    (BF16, 128, True, 3, 3),
+    (FP32, 128, True, 2, 2),
+    (FP16, 132, True, 2, 2),
+    (FP32, 130, True, 1, 1),
+]
+
+
+@pytest.mark.parametrize("dtype,D,eight,one,several", LIMITS)
+@pytest.mark.parametrize("sequences", [1, 3, 1024, 1025])
+def test_one_launch_for_short_inputs(gdn, dtype, D, eight, one, several, sequences):
+    limit = 64 * (one if sequences == 1 else several)
+    for T in (limit, limit + 1):
+        lens = [T] if sequences == 1 else [0] * (sequences - 3) + [T // 3, 0, T - T // 3]
+        args = inputs(lens, D, dtype, T, slow=True)
+        cu = cumulative(lens)
+        packed = None
+        if eight:
+            packed = torch.empty(gdn.recurrence._saved_bytes(T, D)[1], dtype=torch.uint8, device="cuda")
+        got, head = forward(gdn, dev(args), cu, packed)
+        assert (head is None) == (T == limit and sequences <= 1024), (T, head)
+        check_forward(got, args, cu, f"{dtype} {D} {T}")
+        if eight:
+            check_packed(packed, args)
 
 
 # ---------------------------------------------------------------------------
@@ -124,17 +143,17 @@ def test_types_and_widths_over_many_chunks(gdn, dtype, D, fused, eight):
     out, final = gdn.recurrence.run_autograd(*leaves, cu.cuda(), checkpoint="int8" if eight else None)
     check_forward((out.detach(), final.detach()), args, cu, f"{dtype} D={D}")
     if eight:
-        check_packed(out, args)
+        check_packed(out.grad_fn.saved_tensors[3], args)
     d_out, d_final = grads_of(lens, D, dtype, 9)
     grads = torch.autograd.grad((out, final), leaves, (d_out.cuda(), d_final.cuda()))
     check_gradients(dict(zip(NAMES, grads)), ref.backward(*args, cu.tolist(), d_out, d_final, eight), dtype,
                     f"{dtype} D={D} eight={eight}")
 
 
-def check_packed(out, args):
+def check_packed(packed, args):
     """The 8-bit x, a, b that the forward kept, bit for bit."""
-    T, D = out.shape
-    packed = out.grad_fn.saved_tensors[3].cpu()
+    T, D = args[0].shape
+    packed = packed.cpu()
     groups = -(-D // 128)
     values = packed[:3 * T * D].view(torch.int8).view(3, T, D).double()
     E = packed[3 * T * D:3 * T * (D + groups)].view(3, T, groups).int()
@@ -162,7 +181,7 @@ def test_packed_special_groups(gdn, dtype, D, T):
     p = torch.zeros(D)
     leaves = [v.cuda().requires_grad_(True) for v in (x, p, a, p.clone(), b)]
     out, _ = gdn.recurrence.run_autograd(leaves[0], None, *leaves[1:], checkpoint="int8")
-    check_packed(out, (x, None, p, a, p, b))
+    check_packed(out.grad_fn.saved_tensors[3], (x, None, p, a, p, b))
 
 
 # ---------------------------------------------------------------------------
@@ -192,7 +211,7 @@ def test_groups_of_one(gdn, dtype, D, eight):
     leaves = [t.detach().requires_grad_(True) for t in d]
     out, final = gdn.recurrence.run_autograd(*leaves, cu.cuda(), checkpoint="int8")
     assert torch.equal(out, got[0]) and torch.equal(final, got[1])
-    check_packed(out, args)
+    check_packed(out.grad_fn.saved_tensors[3], args)
     grads = torch.autograd.grad((out, final), leaves, (d_out.cuda(), d_final.cuda()))
     check_gradients(dict(zip(NAMES, grads)), ref.backward(*args, cu.tolist(), d_out, d_final, True), dtype,
                     f"{dtype} {D} 8 bits")

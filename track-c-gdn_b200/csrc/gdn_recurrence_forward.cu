@@ -630,10 +630,30 @@ recurrence_forward_kernel(const __grid_constant__ Forward p) {
 
 // ---- launch ---------------------------------------------------------------------
 // Inputs of up to this many chunks are walked by one CTA per 64 or 128 channels, in
-// one launch without a look-back.  A call alone, inputs not in L2, bf16 x 1024:
-// 269 tokens 16.4 us against 21.5 with two launches, 512 tokens 20.5 against 21.5;
-// 1024 tokens 30.7 against 23.6.
-constexpr int64_t kSerialChunks = 8;
+// one launch without a look-back.  What that costs grows with the chunks, the more
+// so where a chunk takes long; two launches take 20 to 30 us whatever they are.
+// A call alone, inputs not in L2, 1024 channels (1021 where rows are copied), us in
+// one launch and in two at the largest number of chunks that takes one, and at the
+// next:
+//                         one sequence                   four
+//   2-byte                8  20.8, 21.0                  7  21.1, 23.4  8  25.1, 21.5
+//   4-byte                5  21.1, 21.5  6  23.5, 21.4   4  21.0, 21.4  5  24.2, 23.5
+//   2-byte, row by row    5  22.1, 21.5  6  24.9, 21.5   5  22.8, 25.5  6  26.1, 25.1
+//   4-byte, row by row    3  17.9, 21.5  4  20.9, 19.4   3  19.1, 25.6  4  22.9, 23.6
+// and with 8-bit copies
+//   2-byte                3  24.3, 25.6  4  27.0, 27.0   3  27.1, 30.2  4  34.5, 25.6
+//   4-byte                2  21.1, 27.1  3  26.9, 25.5   2  23.0, 25.6  3  30.3, 30.7
+//   2-byte, row by row    2  25.0, 27.6  3  32.6, 29.2   2  26.2, 27.6  3  33.3, 35.8
+//   4-byte, directly      1  21.2, 31.7  2  33.2, 31.0   1  22.7, 31.7  2  34.2, 34.7
+// (2-byte, one sequence of 16 chunks, with both in L2: 26.7 against 17.8.)
+// From 64 to 4096 channels both sides change by at most a few us.
+template <typename E, Fetch kFetch, bool kPack>
+constexpr int64_t serial_chunks(bool one_sequence) {
+  constexpr bool kTwo = sizeof(E) == 2;
+  if (kPack) return kFetch == kTmaTile ? (kTwo ? 3 : 2) : (kTwo ? 2 : 1);
+  if (kFetch != kTmaTile) return kTwo ? 5 : 3;
+  return (kTwo ? 7 : 4) + (one_sequence ? 1 : 0);
+}
 constexpr int64_t kSerialSeqs = 1024;  // each CTA checks all of cu_seqlens then
 
 template <typename E, Fetch kFetch, bool kPack>
@@ -657,7 +677,8 @@ cudaError_t launch_forward_t(Forward p, void *workspace, int sms, cudaStream_t s
         !make_row_map<E>(&p.tb, p.b, p.D, p.s.T, p.b_stride, 64, kRows))
       return cudaErrorInvalidValue;
   }
-  const bool serial = chunks <= kSerialChunks && (p.s.cu == nullptr || p.s.N <= kSerialSeqs);
+  const bool serial =
+      chunks <= serial_chunks<E, kFetch, kPack>(p.s.N == 1) && (p.s.cu == nullptr || p.s.N <= kSerialSeqs);
   auto kernel = serial ? recurrence_forward_kernel<E, kFetch, kPack, false>
                        : recurrence_forward_kernel<E, kFetch, kPack, true>;
   static std::atomic<unsigned long long> allowed[2];
