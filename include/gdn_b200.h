@@ -383,6 +383,7 @@ int gdn_recurrence_decode(int type, const void *x, int64_t x_stride, const void 
  * one launch.  `data` is read by pack (row r at (r / inner) * outer_stride +
  * (r % inner) * inner_stride elements, its cols contiguous) and written by
  * unpack (contiguous [rows, cols]; inner and strides unused but inner >= 1).
+ * rows, cols, inner and the groups of a tensor are below 2^31 each.
  */
 #define GDN_CHECKPOINT_MAX_TENSORS 4
 typedef struct {

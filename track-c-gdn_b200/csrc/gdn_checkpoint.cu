@@ -32,6 +32,7 @@ struct Pack {
 };
 
 // A group's elements, from the start of the data (as it lies) and of the values.
+// (32-bit numbers: rows, columns and groups in all are below 2^31.)
 struct Place {
   int64_t data, values;
   int left;  // values of the row from there on

@@ -267,8 +267,7 @@ int checkpoint_call(int type, const gdn_checkpoint_tensor *tensors, int count, b
   int64_t warps = 0;
   for (int i = 0; i < count; ++i) {
     const gdn_checkpoint_tensor &t = tensors[i];
-    if (t.rows < 0 || t.cols < 0 || t.inner < 1 || t.rows > INT32_MAX || t.inner > INT32_MAX ||
-        t.cols > (int64_t{1} << 24))
+    if (t.rows < 0 || t.cols < 0 || t.inner < 1 || t.rows > INT32_MAX || t.inner > INT32_MAX || t.cols > INT32_MAX)
       return GDN_ERR_BAD_SIZE;
     if (t.rows == 0 || t.cols == 0) continue;
     if (!t.data || !t.values || !t.scales) return GDN_ERR_NULL_POINTER;
