@@ -286,8 +286,13 @@ int gdn_prefill_backward_qk4_v8_d128_k_last(
  *           token to the next, not negative (parts of one projection's output)
  * A_log, dt_bias [D] fp32
  * Pointers need the alignment of their elements; the kernels are fastest where
- * rows and pointers of the inputs are multiples of 16 bytes.  1 <= D <= 2^24,
- * T <= 2^31.
+ * rows and pointers of the inputs are multiples of 16 bytes.  Where they are
+ * not, prefill and backward fetch inputs in the aligned 16-byte blocks that
+ * hold them: up to 15 bytes before and behind a row are read, and not used,
+ * which may lie outside the caller's buffer (never on another page).
+ * 1 <= D <= 2^24, T <= 2^31, N <= 2^24.
+ * Behind an infinite state the outputs are not finite, infinite or NaN (products
+ * of gates may underflow to 0).
  */
 #define GDN_BF16 0
 #define GDN_FP16 1
@@ -305,8 +310,9 @@ int gdn_prefill_backward_qk4_v8_d128_k_last(
  *             ([N] int32 on the device, distinct) a pool [pool_slots,D] of
  *             which sequence n uses row slots[n] (outside the pool: device
  *             status 3, nothing is written)
- * out         [T,D], sharing no memory with x, a or b; final_state [N,D] fp32 (the pool with `slots`), may be
- *             `state`; an empty sequence's final state is its initial state
+ * out         [T,D], sharing no memory with x, a or b
+ * final_state [N,D] fp32 (the pool with `slots`), may be `state`; an empty
+ *             sequence's final state is its initial state
  * carries     NULL, or gdn_recurrence_carry_bytes(T, D) bytes (16-byte
  *             aligned) that receive the state before every 64th row, which
  *             the backward takes
@@ -376,8 +382,9 @@ int gdn_recurrence_decode(int type, const void *x, int64_t x_stride, const void 
  * two 2^(E-127), E in one byte: the smallest with max|v| <= 127 2^(E-127), at
  * least 1 and at most 248 (136 for fp16), beyond which values are limited to
  * 127 2^(E-127).  A value is int8 rint(v / 2^(E-127)), ties to even; the error
- * is at most half a unit, and unpacking is exact in bf16 and fp32 (in fp16
- * down to its smallest subnormal).  A group that holds a NaN or an infinity
+ * is at most half a unit (less than a whole one for values that were limited),
+ * and unpacking is exact in bf16 and fp32 (in fp16 down to its smallest
+ * subnormal).  A group that holds a NaN or an infinity
  * gets E = 255 and unpacks to NaN.
  * Each call handles up to GDN_CHECKPOINT_MAX_TENSORS tensors of one type in
  * one launch.  `data` is read by pack (row r at (r / inner) * outer_stride +

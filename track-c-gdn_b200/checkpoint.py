@@ -7,6 +7,12 @@ two 2^e with max|v| <= 127 2^e, so a value is off by at most 2^(e-1), less
 than max|v| / 126 of its group, and unpacking itself rounds nothing in bf16 and
 fp32.  A group that holds a NaN or an infinity unpacks to NaN.
 
+At the ends of a type's range e is limited.  It is at least -126: a group with
+max|v| below 2^-120 or so is off by up to 2^-127, which may be more than
+max|v| / 126.  It is at most 9 in fp16 and 121 in bf16 and fp32, so that the
+restored values are finite: beyond 127 2^e (65024 in fp16, 3.376e38) a value
+comes back as that, off by less than 2^e.
+
 `prefill.run_autograd(..., checkpoint="int8")` and
 `recurrence.run_autograd(..., checkpoint="int8")` keep their inputs this way
 between forward and backward.  No counterpart in the reference.

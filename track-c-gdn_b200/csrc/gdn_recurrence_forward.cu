@@ -97,8 +97,9 @@ struct FwdShared {
 // What bounds it: instructions, not memory.  8 x 4096 x 2048 bf16 takes 120 us
 // (4.5 TB/s; 82 us at the rate of a copy): 37 warp instructions for 32 values,
 // 2.2 a cycle of 4, the exponentials' pipe half busy.  256 sequences, 1.15 M x
-// 1024 bf16: 1.89 ms, 5.0 TB/s.  One sequence of 65536 x 1024: 171 us in bf16,
-// bound by the chain's links, 209 us in fp32 (5.1 TB/s).  With 8-bit copies 190
+// 1024 bf16: 1.90 ms, 5.0 TB/s.  One sequence of 65536 x 1024: 171 us in bf16,
+// where a copy takes 82 and 128 links in series 109 (0.85 us each, see kGroupLen);
+// 209 to 223 us in fp32 (4.9 TB/s).  With 8-bit copies 190
 // us for 8 x 4096 x 2048 (3.9 TB/s), bound by integer work on groups and bytes.
 // Rows that no tensor copy fits, 47000 x 1021 fp16: 191 us, 2.0 TB/s, bound by
 // instructions (two 16-bit accesses for each pair of values, copies by address).

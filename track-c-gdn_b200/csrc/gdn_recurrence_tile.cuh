@@ -14,9 +14,10 @@ namespace gdn {
 namespace rec {
 
 // Chunks joined through one published state: 8 where one sequence (or a few) has
-// to be worked on by all CTAs at once -- a state then travels one link of about
-// 0.75 us for 8 chunks (65536 x 1024 bf16: 171 us; groups of 4: 218, of 16: 317,
-// with more maps to fetch and apply for each tile) -- and 1 where streams and
+// to be worked on by all CTAs at once -- a state then travels one link for 8
+// chunks (65536 x 1024 bf16: 171 us with 128 links; groups of 4: 218 us, 0.85 for
+// each of 256; of 16: 317 us, with more maps to fetch and apply for each tile) --
+// and 1 where streams and
 // tiles of channels together give most CTAs a tile of a chunk whose predecessor
 // is done: then a state per chunk is all that is published.
 constexpr int kGroupLen = 8;
@@ -306,8 +307,9 @@ __device__ __forceinline__ bool last_bits(const uint32_t (&words)[2], int row) {
 // ---- how inputs reach shared memory ------------------------------------------------
 // kTmaTile: one tensor copy a plane, rows of 64 channels side by side.  It wants
 // 16-byte rows.  kRowCopies: asynchronous copies of the 16-byte blocks that hold
-// a row's 64 channels (blocks never leave the pages of the data that they hold);
-// the row then starts up to 15 bytes into its place.  A bulk copy a row instead
+// a row's 64 channels (blocks never leave the pages of the data that they hold,
+// but hold up to 15 bytes before and behind it, perhaps of another buffer); the
+// row then starts up to 15 bytes into its place.  A bulk copy a row instead
 // took 49 cycles a row and was slower than loads without any stage (494 against
 // 328 us, 47000 x 1021 fp16).  kDirect: none; the consumers load from global
 // memory (4-byte types that are packed as well, whose rows with gaps do not fit).

@@ -12,7 +12,8 @@ packed ([T, D] with `cu_seqlens` [N+1] int64) or dense ([N, S, D] without).
 The channels of a token must lie next to one another; tokens may be apart, so
 x, a and b may be slices of one projection's output (any other layout is
 copied first).  Everything is computed and carried in fp32, and a result is
-rounded once, when it is stored.
+rounded once, when it is stored.  Behind an infinite state the outputs are not
+finite, infinite or NaN (products of gates may underflow to 0).
 
 Nothing here synchronises the host.  cu_seqlens and slots are checked on the
 device: bad values are reported by `_native.read_device_status` (1 and 3) and
@@ -388,7 +389,7 @@ def _saved_bytes(total_tokens: int, channels: int):
 
 class _RecurrenceFunction(torch.autograd.Function):
     """run(...) with gradients.  The forward keeps the state before every 64th
-    row (1/16 of x's bytes for a 2-byte type), and x, a, b themselves or their
+    row (1/32 of x's bytes for a 2-byte type), and x, a, b themselves or their
     8-bit form."""
 
     @staticmethod
