@@ -322,6 +322,7 @@ int gdn_prefill_backward_qk4_v8_d128_k_last(
  *             [3,T,ceil(D/128)] scales
  * workspace   gdn_recurrence_workspace_bytes(T, D) bytes, 1024-byte aligned;
  *             calls that overlap in time need one each
+ * No output shares memory with another or with the workspace.
  * One launch for short inputs (up to 512 rows of one sequence of 2-byte
  * elements, less for other forms; at most 1024 sequences in cu_seqlens), else
  * two.  Results are the same bits on every run.
@@ -349,6 +350,7 @@ int gdn_recurrence_prefill(int type, const void *x, int64_t x_stride, const void
  *             values, the states before the tokens restarted from `carries`
  *             (required) at every 64th row
  * workspace   gdn_recurrence_backward_workspace_bytes(T, D) bytes
+ * No output shares memory with another, with the workspace, or with an input.
  * Deterministic.  No host synchronisation.
  */
 size_t gdn_recurrence_backward_workspace_bytes(int64_t total_tokens, int64_t channels);

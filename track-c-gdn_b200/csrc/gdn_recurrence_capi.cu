@@ -49,6 +49,25 @@ bool rows_overlap(const void *p, int64_t stride, const void *q, int type, int64_
   return p && q && T > 0 && overlap(p, ((T - 1) * stride + D) * e, q, static_cast<size_t>(T) * D * e);
 }
 
+// Memory that a call writes to or reads; nothing where the pointer is NULL.
+struct Region {
+  const void *p;
+  size_t bytes;
+};
+bool meet(const Region &a, const Region &b) {
+  return a.p && b.p && a.bytes && b.bytes && overlap(a.p, a.bytes, b.p, b.bytes);
+}
+// Whether an output shares memory with an input or with another output.
+bool outputs_meet(std::initializer_list<Region> outs, std::initializer_list<Region> ins) {
+  for (const Region *a = outs.begin(); a != outs.end(); ++a) {
+    for (const Region &b : ins)
+      if (meet(*a, b)) return true;
+    for (const Region *b = outs.begin(); b != a; ++b)
+      if (meet(*a, *b)) return true;
+  }
+  return false;
+}
+
 gdn::rec::Seqs sequences(const int64_t *cu, int64_t N, int64_t T, const int32_t *slots, int64_t pool) {
   return gdn::rec::Seqs{cu, N, T, N > 0 ? T / N : 0, slots, pool};
 }
@@ -116,6 +135,15 @@ int gdn_recurrence_prefill(int type, const void *x, int64_t x_stride, const void
       rows_overlap(a, a_stride, out, type, total_tokens, channels) ||
       rows_overlap(b, b_stride, out, type, total_tokens, channels))
     return GDN_ERR_ALIASING;
+  const size_t outs = static_cast<size_t>(total_tokens) * channels * type_size(type);
+  if (outputs_meet({{out, outs},
+                    {final_state, states},
+                    {carries, gdn_recurrence_carry_bytes(total_tokens, channels)},
+                    {packed, gdn_recurrence_packed_bytes(total_tokens, channels)},
+                    {workspace, gdn_recurrence_workspace_bytes(total_tokens, channels)}},
+                   {}) ||
+      (state != final_state && meet({state, states}, {out, outs})))
+    return GDN_ERR_ALIASING;
   int sms = 0;
   if (int st = check_device(&sms)) return st;
   gdn::rec::Forward p{};
@@ -162,6 +190,17 @@ int gdn_recurrence_backward(int type, const void *x, int64_t x_stride, const voi
                     rows_overlap(b, b_stride, g, type, total_tokens, channels)))
       return GDN_ERR_ALIASING;
   }
+  const size_t rows = static_cast<size_t>(total_tokens) * channels * type_size(type);
+  if (outputs_meet({{dx, rows},
+                    {da, rows},
+                    {db, rows},
+                    {d_state, states},
+                    {workspace, gdn_recurrence_backward_workspace_bytes(total_tokens, channels)}},
+                   {{state, states},
+                    {d_final_state, states},
+                    {carries, gdn_recurrence_carry_bytes(total_tokens, channels)},
+                    {packed, gdn_recurrence_packed_bytes(total_tokens, channels)}}))
+    return GDN_ERR_ALIASING;
   int sms = 0;
   if (int st = check_device(&sms)) return st;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
