@@ -7,6 +7,7 @@
 // synchronises the host.
 #include <cuda_runtime.h>
 
+#include <atomic>
 #include <cstdint>
 #include <cstdio>
 
@@ -60,27 +61,27 @@ bool overlap(const void *a, size_t na, const void *b, size_t nb) {
   return x < y + nb && y < x + na;
 }
 
-// Current device must be sm_100 (B200 family); cached per device ordinal.  Makes
+// Current device must be sm_100 (B200 family); cached per device ordinal, in one
+// word for calls from several threads at once (autograd has one a device).  Makes
 // its primary context current for a calling thread that has none: a thread that
 // has not used CUDA yet (autograd's, for one), where tensor maps cannot be
 // encoded.  A caller's own context stays current: its streams and memory are
 // valid there alone.
 int check_device(int *num_sms) {
-  static int cached_dev = -1, cached_ok = 0, cached_sms = 0;
+  static std::atomic<int> known[64];  // 0: not asked yet; else SMs << 1, and 1 where it is sm_100
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess) return GDN_ERR_DEVICE;
   if (gdn::current_context() == nullptr && cudaSetDevice(dev) != cudaSuccess) return GDN_ERR_DEVICE;
-  if (dev != cached_dev) {
+  int facts = dev < 64 ? known[dev].load(std::memory_order_relaxed) : 0;
+  if (facts == 0) {
     cudaDeviceProp prop;
     if (cudaGetDeviceProperties(&prop, dev) != cudaSuccess) return GDN_ERR_DEVICE;
-    cached_ok = prop.major == 10 && prop.minor == 0;
-    cached_sms = prop.multiProcessorCount;
-    cached_dev = dev;
+    facts = prop.multiProcessorCount << 1 | (prop.major == 10 && prop.minor == 0);
+    if (dev < 64) known[dev].store(facts, std::memory_order_relaxed);
   }
-  if (num_sms) *num_sms = cached_sms;
-  return cached_ok ? GDN_OK : GDN_ERR_DEVICE;
+  if (num_sms) *num_sms = facts >> 1;
+  return facts & 1 ? GDN_OK : GDN_ERR_DEVICE;
 }
-
 
 // Argument checks of the dense prefill entry points, then the launches.
 int prefill_checked(const void *q, const void *k, const void *v, const float *state,
