@@ -156,6 +156,7 @@ recurrence_backward_kernel(const __grid_constant__ Backward p) {
         }
       }
       const int64_t c0 = static_cast<int64_t>(d) * 64, base = chunk * kRows;
+      GDN_DCHECK(chunk < 0 || (d >= 0 && d < nt && base < max(p.s.T, int64_t{1})));
       const int left = static_cast<int>(min(p.D - c0, int64_t{64}));
       if (chunk >= 0 && p.zero_behind && !only_map) {
         for (int64_t t = max(base, total); t < min(base + kRows, p.s.T); ++t) {
@@ -255,6 +256,9 @@ recurrence_backward_kernel(const __grid_constant__ Backward p) {
       const bool from_state = tab.ahead > place;  // the sequence goes on beyond the group
       const int before = from_state ? place : static_cast<int>(tab.ahead);
       const bool looks = enters && !tab.only_map, groups = group_len > 1;
+      // the words that are looked at are those of chunks behind this one
+      GDN_DCHECK(!looks || (before >= 0 && before < kGroupLen && (from_state || before >= 1) && chunk + before <= last &&
+                            (!from_state || (group_len == 1 ? chunk + 1 : (chunk / kGroupLen + 1) * kGroupLen) <= last)));
       Words2 w[kGroupLen];
       auto src = [&](int j) {
         return j > 0 ? p.maps + (chunk + before - j + 1) * row_ch + lane_ch : states + (group + 1) * row_ch + lane_ch;
@@ -339,11 +343,13 @@ recurrence_backward_kernel(const __grid_constant__ Backward p) {
     }
   };
   auto initial = [&](const Table<kRows> &tab, int64_t c0, int i) {  // the state before a first token
+    GDN_DCHECK(tab.start[row0 + i] >= 0 && tab.start[row0 + i] < p.s.N);
     return p.state != nullptr ? load2_f32<kVec>(p.state + tab.start[row0 + i] * p.D + c0, lane,
                                                 static_cast<int>(min(p.D - c0, int64_t{64})))
                               : 0;
   };
   auto final = [&](const Table<kRows> &tab, int64_t c0, int i) {  // R behind a last token
+    GDN_DCHECK(tab.end[row0 + i] >= 0 && tab.end[row0 + i] < p.s.N);
     return p.d_final != nullptr ? load2_f32<kVec>(p.d_final + tab.end[row0 + i] * p.D + c0, lane,
                                                   static_cast<int>(min(p.D - c0, int64_t{64})))
                                 : 0;
@@ -463,6 +469,7 @@ recurrence_backward_kernel(const __grid_constant__ Backward p) {
               if (i >= valid) continue;
               if ((ends >> i) & 1) R = final(tab, c0, i);
             }
+            GDN_DCHECK(tab.chunk * kRows + row0 + i < total && (!edge || i < valid));
             const uint64_t dh = f2_add(o[j], R);
             R = f2_mul(g[j], dh);
             const uint64_t da = f2_mul(ca[j], dh);

@@ -184,6 +184,7 @@ recurrence_forward_kernel(const __grid_constant__ Forward p) {
         if (next * kRows < max(p.s.T, int64_t{1})) chunk = next++;
       }
       const int64_t c0 = static_cast<int64_t>(d) * kCh, base = chunk * kRows;
+      GDN_DCHECK(chunk < 0 || (d >= 0 && d < nt && base < max(p.s.T, int64_t{1})));
       if (chunk >= 0 && p.zero_behind && !only_map) {
         for (int64_t t = max(base, total); t < min(base + kRows, p.s.T); ++t)
 #pragma unroll
@@ -301,6 +302,9 @@ recurrence_forward_kernel(const __grid_constant__ Forward p) {
       // of the chunks before, and the state that enters the first of them
       const bool looks = kChain && enters && !only_map;
       const bool groups = kChain && group_len > 1;
+      // the words that are looked at are those of chunks before this one
+      GDN_DCHECK(!looks || tab.valid <= 0 ||
+                 (before >= 0 && before < kGroupLen && (from_state ? group >= 1 : before >= 1) && chunk - before >= 0));
       Words2 w[kGroupLen];
       auto src = [&](int j) {
         return j > 0 ? p.maps + (chunk - before + j - 1) * row_ch + lane_ch : states + (group - 1) * row_ch + lane_ch;
@@ -400,6 +404,7 @@ recurrence_forward_kernel(const __grid_constant__ Forward p) {
     };
     const Tile before = sh.tiles[s1];
     E *out = static_cast<E *>(p.out) + before.at + row0 * p.D + 64 * half;
+    GDN_DCHECK(!before.plain || (before.at >= 0 && before.at + (kRows - 1) * p.D + kCh <= total * p.D));
     if (before.plain) {
 #pragma unroll
       for (int i = 0; i < kTokW; ++i) {
@@ -418,6 +423,8 @@ recurrence_forward_kernel(const __grid_constant__ Forward p) {
       for (int i = 0; i < kTokW; ++i) {
         const ulonglong2 v = kept(i);
         const uint64_t r = i < first ? f2_fma(v.y, h, v.x) : v.x;
+        GDN_DCHECK(i >= valid || (tab.chunk * kRows + row0 + i < total && c0 < p.D + 64));
+        GDN_DCHECK(!((ends >> i) & 1) || (i < valid && tab.end[row0 + i] >= 0 && tab.end[row0 + i] < p.s.N));
         if (p.out != nullptr && i < valid) store2<E, kVec>(out + i * p.D, lane, left, r);
         if (((ends >> i) & 1) && p.final != nullptr)
           store2_f32<kVec>(p.final + p.s.row(tab.end[row0 + i]) * p.D + c0, lane, left, r);
@@ -503,6 +510,7 @@ recurrence_forward_kernel(const __grid_constant__ Forward p) {
         const uint32_t ex =
             group_exponent(Raw2<E>::magnitude(max(mine, amax[32 * (half ^ 1) + lane])), exp_cap<E>());
         const int64_t t0 = tab.chunk * kRows + row0;
+        GDN_DCHECK(t0 + valid <= p.s.T || valid == 0);
         const int left = static_cast<int>(min(p.D - c0, int64_t{64}));
         if (half == 0 && lane < 3 * kTokW && lane % kTokW < valid)
           p.packed[3 * p.s.T * p.D + (lane / kTokW * p.s.T + t0 + lane % kTokW) * nt + tile.d] =
@@ -576,6 +584,7 @@ recurrence_forward_kernel(const __grid_constant__ Forward p) {
           gate_pair(r[0].pair(), r[1].pair(), r[2].pair(), par.dt, par.c, g, u);
           if (i >= valid) g = f2_dup(1.f), u = 0;
           if ((starts >> i) & 1) {  // y is the state itself from here on
+            GDN_DCHECK(tab.start[row0 + i] >= 0 && tab.start[row0 + i] < p.s.N && tab.cut < kStreams);
             const int left = static_cast<int>(min(p.D - c0, int64_t{64}));
             const int row = row0 + i;
             // of a cut chunk the last sequence's was set aside if it goes on

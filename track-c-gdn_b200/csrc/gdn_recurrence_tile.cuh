@@ -55,7 +55,10 @@ struct Seqs {
   const int32_t *slots;  // state row of a sequence, or null: its number
   int64_t pool;
   __device__ __forceinline__ int64_t at(int64_t n) const { return cu != nullptr ? cu[n] : n * S; }
-  __device__ __forceinline__ int64_t row(int64_t n) const { return slots != nullptr ? slots[n] : n; }
+  __device__ __forceinline__ int64_t row(int64_t n) const {
+    GDN_DCHECK(n >= 0 && n < N);
+    return slots != nullptr ? slots[n] : n;
+  }
   __device__ __forceinline__ int64_t total() const { return cu != nullptr ? cu[N] : T; }
 };
 
@@ -244,6 +247,7 @@ template <int kRows, typename F>
 __device__ __forceinline__ bool fill_table(const Seqs &s, Table<kRows> &t, int64_t base, bool last, int lane,
                                            const int *first, F on_empty) {
   const int64_t lo = first != nullptr ? first[base / kRows] : first_at_or_after(s, base, lane);
+  GDN_DCHECK(base >= 0 && base < max(s.T, int64_t{1}) && lo >= 0 && lo <= s.N);
   // the sequence that covers the first row, if it does not start there
   if (lane == 0) t.reach = lo > 0 ? base / kRows - s.at(lo - 1) / kRows : 0;
   const int64_t next = lo < s.N ? s.at(lo) : s.total();
@@ -257,6 +261,7 @@ __device__ __forceinline__ bool fill_table(const Seqs &s, Table<kRows> &t, int64
   const int64_t hi = last               ? s.N
                      : first != nullptr ? first[base / kRows + 1]
                                         : first_at_or_after(s, base + kRows, lane);
+  GDN_DCHECK(hi >= lo && hi <= s.N && (last || hi < s.N || s.total() >= base + kRows));
   if (lane == 0) t.ahead = last ? 0 : (s.at(hi) - 1) / kRows - base / kRows;
   __syncwarp();
   for (int64_t n0 = max(lo - 1, int64_t{0}); n0 < hi; n0 += 32) {
